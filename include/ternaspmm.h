@@ -687,6 +687,54 @@ int ternaspmm_probe_decode_step(const ternaspmm_step_desc* desc, const ternaspmm
                                 terna_stream stream);
 int ternaspmm_probe_barrier(void* state, int workgroups, int rounds, unsigned first_tag, terna_stream stream);
 
+/* ---- Long contexts: rotary positions, a cache in 4 bits, log probabilities (no counterpart in the reference) ----------------
+ * Each entry point returns 0, or -1 with nothing enqueued where it does not take its arguments.  All only enqueue and are safe under capture; scratch
+ * memory is the caller's, needs no initialisation, and must not be shared by calls that overlap.
+ *
+ * ternaspmm_rotary: rotary positions on rows of heads.  x [B][T][H][D] (fp32 or, with fp32 == 0, bf16), strides of its first three dimensions in
+ * elements, the last contiguous; out likewise, or x itself with x's strides; no other overlap.  pos int64 [T] ([B][T] with per_sequence); frequency
+ * float64 [pairs], radians a position.  Pair j = dimensions (2j, 2j + 1) when adjacent, else (j, j + pairs); (a, b) becomes
+ * (a cos - b sin, b cos + a sin), cos and sin of pos * frequency[j] (formed in 64 bits) times amplitude.  Dimensions from 2 * pairs on are copied.
+ * 2 * pairs <= D <= 1024, H <= 65535. */
+int ternaspmm_rotary(const void* x, const long long* x_strides, void* out, const long long* out_strides, int fp32, const long long* pos, int per_sequence,
+                     const double* frequency, int pairs, double amplitude, int B, int T, int H, int D, int adjacent, terna_stream stream);
+
+/* A key/value cache in 4 bits: codes [B][KV][S][D / 2] and scale bytes [B][KV][S][D / 32].  A code is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign, the
+ * even dimension in the lower half of a byte) and stands for code * 2^(byte - 127) of its 32 dimensions' scale byte: the smallest exponent e in
+ * -125 .. 125 with max |x| <= 7 * 2^e, codes rounded to nearest (ties to even) and held to 6; byte 255 -- one of the 32 was NaN or infinite -- stands
+ * for NaN.  Codes 16-byte aligned; D 64 or 128; S <= 2^25. */
+typedef struct ternaspmm_kv4 {
+    uint8_t *k, *k_scale, *v, *v_scale;
+} ternaspmm_kv4;
+
+/* New rows: qkv bf16 rows b * T + t of `row` elements (H query, KV key, KV value heads) -> q_out bf16 [B][H][T][D], turned as ternaspmm_rotary does, and
+ * slot pos of the cache (keys turned, in fp32, unrounded before they are quantised).  A position outside [0, S) stores nothing.  The positions of one
+ * sequence have to differ: of two rows for one slot the codes and scales that stay may be of either. */
+int ternaspmm_kv4_store(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
+                        terna_bf16* q_out, const ternaspmm_kv4* cache, int B, int T, int H, int KV, int D, int S, int adjacent, terna_stream stream);
+/* Slots pos of the cache as bf16 [B][T][KV][D] (their values are bf16 numbers); a row of NaN for a position outside [0, S). */
+int ternaspmm_kv4_rows(const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* k_out, terna_bf16* v_out, int B, int T, int KV, int D, int S,
+                       terna_stream stream);
+/* Attention over the cache: out bf16 [B * T][H * D], row (b, t) = softmax over the slots 0 .. pos of scale * q . k, times the values; q bf16
+ * [B][H][T][D].  A negative position sees nothing: zeros.  One from S on: NaN.  Slots that a row does not see do not reach it, whatever they hold.
+ * workspace: ternaspmm_kv4_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for long caches of few rows.
+ * ternaspmm_kv4_splits: the number of parts a row's slots are read in. */
+int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S);
+long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S);
+int ternaspmm_kv4_attention(const terna_bf16* q, const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* out, void* workspace, int B, int T, int H,
+                            int KV, int D, int S, float scale, terna_stream stream);
+/* One new token per sequence: ternaspmm_kv4_store and ternaspmm_kv4_attention in one launch (two with splits), their bits; T = 1. */
+int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
+                       const ternaspmm_kv4* cache, terna_bf16* out, void* workspace, int B, int H, int KV, int D, int S, float scale, int adjacent, terna_stream stream);
+
+/* Of M rows of V logits (bf16, or fp32; `row` elements apart): logprob fp32 [M] of targets int64 [M] (NaN for one outside [0, V); both may be NULL),
+ * entropy fp32 [M] in nats, and the `top` (0 .. 64, at most V) largest: ids int64 [M][top], by value, equal values by lower index, NaN last, with
+ * their log probabilities.  A row with NaN or +inf, or of -inf alone, has no distribution: its probabilities and entropy are NaN.
+ * workspace: ternaspmm_token_logprobs_workspace_bytes, 8-byte aligned; NULL: slower for few rows. */
+long long ternaspmm_token_logprobs_workspace_bytes(int M, int V, int top);
+int ternaspmm_token_logprobs(const void* logits, long long row, int fp32, const long long* targets, float* logprob, float* entropy, long long* top_ids,
+                             float* top_logprobs, int top, void* workspace, int M, int V, terna_stream stream);
+
 /* Library version string, e.g. "ternaspmm-gfx950 0.1". */
 const char* ternaspmm_version(void);
 

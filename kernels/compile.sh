@@ -37,6 +37,10 @@ compile launch_step_ordered.hip launch_step_ordered.o -mllvm -disable-machine-li
 # accumulators of the prompt-pass attention in ordinary vector registers (they are rescaled between matrix instructions)
 compile abi_prefill_attention.hip abi_prefill_attention.o -mllvm -amdgpu-mfma-vgpr-form
 compile abi_head.hip abi_head.o
+compile abi_rotary.hip abi_rotary.o
+# (the output accumulators are rescaled between matrix instructions here too)
+compile abi_kv4.hip abi_kv4.o -mllvm -amdgpu-mfma-vgpr-form
+compile abi_logprobs.hip abi_logprobs.o
 compile abi_probe.hip abi_probe.o
 compile format_host.cpp format_host.o
 # The host path of the Python package: a CPython module on torch's C++ headers, bound to the library at run time.  The library

@@ -7,5 +7,7 @@ from .convert_utils import (  # noqa: F401
 from .linear import (  # noqa: F401
     BF16BitLinear, SpBitLinear, argmax_rows, greedy_step, greedy_step_state, lm_head, SpBitLinearBF16, TernaInfer_linear, TernaInfer_linear_bf16,
     TernaInfer_linear_packed, fused_linear, get_global_workspace, interleave_gate_up, row_stats, relu2_mul_rmsnorm_linear_packed, relu2_mul_rmsnorm_quant, repack_weight, rmsnorm_linear_packed, rmsnorm_quant)
+from .long_context import (  # noqa: F401
+    Kv4Cache, TokenLogprobs, kv4_attention, kv4_rows, kv4_step, kv4_store, rotary_embed, rotary_frequencies, token_logprobs)
 
 __version__ = "0.1"

@@ -103,6 +103,15 @@ PROTOTYPES = {
     "ternaspmm_prompt_inputs": ([_vp, _vp, _ci, _vp, _ci, _ci, _vp, _ci, _ci, _vp, _vp, _ci, _vp], _ci),
     "ternaspmm_decode_step_bytes": ([_vp], ctypes.c_longlong),
     "ternaspmm_decode_step": ([_vp] * 9, _ci),
+    "ternaspmm_rotary": ([_vp] * 4 + [_ci, _vp, _ci, _vp, _ci, ctypes.c_double] + [_ci] * 5 + [_vp], _ci),
+    "ternaspmm_kv4_store": ([_vp, ctypes.c_longlong, _vp, _ci, _vp, _ci, ctypes.c_double, _vp, _vp] + [_ci] * 7 + [_vp], _ci),
+    "ternaspmm_kv4_rows": ([_vp, _vp, _ci, _vp, _vp] + [_ci] * 5 + [_vp], _ci),
+    "ternaspmm_kv4_splits": ([_ci] * 6, _ci),
+    "ternaspmm_kv4_workspace_bytes": ([_ci] * 6, ctypes.c_longlong),
+    "ternaspmm_kv4_attention": ([_vp, _vp, _vp, _ci, _vp, _vp] + [_ci] * 6 + [ctypes.c_float, _vp], _ci),
+    "ternaspmm_kv4_step": ([_vp, ctypes.c_longlong, _vp, _ci, _vp, _ci, ctypes.c_double, _vp, _vp, _vp] + [_ci] * 5 + [ctypes.c_float, _ci, _vp], _ci),
+    "ternaspmm_token_logprobs_workspace_bytes": ([_ci] * 3, ctypes.c_longlong),
+    "ternaspmm_token_logprobs": ([_vp, ctypes.c_longlong, _ci] + [_vp] * 5 + [_ci, _vp, _ci, _ci, _vp], _ci),
     "ternaspmm_version": ([], ctypes.c_char_p),
 }
 

@@ -1,0 +1,133 @@
+// C ABI of the 4-bit key/value cache: store, rows of it, attention of few query rows, the single-token step (kv4_*_kernel.h).
+// Declarations: include/ternaspmm.h.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdio>
+#include <cstdlib>
+
+#include "../../include/ternaspmm.h"
+#include "host_util.h"
+#include "kv4_attention_kernel.h"
+
+using namespace terna;
+
+namespace {
+
+constexpr int kMaxSplits = 128;
+
+bool kv4_shape_ok(int B, int T, int H, int KV, int D, int S)
+{
+    return B >= 1 && T >= 1 && H >= 1 && KV >= 1 && H % KV == 0 && (D == 64 || D == 128) && S >= 1 && S <= 1 << 25 && H <= 4096 &&
+           static_cast<long long>(B) * T <= 1 << 24 && static_cast<long long>(B) * T * H <= 1 << 28;
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool kv4_cache_ok(const ternaspmm_kv4* c) { return c && c->k && c->k_scale && c->v && c->v_scale && aligned16(c->k) && aligned16(c->v); }
+
+// Workgroups of the attention: sixteen rows of a kv head and a split each.
+long long kv4_workgroups(int B, int T, int H, int KV) { return static_cast<long long>(B) * KV * ((static_cast<long long>(T) * (H / KV) + 15) / 16); }
+
+template <bool STEP>
+int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, hipStream_t st)
+{
+    const int rows = a.T * (a.H / a.KV);
+    a.tiles = (rows + 15) / 16;
+    const long long groups = static_cast<long long>(a.B) * a.KV * a.splits, grid = (groups + 7) / 8 * 8 * a.tiles;
+    if (grid >= 1ll << 31) return -1;
+    auto kernel = D == 128 ? terna_kv4_attention_kernel<128, STEP, true> : terna_kv4_attention_kernel<64, STEP, true>;
+    if constexpr (STEP) {
+        if (!adjacent) kernel = D == 128 ? terna_kv4_attention_kernel<128, true, false> : terna_kv4_attention_kernel<64, true, false>;
+    }
+    launch(kernel, dim3(grid), dim3(64 * kKv4Waves), 0, st, a);
+    if (a.splits > 1)
+        launch(D == 128 ? terna_kv4_merge_kernel<128> : terna_kv4_merge_kernel<64>, dim3(a.B * a.T * a.H), dim3(D), 0, st, a.partial, a.pos, a.out, a.T, a.H, a.splits,
+               a.per_seq);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) die(who, e, __LINE__);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S)
+{
+    if (!kv4_shape_ok(B, T, H, KV, D, S)) return -1;
+    // as many as give the 256 CUs two workgroups each, while each keeps a step for every wave
+    const long long wgs = kv4_workgroups(B, T, H, KV);
+    const int most = (S + kKv4Step * kKv4Waves - 1) / (kKv4Step * kKv4Waves);
+    long long splits = 512 / wgs;
+    splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+    return static_cast<int>(splits < most ? splits : most);
+}
+
+long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S)
+{
+    const int splits = ternaspmm_kv4_splits(B, T, H, KV, D, S);
+    return splits < 0 ? -1 : splits == 1 ? 0 : 4ll * B * T * H * splits * (D + 2);
+}
+
+int ternaspmm_kv4_store(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
+                        terna_bf16* q_out, const ternaspmm_kv4* cache, int B, int T, int H, int KV, int D, int S, int adjacent, terna_stream stream)
+{
+    if (!kv4_shape_ok(B, T, H, KV, D, S) || !kv4_cache_ok(cache) || !qkv || !pos || !frequency || !q_out || pairs < 1 || 2 * pairs > D || row < (H + 2ll * KV) * D || (row & 7) ||
+        !aligned16(qkv) || !aligned16(q_out) || KV > 4096)
+        return -1;
+    RotaryShape s{T, H, D, pairs, per_sequence != 0, B * T, 1, amplitude};
+    const int steps = (H + 2 * KV) * (D / 8);
+    while (2 * s.tokens_a_group * pairs <= kRotaryMaxAngles && s.tokens_a_group * steps < 4 * kRotaryThreads && s.tokens / (2 * s.tokens_a_group) >= 512 &&
+           (T == 1 || 2 * s.tokens_a_group <= T))
+        s.tokens_a_group *= 2;
+    const int groups = (s.tokens + s.tokens_a_group - 1) / s.tokens_a_group;
+    int slices = 1;
+    while (slices < 64 && groups * slices < 512 && 2 * slices * kRotaryThreads <= s.tokens_a_group * steps) slices *= 2;
+    auto kernel = D == 128 ? (adjacent ? terna_kv4_store_kernel<128, true> : terna_kv4_store_kernel<128, false>)
+                           : (adjacent ? terna_kv4_store_kernel<64, true> : terna_kv4_store_kernel<64, false>);
+    launch(kernel, dim3(groups, slices), dim3(kRotaryThreads), 0, static_cast<hipStream_t>(stream), qkv, pos, frequency, q_out, cache->k, cache->k_scale, cache->v,
+           cache->v_scale, s, KV, S, row);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) die("ternaspmm_kv4_store", e, __LINE__);
+    return 0;
+}
+
+int ternaspmm_kv4_rows(const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* k_out, terna_bf16* v_out, int B, int T, int KV, int D, int S,
+                       terna_stream stream)
+{
+    if (!kv4_shape_ok(B, T, KV, KV, D, S) || !kv4_cache_ok(cache) || !pos || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) return -1;
+    const long long groups = static_cast<long long>(B) * T * KV * (D / kKv4Group);
+    launch(terna_kv4_rows_kernel, dim3(static_cast<unsigned>((2 * groups + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), cache->k, cache->k_scale, cache->v,
+           cache->v_scale, pos, k_out, v_out, T, KV, S, D, per_sequence != 0, groups);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) die("ternaspmm_kv4_rows", e, __LINE__);
+    return 0;
+}
+
+int ternaspmm_kv4_attention(const terna_bf16* q, const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* out, void* workspace, int B, int T, int H,
+                            int KV, int D, int S, float scale, terna_stream stream)
+{
+    if (!kv4_shape_ok(B, T, H, KV, D, S) || !kv4_cache_ok(cache) || !q || !pos || !out || !aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
+    Kv4Attention a{};
+    a.splits = workspace ? ternaspmm_kv4_splits(B, T, H, KV, D, S) : 1;
+    a.q = q, a.k = cache->k, a.k_scale = cache->k_scale, a.v = cache->v, a.v_scale = cache->v_scale, a.pos = pos, a.out = out, a.partial = static_cast<float*>(workspace);
+    a.B = B, a.T = T, a.H = H, a.KV = KV, a.S = S, a.per_seq = per_sequence != 0;
+    a.scale = scale * static_cast<float>(M_LOG2E);
+    return launch_kv4_attention<false>("ternaspmm_kv4_attention", a, D, 1, static_cast<hipStream_t>(stream));
+}
+
+int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
+                       const ternaspmm_kv4* cache, terna_bf16* out, void* workspace, int B, int H, int KV, int D, int S, float scale, int adjacent, terna_stream stream)
+{
+    if (!kv4_shape_ok(B, 1, H, KV, D, S) || !kv4_cache_ok(cache) || !qkv || !pos || !frequency || !out || pairs < 1 || 2 * pairs > D || row < (H + 2ll * KV) * D || (row & 7) ||
+        !aligned16(qkv) || !aligned16(out) || !aligned16(workspace))
+        return -1;
+    Kv4Attention a{};
+    a.splits = workspace ? ternaspmm_kv4_splits(B, 1, H, KV, D, S) : 1;
+    a.q = qkv, a.k = cache->k, a.k_scale = cache->k_scale, a.v = cache->v, a.v_scale = cache->v_scale, a.pos = pos, a.out = out, a.partial = static_cast<float*>(workspace);
+    a.frequency = frequency, a.amplitude = amplitude, a.row = row, a.pairs = pairs;
+    a.B = B, a.T = 1, a.H = H, a.KV = KV, a.S = S, a.per_seq = per_sequence != 0;
+    a.scale = scale * static_cast<float>(M_LOG2E);
+    return launch_kv4_attention<true>("ternaspmm_kv4_step", a, D, adjacent, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

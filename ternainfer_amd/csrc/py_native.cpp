@@ -12,12 +12,15 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <ATen/EmptyTensor.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <array>
 #include <cstdarg>
+#include <optional>
 #include <vector>
 
 #include "../../include/ternaspmm.h"
@@ -60,7 +63,15 @@ namespace {
     X(ternaspmm_step_inputs)                                                                                           \
     X(ternaspmm_prompt_inputs)                                                                                         \
     X(ternaspmm_decode_step_bytes)                                                                                     \
-    X(ternaspmm_decode_step)
+    X(ternaspmm_decode_step)                                                                                           \
+    X(ternaspmm_rotary)                                                                                                \
+    X(ternaspmm_kv4_store)                                                                                             \
+    X(ternaspmm_kv4_rows)                                                                                              \
+    X(ternaspmm_kv4_workspace_bytes)                                                                                   \
+    X(ternaspmm_kv4_attention)                                                                                         \
+    X(ternaspmm_kv4_step)                                                                                              \
+    X(ternaspmm_token_logprobs_workspace_bytes)                                                                        \
+    X(ternaspmm_token_logprobs)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     TERNA_ENTRY_POINTS(X)
@@ -887,6 +898,297 @@ TERNA_FUNCTION(decode_step, 10)
     return wrap(std::move(x), unlocked);
 }
 
+// ---- long contexts: rotary positions, the 4-bit cache, log probabilities.  These take tensors of any device: the current one is changed for the call.
+using Guard = std::optional<c10::DeviceGuard>;
+void on_device_of(Guard& guard, const at::Tensor& x)
+{
+    if (x.device().index() != c10::hip::current_device()) guard.emplace(x.device());
+}
+void check_device(const char* who, const char* name, const at::Tensor& t, const at::Tensor& with)
+{
+    if (!t.is_cuda() || t.device() != with.device()) refuse("%s: %s has to be on the GPU, with the other tensors", who, name);
+}
+
+// int64 positions [T], or [B, T]: of every sequence its own
+struct Positions {
+    at::Tensor pos;
+    int each;
+
+    Positions(const char* who, PyObject* o, const at::Tensor& with, int64_t batch, int64_t tokens) : pos(tensor(o)), each(pos.dim() == 2)
+    {
+        if (pos.scalar_type() != at::kLong || !(each ? pos.size(0) == batch && pos.size(1) == tokens : pos.dim() == 1 && pos.size(0) == tokens))
+            refuse("%s: positions are int64 [T] or [B, T] with B = %lld, T = %lld", who, static_cast<long long>(batch), static_cast<long long>(tokens));
+        check_device(who, "pos", pos, with);
+        pos = pos.contiguous();
+    }
+    const long long* data() const { return reinterpret_cast<const long long*>(pos.const_data_ptr<int64_t>()); }
+};
+
+struct Frequencies {
+    at::Tensor held;
+
+    Frequencies(const char* who, PyObject* o, const at::Tensor& with, int64_t dim) : held(tensor(o))
+    {
+        if (held.scalar_type() != at::kDouble || held.dim() != 1 || held.size(0) < 1 || 2 * held.size(0) > dim)
+            refuse("%s: inv_freq is a float64 vector of 1 to %lld elements", who, static_cast<long long>(dim / 2));
+        check_device(who, "inv_freq", held, with);
+        held = held.contiguous();
+    }
+    const double* data() const { return held.const_data_ptr<double>(); }
+    int pairs() const { return static_cast<int>(held.size(0)); }
+};
+
+// bytes from a tensor's first element to behind its last
+int64_t byte_extent(const at::Tensor& t)
+{
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * static_cast<int64_t>(t.element_size());
+}
+// whether two indexes may name the same element
+bool overlaps_itself(const at::Tensor& t)
+{
+    std::vector<std::pair<int64_t, int64_t>> dims;             // (stride, size)
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+    std::sort(dims.begin(), dims.end());
+    int64_t extent = 1;
+    for (const auto& [stride, size] : dims) {
+        if (stride < extent) return true;
+        extent = stride * (size - 1) + extent;
+    }
+    return false;
+}
+bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
+
+// (x [B, T, H, D], pos, inv_freq, amplitude, adjacent, out | None) -> out
+TERNA_FUNCTION(rotary_embed, 6)
+{
+    const char* who = "rotary_embed";
+    const at::Tensor& x = tensor(a[0]);
+    const at::Tensor* given = optional(a[5]);
+    const double amplitude = PyFloat_AsDouble(a[3]);
+    if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
+    const int adjacent = PyObject_IsTrue(a[4]);
+    if (x.dim() != 4 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat)) refuse("%s: x is a bfloat16 or float32 [B, T, H, D] tensor", who);
+    check_device(who, "x", x, x);
+    const int64_t b = x.size(0), t = x.size(1), h = x.size(2), d = x.size(3);
+    if (d > 1024 || h > 65535 || b * t > 1 << 30) refuse("%s: at most 65535 heads of 1024 dimensions and 2^30 tokens", who);
+    if (d < 2) refuse("%s: heads have two dimensions at least", who);
+    const Positions pos(who, a[1], x, b, t);
+    const Frequencies frequency(who, a[2], x, d);
+    if (given != nullptr) {
+        if (given->scalar_type() != x.scalar_type() || given->sizes() != x.sizes()) refuse("%s: out has another shape or type than x", who);
+        check_device(who, "out", *given, x);
+        const char *p = static_cast<const char*>(x.const_data_ptr()), *q = static_cast<const char*>(given->const_data_ptr());
+        const bool same = p == q && x.strides() == given->strides();
+        if (x.numel() != 0 && (overlaps_itself(*given) || given->stride(3) != 1 || (!same && p < q + byte_extent(*given) && q < p + byte_extent(x))))
+            refuse("%s: out is x itself, or rows of their own, its last dimension contiguous", who);
+    }
+    Guard guard;
+    on_device_of(guard, x);
+    Unlocked unlocked;
+    // (a last dimension of other strides: a copy, which an out that is x is not written through, but its own memory)
+    const at::Tensor rows = x.stride(3) == 1 ? x : x.contiguous();
+    at::Tensor out = given != nullptr ? *given : make(x.sizes(), x.scalar_type(), x);
+    if (x.numel() == 0) return wrap(std::move(out), unlocked);
+    const long long in_strides[3] = {rows.stride(0), rows.stride(1), rows.stride(2)}, out_strides[3] = {out.stride(0), out.stride(1), out.stride(2)};
+    const int rc = lib.ternaspmm_rotary(rows.const_data_ptr(), in_strides, out.mutable_data_ptr(), out_strides, x.scalar_type() == at::kFloat, pos.data(), pos.each,
+                                        frequency.data(), frequency.pairs(), amplitude, b, t, h, d, adjacent, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// k, k_scale, v, v_scale from a[0 .. 3]
+struct Kv4 {
+    ternaspmm_kv4 c;
+    int64_t batch, kv, slots, dim;
+
+    Kv4(const char* who, PyObject* const* a)
+    {
+        const at::Tensor *t[4] = {&tensor(a[0]), &tensor(a[1]), &tensor(a[2]), &tensor(a[3])};
+        if (t[0]->dim() != 4) refuse("%s: the cache's codes are uint8 [B, KV, S, D / 2]", who);
+        batch = t[0]->size(0), kv = t[0]->size(1), slots = t[0]->size(2), dim = 2 * t[0]->size(3);
+        if ((dim != 64 && dim != 128) || kv < 1 || kv > 4096 || slots < 1 || slots > 1 << 25)
+            refuse("%s: a cache has heads of 64 or 128 dimensions and 1 to 2^25 slots", who);
+        for (int i = 0; i < 4; ++i) {
+            const std::array<int64_t, 4> want{batch, kv, slots, i & 1 ? dim / 32 : dim / 2};
+            if (t[i]->scalar_type() != at::kByte || t[i]->sizes() != at::IntArrayRef(want) || !t[i]->is_contiguous() || !(i & 1 || aligned16(*t[i])))
+                refuse("%s: the cache is contiguous uint8: codes [B, KV, S, D / 2] from a multiple of 16 bytes on, scales [B, KV, S, D / 32]", who);
+            check_device(who, "the cache", *t[i], *t[0]);
+        }
+        c = ternaspmm_kv4{data<uint8_t>(t[0]), data<uint8_t>(t[1]), data<uint8_t>(t[2]), data<uint8_t>(t[3])};
+    }
+};
+
+// rows of a fused projection: bf16 [B * T, (H + 2 KV) D]
+at::Tensor projection_rows(const char* who, const at::Tensor& x, const at::Tensor& codes, const Kv4& cache, int64_t heads, int64_t* tokens)
+{
+    if (x.dim() != 2 || x.scalar_type() != at::kBFloat16 || heads < 1 || heads > 4096 || heads % cache.kv != 0 || x.size(1) != (heads + 2 * cache.kv) * cache.dim)
+        refuse("%s: xqkv is bfloat16 [B * T, (H + 2 KV) D] with H a multiple of KV", who);
+    check_device(who, "xqkv", x, codes);
+    if (cache.batch < 1 ? x.size(0) != 0 : x.size(0) % cache.batch != 0) refuse("%s: %lld rows for %lld sequences", who, static_cast<long long>(x.size(0)), static_cast<long long>(cache.batch));
+    *tokens = cache.batch < 1 ? 0 : x.size(0) / cache.batch;
+    if (x.size(0) * heads > 1 << 28 || x.size(0) > 1 << 24) refuse("%s: too many rows", who);
+    return x.stride(1) == 1 && x.stride(0) >= x.size(1) && x.stride(0) % 8 == 0 && aligned16(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+c10::DataPtr kv4_workspace(int64_t b, int64_t t, int64_t h, const Kv4& cache)
+{
+    const long long bytes = lib.ternaspmm_kv4_workspace_bytes(b, t, h, cache.kv, cache.dim, cache.slots);
+    return bytes > 0 ? device_allocator()->allocate(bytes) : c10::DataPtr();
+}
+
+// (xqkv, pos, inv_freq, amplitude, k, k_scale, v, v_scale, heads, adjacent) -> q [B, H, T, D]
+TERNA_FUNCTION(kv4_store, 10)
+{
+    const char* who = "kv4_store";
+    const at::Tensor &x = tensor(a[0]), &codes = tensor(a[4]);
+    const double amplitude = PyFloat_AsDouble(a[3]);
+    if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
+    const Kv4 cache(who, a + 4);
+    const int64_t heads = integer32(a[8]);
+    const int adjacent = PyObject_IsTrue(a[9]);
+    check_device(who, "the cache", codes, codes);
+    Guard guard;
+    on_device_of(guard, codes);
+    int64_t t;
+    const at::Tensor rows = projection_rows(who, x, codes, cache, heads, &t);
+    const Positions pos(who, a[1], codes, cache.batch, t);
+    const Frequencies frequency(who, a[2], codes, cache.dim);
+    Unlocked unlocked;
+    at::Tensor q = make({cache.batch, heads, t, cache.dim}, at::kBFloat16, codes);
+    if (q.numel() == 0) return wrap(std::move(q), unlocked);
+    const int rc = lib.ternaspmm_kv4_store(data<terna_bf16>(&rows), rows.stride(0), pos.data(), pos.each, frequency.data(), frequency.pairs(), amplitude, data<terna_bf16>(&q),
+                                           &cache.c, cache.batch, t, heads, cache.kv, cache.dim, cache.slots, adjacent, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(q));
+}
+
+// (k, k_scale, v, v_scale, pos) -> (keys, values) bf16 [B, T, KV, D]
+TERNA_FUNCTION(kv4_rows, 5)
+{
+    const char* who = "kv4_rows";
+    const at::Tensor &codes = tensor(a[0]), &at_slot = tensor(a[4]);
+    const Kv4 cache(who, a);
+    check_device(who, "the cache", codes, codes);
+    if (at_slot.dim() < 1) refuse("%s: positions are int64 [T] or [B, T]", who);
+    Guard guard;
+    on_device_of(guard, codes);
+    const int64_t t = at_slot.size(-1);
+    const Positions pos(who, a[4], codes, cache.batch, t);
+    if (cache.batch * t * cache.kv > 1 << 28 || cache.batch * t > 1 << 24) refuse("%s: too many rows", who);
+    Unlocked unlocked;
+    at::Tensor k = make({cache.batch, t, cache.kv, cache.dim}, at::kBFloat16, codes), v = make({cache.batch, t, cache.kv, cache.dim}, at::kBFloat16, codes);
+    const int rc = k.numel() == 0 ? 0
+                                  : lib.ternaspmm_kv4_rows(&cache.c, pos.data(), pos.each, data<terna_bf16>(&k), data<terna_bf16>(&v), cache.batch, t, cache.kv, cache.dim,
+                                                           cache.slots, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return pack(unlocked, std::move(k), std::move(v));
+}
+
+// (q [B, H, T, D], pos, k, k_scale, v, v_scale, scale) -> [B * T, H * D]
+TERNA_FUNCTION(kv4_attention, 7)
+{
+    const char* who = "kv4_attention";
+    const at::Tensor &q = tensor(a[0]), &codes = tensor(a[2]);
+    const Kv4 cache(who, a + 2);
+    const float scale = real(a[6]);
+    check_device(who, "the cache", codes, codes);
+    if (q.dim() != 4 || q.scalar_type() != at::kBFloat16 || q.size(0) != cache.batch || q.size(3) != cache.dim || q.size(1) < 1 || q.size(1) > 4096 || q.size(1) % cache.kv != 0)
+        refuse("%s: q is bfloat16 [B, H, T, D] with the cache's B and D and H a multiple of its KV", who);
+    check_device(who, "q", q, codes);
+    const int64_t h = q.size(1), t = q.size(2);
+    if (cache.batch * t * h > 1 << 28 || cache.batch * t > 1 << 24) refuse("%s: too many rows", who);
+    Guard guard;
+    on_device_of(guard, codes);
+    const Positions pos(who, a[1], codes, cache.batch, t);
+    const at::Tensor rows = q.is_contiguous() && aligned16(q) ? q : q.clone(at::MemoryFormat::Contiguous);
+    Unlocked unlocked;
+    at::Tensor out = make({cache.batch * t, h * cache.dim}, at::kBFloat16, codes);
+    if (out.numel() == 0) return wrap(std::move(out), unlocked);
+    const c10::DataPtr work = kv4_workspace(cache.batch, t, h, cache);
+    const int rc = lib.ternaspmm_kv4_attention(data<terna_bf16>(&rows), &cache.c, pos.data(), pos.each, data<terna_bf16>(&out), work.get(), cache.batch, t, h, cache.kv, cache.dim,
+                                               cache.slots, scale, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// (xqkv, pos, inv_freq, amplitude, k, k_scale, v, v_scale, heads, adjacent, scale) -> [B, H * D]
+TERNA_FUNCTION(kv4_step, 11)
+{
+    const char* who = "kv4_step";
+    const at::Tensor &x = tensor(a[0]), &codes = tensor(a[4]);
+    const double amplitude = PyFloat_AsDouble(a[3]);
+    if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
+    const Kv4 cache(who, a + 4);
+    const int64_t heads = integer32(a[8]);
+    const int adjacent = PyObject_IsTrue(a[9]);
+    const float scale = real(a[10]);
+    check_device(who, "the cache", codes, codes);
+    Guard guard;
+    on_device_of(guard, codes);
+    int64_t t;
+    const at::Tensor rows = projection_rows(who, x, codes, cache, heads, &t);
+    if (cache.batch > 0 && t != 1) refuse("%s: one new token per sequence", who);
+    const Positions pos(who, a[1], codes, cache.batch, 1);
+    const Frequencies frequency(who, a[2], codes, cache.dim);
+    Unlocked unlocked;
+    at::Tensor out = make({cache.batch, heads * cache.dim}, at::kBFloat16, codes);
+    if (out.numel() == 0) return wrap(std::move(out), unlocked);
+    const c10::DataPtr work = kv4_workspace(cache.batch, 1, heads, cache);
+    const int rc = lib.ternaspmm_kv4_step(data<terna_bf16>(&rows), rows.stride(0), pos.data(), pos.each, frequency.data(), frequency.pairs(), amplitude, &cache.c,
+                                          data<terna_bf16>(&out), work.get(), cache.batch, heads, cache.kv, cache.dim, cache.slots, scale, adjacent, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// (logits [M, V], targets | None, top) -> (logprob | None, entropy, top_ids | None, top_logprobs | None)
+TERNA_FUNCTION(token_logprobs, 3)
+{
+    const char* who = "token_logprobs";
+    const at::Tensor& logits = tensor(a[0]);
+    const at::Tensor* targets = optional(a[1]);
+    const int top = integer32(a[2]);
+    if (logits.dim() != 2 || (logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)) refuse("%s: logits are bfloat16 or float32 [M, V]", who);
+    check_device(who, "logits", logits, logits);
+    const int64_t m = logits.size(0), v = logits.size(1);
+    if (v < 1 || v > 1 << 30 || m > 1 << 24) refuse("%s: 1 to 2^30 logits in at most 2^24 rows", who);
+    if (top < 0 || top > 64 || top > v) refuse("%s: top is 0 to 64 and at most V", who);
+    if (targets != nullptr) {
+        if (targets->scalar_type() != at::kLong || targets->dim() != 1 || targets->size(0) != m) refuse("%s: targets are int64 [M]", who);
+        check_device(who, "targets", *targets, logits);
+    }
+    Guard guard;
+    on_device_of(guard, logits);
+    Unlocked unlocked;
+    const at::Tensor rows = v == 1 || logits.stride(1) == 1 ? logits : logits.contiguous();
+    at::Tensor wanted, logprob, entropy = make({m}, at::kFloat, logits), ids, values;
+    if (targets != nullptr) {
+        wanted = targets->contiguous();
+        logprob = make({m}, at::kFloat, logits);
+    }
+    if (top > 0) {
+        ids = make({m, top}, at::kLong, logits);
+        values = make({m, top}, at::kFloat, logits);
+    }
+    int rc = 0;
+    if (m > 0) {
+        const long long bytes = lib.ternaspmm_token_logprobs_workspace_bytes(m, v, top);
+        const c10::DataPtr work = bytes > 0 ? device_allocator()->allocate(bytes) : c10::DataPtr();
+        rc = lib.ternaspmm_token_logprobs(rows.const_data_ptr(), rows.stride(0), logits.scalar_type() == at::kFloat, targets != nullptr ? data<long long>(&wanted) : nullptr,
+                                          targets != nullptr ? data<float>(&logprob) : nullptr, data<float>(&entropy), top > 0 ? data<long long>(&ids) : nullptr,
+                                          top > 0 ? data<float>(&values) : nullptr, top, work.get(), m, v, stream());
+    }
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return pack(unlocked, std::move(logprob), std::move(entropy), std::move(ids), std::move(values));
+}
+
 // (path of libternaspmm.so)
 TERNA_FUNCTION(init, 1)
 {
@@ -911,7 +1213,8 @@ TERNA_FUNCTION(init, 1)
 PyMethodDef methods[] = {METHOD(init), METHOD(bit_linear), METHOD(bit_linear_bf16), METHOD(quant_input), METHOD(linear_packed),
                          METHOD(linear_bf16_packed), METHOD(rmsnorm_quant), METHOD(relu2_mul_rmsnorm_quant), METHOD(quant_from_stats),
                          METHOD(fused_linear), METHOD(fused_linear_own_stats), METHOD(prompt_attention), METHOD(decode_attention), METHOD(block),
-                         METHOD(attention_merge_rmsnorm_quant), METHOD(step_attention_merge), METHOD(step_inputs), METHOD(prompt_inputs), METHOD(decode_step), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(attention_merge_rmsnorm_quant), METHOD(step_attention_merge), METHOD(step_inputs), METHOD(prompt_inputs), METHOD(decode_step),
+                         METHOD(rotary_embed), METHOD(kv4_store), METHOD(kv4_rows), METHOD(kv4_attention), METHOD(kv4_step), METHOD(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

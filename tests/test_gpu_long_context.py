@@ -1,0 +1,589 @@
+"""The operators of ternainfer_amd/long_context.py against plain implementations in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import ternainfer_amd as T
+from ternainfer_amd import _lib
+from tests import _long_context as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(shape, seed, dtype=torch.bfloat16):
+    return torch.randn(shape, generator=_gen(seed), device="cuda").to(dtype)
+
+
+def _say(*what):
+    print("[case]", *what, flush=True)
+
+
+# ---- rotary ------------------------------------------------------------------------------------------------------------------------
+
+
+def _check_rotary(x, got, pos, inv_freq, amplitude, adjacent):
+    want, bound = P.turned(x.double(), pos, inv_freq, amplitude, adjacent)
+    # cos or sin rounded (and times the amplitude: the rounding covers both), a product, the sum: three roundings of at most amplitude (|a| + |b|) each;
+    # then the output's own.  Copied elements are the same.
+    out = P.HALF_BF16 if x.dtype == torch.bfloat16 else P.HALF_FP32
+    tol = 3.01 * P.HALF_FP32 * bound + out * (want.abs() + 3.01 * P.HALF_FP32 * bound) * (bound > 0)
+    assert got.dtype == x.dtype and got.shape == x.shape
+    assert P.same_or_near(got, want, tol) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("adjacent", [True, False])
+@pytest.mark.parametrize("b,t,h,d,r", [(1, 1, 1, 2, 2), (3, 1, 25, 128, 128), (2, 37, 5, 64, 32), (1, 700, 3, 80, 20), (2, 5, 7, 66, 66), (5, 3, 4, 256, 2), (1, 3, 2, 1024, 1024), (4, 300, 1, 8, 6)])
+def test_rotary(dtype, adjacent, b, t, h, d, r):
+    _say("rotary", dtype, adjacent, b, t, h, d, r)
+    x = _randn((b, t, h, d), 1, dtype)
+    inv, _ = T.rotary_frequencies(r, 10000.0)
+    pos = torch.randint(0, 200000, (b, t), generator=_gen(2), device="cuda")
+    got = T.rotary_embed(x, pos, inv, adjacent=adjacent, amplitude=1.25)
+    assert got.is_contiguous()
+    _check_rotary(x, got, pos, inv, 1.25, adjacent)
+    shared = T.rotary_embed(x, pos[0], inv, adjacent=adjacent)
+    _check_rotary(x, shared, pos[0], inv, 1.0, adjacent)
+
+
+@pytest.mark.parametrize("adjacent", [True, False])
+@pytest.mark.parametrize("cut", [0, 3, 8])
+def test_rotary_on_views_and_in_place(adjacent, cut):
+    """A view of a projection's rows: the other heads stay; rows that start at any element; a broadcast head; a last dimension that is not contiguous."""
+    rows = _randn((2, 9, 12, 128), 3)
+    inv, _ = T.rotary_frequencies(64)
+    pos = torch.arange(100, 109, device="cuda")
+    x = rows[:, :, 2:9, cut:cut + 72]
+    before = rows.clone()
+    _check_rotary(x, T.rotary_embed(x, pos, inv, adjacent=adjacent), pos, inv, 1.0, adjacent)
+    assert torch.equal(rows, before)
+    out = torch.zeros((2, 9, 7, 80), dtype=torch.bfloat16, device="cuda")
+    assert T.rotary_embed(x, pos, inv, adjacent=adjacent, out=out[..., 1:73]).data_ptr() == out[..., 1:].data_ptr()
+    _check_rotary(x, out[..., 1:73], pos, inv, 1.0, adjacent)
+    assert not out[..., 0].any() and not out[..., 73:].any()
+    assert T.rotary_embed(x, pos, inv, adjacent=adjacent, out=x) is not None
+    _check_rotary(before[:, :, 2:9, cut:cut + 72], x, pos, inv, 1.0, adjacent)
+    rows[:, :, 2:9, cut:cut + 72] = before[:, :, 2:9, cut:cut + 72]
+    assert torch.equal(rows, before)
+    wide = before[:, :, :1].expand(2, 9, 4, 128)
+    _check_rotary(wide, T.rotary_embed(wide, pos, inv, adjacent=adjacent), pos, inv, 1.0, adjacent)
+    across = before.transpose(2, 3)[..., :64, :].transpose(2, 3)
+    _check_rotary(across, T.rotary_embed(across, pos, inv, adjacent=adjacent), pos, inv, 1.0, adjacent)
+    turned = before.transpose(2, 3).contiguous().transpose(2, 3)             # last dimension strided
+    _check_rotary(turned, T.rotary_embed(turned, pos, inv, adjacent=adjacent), pos, inv, 1.0, adjacent)
+
+
+def test_rotary_far_and_negative_positions():
+    x = _randn((1, 6, 2, 64), 4, torch.float32)
+    inv, _ = T.rotary_frequencies(64)
+    pos = torch.tensor([0, -1, -70000, 1 << 20, (1 << 31) + 7, -(1 << 33)], device="cuda")
+    _check_rotary(x, T.rotary_embed(x, pos, inv), pos, inv, 1.0, True)
+    # a quarter, a half, three quarters and whole turns, where the angle's reduction changes its branch
+    quarter = torch.tensor([math.pi / 2], dtype=torch.float64, device="cuda")
+    y = T.rotary_embed(x[..., :2], torch.arange(6, device="cuda"), quarter)
+    _check_rotary(x[..., :2], y, torch.arange(6, device="cuda"), quarter, 1.0, True)
+
+
+def test_rotary_of_nothing_and_refusals():
+    inv = torch.ones(4, dtype=torch.float64, device="cuda")
+    x = _randn((2, 3, 2, 8), 5)
+    pos = torch.arange(3, device="cuda")
+    assert T.rotary_embed(x[:, :0], pos[:0], inv).shape == (2, 0, 2, 8) and T.rotary_embed(x[:0], pos, inv).shape == (0, 3, 2, 8)
+    for call in (lambda: T.rotary_embed(x[0], pos, inv), lambda: T.rotary_embed(x.half(), pos, inv), lambda: T.rotary_embed(x, pos[:2], inv), lambda: T.rotary_embed(x, pos.int(), inv),
+                 lambda: T.rotary_embed(x, pos[None], inv), lambda: T.rotary_embed(x, pos.cpu(), inv), lambda: T.rotary_embed(x, pos, inv.float()), lambda: T.rotary_embed(x, pos, inv.cpu()),
+                 lambda: T.rotary_embed(x, pos, torch.cat([inv, inv])), lambda: T.rotary_embed(x, pos, inv[:0]), lambda: T.rotary_embed(x, pos, inv, out=x[:1]),
+                 lambda: T.rotary_embed(x, pos, inv, out=x.float()), lambda: T.rotary_embed(x[:, :2], pos[:2], inv, out=x[:, 1:]),
+                 lambda: T.rotary_embed(x[:1].expand(2, 3, 2, 8), pos, inv, out=x[:1].expand(2, 3, 2, 8)), lambda: T.rotary_embed(x, pos, inv, out=torch.empty_like(x.transpose(2, 3).contiguous()).transpose(2, 3))):
+        with pytest.raises(ValueError, match="rotary_embed"):
+            call()
+
+
+# ---- store and rows ------------------------------------------------------------------------------------------------------------------
+
+
+def _stored(cache, at):
+    """Values and scale exponents of keys and values at slots at [B, T]: [B, T, KV, ...]."""
+    b = torch.arange(at.shape[0], device="cuda")[:, None]
+    got = []
+    for codes, scales in (cache[:2], cache[2:]):
+        got.append((P.values(codes[b, :, at], scales[b, :, at]), scales[b, :, at].double() - 127))
+    return got
+
+
+@pytest.mark.parametrize("adjacent", [True, False])
+@pytest.mark.parametrize("b,t,h,kv,d,r,slots", [(1, 1, 1, 1, 64, 64, 1), (2, 1, 20, 5, 128, 128, 40), (3, 33, 4, 2, 128, 32, 200), (1, 700, 5, 1, 64, 22, 700), (2, 17, 16, 2, 128, 90, 64)])
+def test_store(adjacent, b, t, h, kv, d, r, slots):
+    _say("store", adjacent, b, t, h, kv, d, r, slots)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 7))
+    before = [c.clone() for c in cache]
+    wide = _randn((b * t, (h + 2 * kv) * d + 8), 8)
+    x = wide[:, :-8]                                                             # rows further apart than their length
+    inv, _ = T.rotary_frequencies(r)
+    pos = torch.stack([torch.randperm(slots, generator=_gen(9 + i), device="cuda")[:t] for i in range(b)])
+    pos[-1, t // 2] = -1 if t > 1 else 0                                         # padding
+    if t > 2:
+        pos[0, 1] = slots                                                        # outside
+    q = T.kv4_store(x, pos, inv, cache, h, adjacent=adjacent, amplitude=1.125)
+    rows = x.double().view(b, t, h + 2 * kv, d)
+    want, bound = P.turned(rows, pos, inv, 1.125, adjacent)
+    arithmetic = 3.01 * P.HALF_FP32 * bound
+    tol = arithmetic + P.HALF_BF16 * (want.abs() + arithmetic)
+    assert q.shape == (b, h, t, d) and P.same_or_near(q, want[:, :, :h].transpose(1, 2), tol[:, :, :h].transpose(1, 2)) <= 0
+
+    inside = (pos >= 0) & (pos < slots)
+    (keys, key_e), (vals, val_e) = _stored(cache, pos.clamp(0, slots - 1))
+    # values are not turned: exactly the nearest codes
+    v = rows[:, :, h + kv:]
+    e = P.scale_exponents(v.abs().unflatten(-1, (-1, 32)).amax(-1))
+    assert torch.equal(val_e[inside], e[inside]) and torch.equal(vals[inside], P.round_codes(v, e)[inside])
+    # keys: turned in fp32 with the error `arithmetic`; rounding and choice of scale are monotonous, so the results of the two ends bracket them
+    k, slack = want[:, :, h:h + kv], arithmetic[:, :, h:h + kv]
+    groups = k.abs().unflatten(-1, (-1, 32))
+    slack_groups = slack.unflatten(-1, (-1, 32))
+    low, high = P.scale_exponents((groups - slack_groups).amax(-1).clamp(min=0)), P.scale_exponents((groups + slack_groups).amax(-1))
+    assert ((low <= key_e) & (key_e <= high))[inside].all()
+    assert ((P.round_codes(k - slack, key_e) <= keys) & (keys <= P.round_codes(k + slack, key_e)))[inside].all()
+
+    # other slots are as they were
+    b_at = torch.arange(b, device="cuda")[:, None].expand(b, t)
+    for now, then in zip(cache, before):
+        then[b_at[inside], :, pos[inside]] = now[b_at[inside], :, pos[inside]]
+        assert torch.equal(now, then)
+    # rows read back: the values, exactly
+    k_rows, v_rows = T.kv4_rows(cache, pos)
+    assert k_rows.dtype == torch.bfloat16 and k_rows.shape == (b, t, kv, d)
+    assert torch.equal(k_rows.double()[inside], keys[inside]) and torch.equal(v_rows.double()[inside], vals[inside])
+    assert torch.isnan(k_rows[~inside]).all() and torch.isnan(v_rows[~inside]).all()
+
+
+def test_store_at_every_border_and_at_the_ends_of_the_range():
+    """Values on the borders between codes and next to them, powers of two over the whole range of bf16, zeros, signs, NaN, infinities."""
+    halves = torch.arange(0, 33, device="cuda").float() / 4
+    near = torch.cat([halves, halves * (1 + 2.0 ** -7), halves * (1 - 2.0 ** -8)])
+    rows = []
+    for e in (-133, -130, -127, -126, -125, -124, -60, -3, 0, 1, 70, 119, 120, 121, 122, 123):
+        for peak in (4.0, 6.0, 6.9375, 7.0, 7.0625, 7.96875):
+            for part in near.split(31):
+                row = torch.zeros(32, device="cuda")
+                row[:part.numel()] = part.clamp(max=peak)
+                row[31] = peak
+                rows.append(torch.ldexp(row.double(), torch.tensor(e, device="cuda")).to(torch.bfloat16))
+    rows.append(torch.zeros(32, device="cuda").to(torch.bfloat16))
+    rows.append(torch.full((32,), torch.finfo(torch.bfloat16).max, device="cuda").to(torch.bfloat16))
+    signs = torch.where(torch.rand((len(rows), 32), generator=_gen(10), device="cuda") < 0.5, -1.0, 1.0).to(torch.bfloat16)
+    x = torch.stack(rows) * signs
+    n = x.shape[0] // 4 * 4
+    x = torch.cat([x[:n], x[-4:]]).view(-1, 128)
+    t = x.shape[0]
+    cache = T.Kv4Cache.empty(1, 1, t, 128)
+    T.kv4_store(torch.cat([x, x, x], 1), torch.arange(t, device="cuda"), torch.zeros(64, dtype=torch.float64, device="cuda"), cache, 1)   # angle 0: nothing turns
+    e = P.scale_exponents(x.double().abs().unflatten(-1, (-1, 32)).amax(-1))
+    want = P.round_codes(x.double(), e)
+    for codes, scales in (cache[:2], cache[2:]):
+        assert torch.equal(scales[0, 0].double() - 127, e)
+        assert torch.equal(P.values(codes[0, 0], scales[0, 0]), want)
+    assert torch.equal(T.kv4_rows(cache, torch.arange(t, device="cuda"))[1][0, :, 0].double(), want)
+    # a group with NaN or an infinity stands for NaN, its neighbours do not
+    for broken in (math.nan, math.inf, -math.inf):
+        row = torch.ones((1, 384), dtype=torch.bfloat16, device="cuda")
+        row[0, 256 + 33] = broken
+        T.kv4_store(row, torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(64, dtype=torch.float64, device="cuda"), cache, 1)
+        assert cache.v_scale[0, 0, 0].tolist() == [125, 255, 125, 125] and cache.v[0, 0, 0, 16:32].eq(0).all()
+        back = T.kv4_rows(cache, torch.zeros(1, dtype=torch.int64, device="cuda"))[1][0, 0, 0]
+        assert torch.isnan(back[32:64]).all() and back[:32].eq(1).all() and back[64:].eq(1).all()
+
+
+def test_store_refusals_and_nothing_to_store():
+    inv = torch.ones(64, dtype=torch.float64, device="cuda")
+    cache = T.Kv4Cache.empty(2, 2, 16, 128)
+    x, pos = _randn((6, 8 * 128), 11), torch.arange(3, device="cuda")
+    assert T.kv4_store(x[:0], pos[:0], inv, cache, 4).shape == (2, 4, 0, 128)
+    assert T.kv4_store(x[:0], pos[:0], inv, T.Kv4Cache.empty(0, 2, 16, 128), 4).shape == (0, 4, 0, 128)
+    assert T.kv4_rows(cache, pos[:0])[0].shape == (2, 0, 2, 128)
+    bad = lambda **kw: T.Kv4Cache(*(kw.get(n, getattr(cache, n)) for n in cache._fields))
+    for call in (lambda: T.kv4_store(x, pos, inv, cache, 3), lambda: T.kv4_store(x[:5], pos, inv, cache, 4), lambda: T.kv4_store(x.float(), pos, inv, cache, 4), lambda: T.kv4_store(x[:, :-8], pos, inv, cache, 4),
+                 lambda: T.kv4_store(x, pos[:2], inv, cache, 4), lambda: T.kv4_store(x, pos, inv.float(), cache, 4), lambda: T.kv4_store(x, pos, torch.cat([inv, inv]), cache, 4),
+                 lambda: T.kv4_store(x, pos.cpu(), inv, cache, 4), lambda: T.kv4_store(x.cpu(), pos, inv, cache, 4), lambda: T.kv4_store(x, pos, inv, bad(k=cache.k[:1]), 4),
+                 lambda: T.kv4_store(x, pos, inv, bad(v_scale=cache.v_scale[:, :, :, :2]), 4), lambda: T.kv4_store(x, pos, inv, bad(v=cache.v.char()), 4),
+                 lambda: T.kv4_store(x, pos, inv, bad(v=cache.v.cpu()), 4), lambda: T.kv4_store(x, pos, inv, bad(k=cache.k.transpose(1, 2).contiguous().transpose(1, 2)), 4),
+                 lambda: T.kv4_store(x, pos, inv, bad(k=torch.empty(cache.k.numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(cache.k.shape)), 4),
+                 lambda: T.kv4_step(x, pos, inv, cache, 4), lambda: T.kv4_step(x[:2], pos[:2], inv, cache, 4), lambda: T.kv4_rows(cache, pos.int()), lambda: T.kv4_rows(cache, torch.zeros((3, 1), dtype=torch.int64, device="cuda")),
+                 lambda: T.kv4_attention(_randn((2, 3, 1, 128), 1), pos[:1], cache), lambda: T.kv4_attention(_randn((1, 4, 1, 128), 1), pos[:1], cache),
+                 lambda: T.kv4_attention(_randn((2, 4, 1, 64), 1), pos[:1], cache), lambda: T.kv4_attention(_randn((2, 4, 1, 128), 1).float(), pos[:1], cache),
+                 lambda: T.kv4_attention(_randn((2, 4, 2, 128), 1), pos[:1], cache)):
+        with pytest.raises(ValueError, match="kv4_"):
+            call()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------------------
+
+
+def _attend(q, pos, cache, scale=None):
+    got = T.kv4_attention(q, pos, cache, scale)
+    b, h, t, d = q.shape
+    want, tol = P.attention(q, pos, cache, d ** -0.5 if scale is None else scale)
+    assert got.dtype == torch.bfloat16 and got.shape == (b * t, h * d)
+    assert P.same_or_near(got.view(b, t, h, d), want, tol) <= 0
+    return got
+
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 300, 511]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,kv", [(1, 1), (4, 1), (20, 5), (10, 2), (16, 1), (17, 1), (6, 3)])
+def test_attention_of_single_tokens(d, h, kv):
+    """Every length around the steps of 32 slots and the four waves' rounds, an empty row, a position behind the cache; the rest of the cache holds other rows."""
+    slots = 512
+    pos = torch.tensor([[n - 1] for n in LENGTHS] + [[slots - 1], [slots], [1 << 40], [-(1 << 40)]], device="cuda")
+    b = pos.shape[0]
+    _say("attention", d, h, kv)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 20))
+    _attend(_randn((b, h, 1, d), 21), pos, cache)
+
+
+@pytest.mark.parametrize("b,t,h,kv,d,slots", [(2, 2, 4, 1, 128, 40), (1, 5, 20, 5, 128, 333), (2, 33, 6, 2, 64, 100), (1, 70, 8, 8, 128, 97), (1, 130, 8, 2, 128, 260), (1, 129, 5, 1, 64, 300), (3, 1, 20, 5, 128, 1),
+                                              (1, 300, 4, 1, 128, 300), (1, 200, 16, 1, 64, 1000), (2, 90, 3, 1, 128, 200)])
+def test_attention_of_several_tokens(b, t, h, kv, d, slots):
+    _say("attention", b, t, h, kv, d, slots)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 30))
+    start = torch.tensor([(slots - t) // (i + 1) for i in range(b)], device="cuda")
+    pos = start[:, None] + torch.arange(t, device="cuda")
+    _attend(_randn((b, h, t, d), 31), pos, cache)
+    _attend(_randn((b, h, t, d), 32), torch.arange(t, device="cuda") + (slots - t), cache, scale=0.02)
+    # in any order, some padded, some behind the cache
+    mixed = torch.randint(-1, slots, (b, t), generator=_gen(33), device="cuda")
+    mixed[0, 0] = slots if t > 1 else 0
+    _attend(_randn((b, h, t, d), 34), mixed, cache)
+
+
+def test_attention_with_nothing_to_see_and_nothing_to_do():
+    cache = T.Kv4Cache(*P.random_cache(2, 1, 64, 128, 40))
+    q = _randn((2, 4, 9, 128), 41)
+    assert not T.kv4_attention(q, torch.full((9,), -1, device="cuda"), cache).any()
+    assert T.kv4_attention(q[:, :, :0], torch.zeros(0, dtype=torch.int64, device="cuda"), cache).shape == (0, 512)
+
+
+@pytest.mark.parametrize("t", [1, 3, 40, 200])
+@pytest.mark.parametrize("d", [64, 128])
+def test_slots_that_a_row_does_not_see_do_not_reach_it(t, d):
+    """Whatever they hold: any byte as a scale, the one that stands for NaN among them."""
+    slots, h, kv = 400, 8, 2
+    cache = T.Kv4Cache(*P.random_cache(1, kv, slots, d, 50))
+    pos = torch.arange(t, device="cuda") * 150 // t + 37
+    q = _randn((1, h, t, d), 51)
+    clean = _attend(q, pos, cache)
+    last = int(pos[-1])
+    for fill in (255, 254, 253, 0):
+        dirty = T.Kv4Cache(*(c.clone() for c in cache))
+        for c in dirty:
+            c[:, :, last + 1:] = torch.randint(0, 256, c[:, :, last + 1:].shape, generator=_gen(52), device="cuda", dtype=torch.uint8)
+        dirty.v_scale[:, :, last + 1:] = fill
+        dirty.k_scale[:, :, last + 1:] = fill
+        assert torch.equal(T.kv4_attention(q, pos, dirty), clean)
+    if t > 1:                                                                    # within the tokens: rows in front of the slot are clean, those behind it see it
+        middle = int(pos[t // 2])
+        for name in ("k_scale", "v_scale"):
+            dirty = T.Kv4Cache(*(c.clone() for c in cache))
+            getattr(dirty, name)[0, 1, middle, -1] = 255
+            got = _attend(q, pos, dirty).view(t, h, d)
+            assert torch.equal(got[:t // 2], clean.view(t, h, d)[:t // 2])
+            assert torch.isnan(got[t // 2:, 4:, -32:]).all() and torch.equal(got[:, :4], clean.view(t, h, d)[:, :4])
+
+
+def test_attention_of_queries_that_are_not_finite():
+    cache = T.Kv4Cache(*P.random_cache(1, 1, 100, 128, 60))
+    for broken in (math.nan, math.inf, -math.inf):
+        q = _randn((1, 4, 3, 128), 61)
+        q[0, 1, 1, 5] = broken
+        clean = q.clone()
+        clean[0, 1, 1] = 0
+        pos = torch.tensor([50, 60, 99], device="cuda")
+        got, want = T.kv4_attention(q, pos, cache).view(3, 4, 128), T.kv4_attention(clean, pos, cache).view(3, 4, 128)
+        assert torch.isnan(got[1, 1]).all()
+        got[1, 1], want[1, 1] = 0, 0
+        assert torch.equal(got, want)
+
+
+def test_attention_of_large_and_of_one_dominating_score():
+    """Scores of thousands, all negative ones, and one key far above the others, first or last."""
+    cache = T.Kv4Cache(*P.random_cache(1, 1, 300, 128, 70))
+    q = _randn((1, 4, 1, 128), 71)
+    pos = torch.tensor([299], device="cuda")
+    for factor in (300.0, -300.0, 1e-20):
+        _attend((q * factor).to(torch.bfloat16), pos, cache)
+    for slot in (0, 150, 299):
+        peaked = T.Kv4Cache(*(c.clone() for c in cache))
+        peaked.k[0, 0, slot] = 0x66                                              # 4s under a large scale
+        peaked.k_scale[0, 0, slot] = 132
+        _attend(q.abs(), pos, peaked)
+
+
+def test_caches_of_more_than_two_gigabytes():
+    """Offsets beyond 2^31: the last sequence's rows."""
+    b, kv, slots, d = 3, 8, 1 << 21, 128
+    cache = T.Kv4Cache(*(torch.zeros((b, kv, slots, w), dtype=torch.uint8, device="cuda") for w in (64, 4, 64, 4)))
+    x = _randn((b, 24 * d), 80)
+    inv, _ = T.rotary_frequencies(d)
+    pos = torch.tensor([[5], [slots - 40], [slots - 1]], device="cuda")
+    assert cache.k.numel() > 1 << 31
+    first = slots - 64
+    small = P.random_cache(b, kv, 64, d, 81)
+    for c, s in zip(cache, small):
+        c[:, :, first:] = s
+    q = T.kv4_store(x, pos, inv, cache, 8)
+    k, v = T.kv4_rows(cache, pos)
+    assert torch.equal(v.view(b, kv, d).double(), P.round_codes(x[:, 16 * d:].double().view(b, kv, d), P.scale_exponents(x[:, 16 * d:].double().view(b, kv, d).abs().unflatten(-1, (-1, 32)).amax(-1))))
+    # keys of zero codes score 0: over n slots, of which the first n - 64 hold zero values
+    got = T.kv4_attention(q, pos, cache).view(b, 8, d)
+    end = int(pos[2])
+    key, value = P.values(cache.k[2, :, first:], cache.k_scale[2, :, first:]), P.values(cache.v[2, :, first:], cache.v_scale[2, :, first:])
+    score = (key * q[2].double()).sum(-1) * d ** -0.5                            # [8, 64]
+    weight = score.exp()
+    want = (weight[..., None] * value).sum(1) / (weight.sum(-1, keepdim=True) + first)
+    ds = (d + 4) * P.HALF_FP32 * d ** -0.5 * float((key.abs() * q[2].double().abs()).sum(-1).max())
+    tol = P.HALF_BF16 * want.abs() + (2 * ds + 2.0 ** -15 + (end + 1) / 8192 * P.HALF_FP32) * (weight[..., None] * value.abs()).sum(1) / (weight.sum(-1, keepdim=True) + first) * 1.0
+    # (equal terms: every wave adds 1 + ... + 1 exactly, so the sum over 2^21 slots has no error beyond the merges')
+    assert P.same_or_near(got[2], want, tol + 2.0 ** -12 * want.abs()) <= 0
+
+
+@pytest.mark.parametrize("adjacent", [True, False])
+@pytest.mark.parametrize("b,h,kv,d,r,slots,filled", [(1, 20, 5, 128, 128, 384, 253), (3, 20, 5, 128, 64, 40, 31), (1, 8, 8, 64, 64, 3000, 2999), (2, 34, 2, 128, 20, 700, 500), (4, 5, 1, 64, 50, 64, 0), (1, 4, 1, 128, 128, 20000, 19999)])
+def test_step_is_store_and_attention(adjacent, b, h, kv, d, r, slots, filled):
+    """Outputs and cache, bit for bit; also with a padded sequence and one behind the cache."""
+    _say("step", adjacent, b, h, kv, d, r, slots, filled)
+    inv, amplitude = T.rotary_frequencies(r, 500000.0, {"type": "yarn", "factor": 4, "original_max_position": 8192})
+    one, two = (T.Kv4Cache(*P.random_cache(b, kv, slots, d, 90)) for _ in range(2))
+    pos = (torch.full((b, 1), filled, device="cuda") - 3 * torch.arange(b, device="cuda")[:, None]).clamp(min=0)
+    for change in range(3):
+        if change == 1:
+            pos[-1] = -1
+        if change == 2:
+            pos[-1] = slots
+        x = _randn((b, (h + 2 * kv) * d), 91 + change)
+        got = T.kv4_step(x, pos, inv, one, h, adjacent=adjacent, amplitude=amplitude)
+        q = T.kv4_store(x, pos, inv, two, h, adjacent=adjacent, amplitude=amplitude)
+        want = T.kv4_attention(q, pos, two)
+        for x1, x2 in zip(one, two):
+            assert torch.equal(x1, x2)
+        same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+        assert same.all()
+        assert torch.isnan(got[-1]).all() == (change == 2) and (change != 1 or not got[-1].any())
+    if b > 1:
+        shared = torch.tensor([filled], device="cuda")
+        x = _randn((b, (h + 2 * kv) * d), 99)
+        assert torch.equal(T.kv4_step(x, shared, inv, one, h, adjacent=adjacent), T.kv4_step(x, shared.expand(b)[:, None].contiguous(), inv, two, h, adjacent=adjacent))
+
+
+def test_step_of_rows_that_are_not_finite():
+    """A key or value with NaN: its group for NaN from then on, other sequences as without."""
+    inv, _ = T.rotary_frequencies(128)
+    for at in (20 * 128 + 5, 25 * 128 + 40):
+        cache, other = (T.Kv4Cache(*P.random_cache(2, 5, 100, 128, 100)) for _ in range(2))
+        x = _randn((2, 30 * 128), 101)
+        pos = torch.tensor([[40], [99]], device="cuda")
+        want = T.kv4_step(x, pos, inv, other, 20)
+        x[0, at] = math.nan
+        got = T.kv4_step(x, pos, inv, cache, 20)
+        assert torch.equal(got[1], want[1])
+        # 4 query heads of the first kv head: everything under a broken key, the second 32 dimensions under a broken value
+        head = torch.isnan(got[0].view(20, 128)[:4])
+        assert head.all() if at < 25 * 128 else (head[:, 32:64].all() and not head[:, :32].any() and not head[:, 64:].any())
+        assert torch.equal(got[0].view(20, 128)[4:], want[0].view(20, 128)[4:])
+
+
+class _Kv4(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "k_scale", "v", "v_scale")]
+
+
+def test_c_entry_point_without_a_workspace():
+    """One part a row: within the tolerance of the split form."""
+    lib = _lib.load()
+    b, h, kv, d, slots = 1, 20, 5, 128, 2000
+    cache = P.random_cache(b, kv, slots, d, 110)
+    q, pos = _randn((b, h, 1, d), 111), torch.tensor([1990], device="cuda")
+    out = torch.empty((b, h * d), dtype=torch.bfloat16, device="cuda")
+    assert lib.ternaspmm_kv4_splits(b, 1, h, kv, d, slots) > 1
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.ternaspmm_kv4_attention(q.data_ptr(), ctypes.byref(_Kv4(*(c.data_ptr() for c in cache))), pos.data_ptr(), 0, out.data_ptr(), None, b, 1, h, kv, d, slots, d ** -0.5, stream) == 0
+    want, tol = P.attention(q, pos, cache, d ** -0.5)
+    assert P.same_or_near(out.view(b, 1, h, d), want, tol) <= 0
+
+
+# ---- log probabilities ---------------------------------------------------------------------------------------------------------------
+
+
+def _check_logprobs(logits, targets, top):
+    got = T.token_logprobs(logits, targets, top)
+    x = logits.double()
+    m, v = x.shape
+    peak = x.amax(-1, keepdim=True)
+    logp = torch.log_softmax(x, -1)
+    p = logp.exp()
+    terms = torch.where(p == 0, torch.zeros_like(p), p * logp)
+    entropy = -terms.sum(-1)
+    # e = exp2((x - m) log2 e): relative error (|x - m| + 4) 2^-23 (difference, product, the exponential's); a sum of V / 256 and more terms in fp32 by one
+    # thread and then a tree; log, and the last differences.
+    far = torch.where(p > 0, (peak - x), torch.zeros_like(x)).amax(-1).clamp(max=110.0)
+    relative = (far + 8) * 2.0 ** -23 + (v / 256 + 64) * P.HALF_FP32
+    spread = (p * torch.where(p > 0, (logp - logp.amax(-1, keepdim=True)).abs(), torch.zeros_like(p))).sum(-1)
+    tol_entropy = relative * (1 + 2 * spread) + 2.0 ** -22 * (spread + math.log(v) + 1)
+    assert got.entropy.dtype == torch.float32 and P.same_or_near(got.entropy, entropy, tol_entropy) <= 0
+    size = lambda lp: relative.view(-1, *[1] * (lp.dim() - 1)) + 2.0 ** -22 * (lp.abs().clamp(max=1e30) + math.log(v) + 1)
+    if targets is not None:
+        inside = (targets >= 0) & (targets < v)
+        want = torch.where(inside, logp.gather(1, targets.clamp(0, v - 1)[:, None])[:, 0], torch.tensor(math.nan, dtype=torch.float64, device="cuda"))
+        assert P.same_or_near(got.logprob, want, size(want)) <= 0
+    else:
+        assert got.logprob is None
+    if top == 0:
+        assert got.top_ids is None and got.top_logprobs is None
+        return got
+    order = torch.where(torch.isnan(logits.float()), -math.inf, logits.float())
+    ids = torch.sort(order, dim=-1, descending=True, stable=True).indices
+    if torch.isnan(logits).any():                                                # numbers first, -inf among them
+        nan = torch.isnan(logits)
+        ids = torch.stack([torch.cat([row[~gone[row]], torch.nonzero(gone)[:, 0]]) for row, gone in zip(ids, nan)])
+    assert torch.equal(got.top_ids, ids[:, :top])
+    want = logp.gather(1, ids[:, :top])
+    assert P.same_or_near(got.top_logprobs, want, size(want)) <= 0
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,v,top", [(1, 1, 1), (1, 1, 0), (3, 2, 2), (5, 7, 5), (2, 64, 64), (4, 100, 64), (1, 2047, 1), (7, 2048, 3), (2, 2049, 33), (1, 32000, 5), (600, 4096, 20), (3, 50021, 64),
+                                     (1, 128256, 5), (40, 128256, 20), (2, 128256, 0)])
+def test_logprobs(dtype, m, v, top):
+    _say("logprobs", dtype, m, v, top)
+    logits = (_randn((m, v), 200 + v, torch.float32) * 3).to(dtype)
+    targets = torch.randint(0, v, (m,), generator=_gen(201), device="cuda")
+    targets[0] = v - 1
+    _check_logprobs(logits, targets, top)
+    _check_logprobs(logits, None, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("v,ld,cut", [(4999, 4999, 0), (4999, 5003, 1), (5000, 5001, 7), (129, 131, 3), (3, 5, 2), (128256, 128259, 5)])
+def test_logprobs_of_rows_at_any_element(dtype, v, ld, cut):
+    wide = (_randn((9, ld + cut), 210, torch.float32) * 2).to(dtype)
+    wide[:, :cut] = math.inf                                                     # what lies around a row does not count
+    wide[:, cut + v:] = math.nan
+    logits = wide[:, cut:cut + v]
+    targets = torch.tensor([0, v - 1, -1, v, 1, 1 << 40, -(1 << 40), 0, 2], device="cuda")
+    _check_logprobs(logits, targets, min(v, 20))
+    _check_logprobs(logits.t().contiguous().t(), targets, min(v, 20))
+    same = logits[:1].expand(9, v)
+    _check_logprobs(same, targets, min(v, 20))
+
+
+def test_logprobs_where_values_tie_and_where_they_are_not_finite():
+    v = 128256
+    gen = _gen(220)
+    base = (_randn((13, v), 221, torch.float32) * 2).to(torch.bfloat16)
+    base[0] = 1.5                                                                # all the same
+    base[1] = -math.inf
+    base[1, [77, 128000, 5, 6000]] = torch.tensor([1.0, 2.0, 1.0, -3.0], device="cuda").to(torch.bfloat16)      # four tokens allowed
+    base[2] = -math.inf                                                          # none
+    base[3, 1000] = math.nan
+    base[4, [3, 99]] = math.inf
+    base[5] = math.nan
+    base[6] = torch.arange(v, device="cuda").to(torch.bfloat16)                  # rising, in runs of equal values
+    base[7] = -torch.arange(v, device="cuda").to(torch.bfloat16)
+    base[8] = torch.where(torch.arange(v, device="cuda") % 2048 < 512, 20.0, -20.0).to(torch.bfloat16)          # all that is large with a quarter of the threads
+    base[8] += torch.randn(v, generator=gen, device="cuda").to(torch.bfloat16)
+    base[9] = 0.0
+    base[9, ::2] = -0.0
+    base[10, :] = math.nan
+    base[10, [4, 9000, 128255]] = torch.tensor([1.0, -math.inf, 7.0], device="cuda").to(torch.bfloat16)
+    base[11, :127000] = -math.inf
+    base[12, 3] = 3e38
+    base[12, 4] = -3e38
+    targets = torch.randint(0, v, (13,), generator=gen, device="cuda")
+    targets[1] = 128000
+    base9 = base.clone()
+    base9[9] = 0.0                                                               # (the oracle's sort: zeros of both signs are equal, the lower index first)
+    for rows in (slice(0, 9), slice(10, 13)):
+        for top in (1, 20, 64):
+            _check_logprobs(base[rows], targets[rows], top)
+            _check_logprobs(base[rows].float(), targets[rows], top)
+    got = T.token_logprobs(base[9:10], None, 20)
+    assert got.top_ids.tolist() == T.token_logprobs(base9[9:10], None, 20).top_ids.tolist() == [list(range(20))]
+
+
+def test_logprobs_many_rows_do_not_depend_on_the_split():
+    """A row alone (split over workgroups) and among many (one workgroup each): same ids, probabilities within two roundings of each sum."""
+    logits = (_randn((700, 20000), 230, torch.float32) * 3).to(torch.bfloat16)
+    many = T.token_logprobs(logits, logits.argmax(-1), 10)
+    for i in (0, 699):
+        one = T.token_logprobs(logits[i:i + 1], logits.argmax(-1)[i:i + 1], 10)
+        assert torch.equal(one.top_ids[0], many.top_ids[i])
+        assert (one.top_logprobs[0] - many.top_logprobs[i]).abs().max() <= 2 * (20000 / 256 + 64) * P.HALF_FP32 + 2.0 ** -20
+    again = T.token_logprobs(logits, logits.argmax(-1), 10)
+    assert all(torch.equal(a, b) for a, b in zip(many, again))
+
+
+def test_logprobs_refusals_and_no_rows():
+    x = _randn((4, 10), 240)
+    targets = torch.zeros(4, dtype=torch.int64, device="cuda")
+    assert T.token_logprobs(x[:0], targets[:0], 3).top_ids.shape == (0, 3)
+    for call in (lambda: T.token_logprobs(x[0], None), lambda: T.token_logprobs(x.half()), lambda: T.token_logprobs(x[:, :0]), lambda: T.token_logprobs(x, targets[:3]),
+                 lambda: T.token_logprobs(x, targets.int()), lambda: T.token_logprobs(x, targets.cpu()), lambda: T.token_logprobs(x, None, 11), lambda: T.token_logprobs(x, None, -1),
+                 lambda: T.token_logprobs(_randn((1, 100), 1), None, 65)):
+        with pytest.raises(ValueError, match="token_logprobs"):
+            call()
+
+
+# ---- a run of them -------------------------------------------------------------------------------------------------------------------
+
+
+def test_a_request_from_positions_to_scores_eager_and_captured():
+    """A prompt stored and attended, then steps and their scores: eager, and as a graph replayed with eager work between, on a stream of its own."""
+    b, h, kv, d, slots, vocab = 2, 20, 5, 128, 1200, 32000
+    inv, amplitude = T.rotary_frequencies(d, 500000.0, {"type": "linear", "factor": 4.0})
+    prompt = torch.tensor([700, 650], device="cuda")
+    head = _randn((h * d, vocab), 300) * 0.05
+    eager, graphed = T.Kv4Cache.empty(b, kv, slots, d), T.Kv4Cache.empty(b, kv, slots, d)
+    x0 = _randn((b * 700, (h + 2 * kv) * d), 301)
+    at = torch.arange(700, device="cuda").expand(b, 700)
+    at = torch.where(at < prompt[:, None], at, -1)
+    outs = []
+    for cache in (eager, graphed):
+        q = T.kv4_store(x0, at, inv, cache, h, amplitude=amplitude)
+        outs.append(T.kv4_attention(q, at, cache))
+    assert torch.equal(outs[0], outs[1]) and not outs[0].view(b, 700, -1)[1, 650:].any()
+    assert not eager.v_scale[1, :, 650:].any()
+
+    def step(x, pos, cache):
+        o = T.kv4_step(x, pos, inv, cache, h, amplitude=amplitude)
+        turned = T.rotary_embed(o.view(b, 1, h, d), pos, inv)
+        logits = torch.matmul(turned.view(b, h * d), head)
+        return (o, *T.token_logprobs(logits, pos[:, 0], 5))
+
+    steps = [_randn((b, (h + 2 * kv) * d), 310 + i) for i in range(6)]
+    x, pos = steps[0].clone(), prompt[:, None].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        spare = T.Kv4Cache(*(c.clone() for c in graphed))
+        step(x, pos, spare)                                                      # loads what a first call loads
+        with torch.cuda.graph(graph, stream=side):
+            captured = step(x, pos, graphed)
+    torch.cuda.current_stream().wait_stream(side)
+    for i, rows in enumerate(steps):
+        want = step(rows, prompt[:, None] + i, eager)
+        torch.cuda.synchronize()
+        x.copy_(rows)
+        pos.copy_(prompt[:, None] + i)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(captured, want):
+            assert torch.equal(got, w), i
+        for one, two in zip(eager, graphed):
+            assert torch.equal(one, two)
