@@ -2,13 +2,14 @@
 // Declarations: include/ternaspmm.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
 
 #include "../../include/ternaspmm.h"
 #include "host_util.h"
-#include "kv4_attention_kernel.h"
+#include "kv4_prefill_kernel.h"
 
 using namespace terna;
 
@@ -24,21 +25,47 @@ bool kv4_shape_ok(int B, int T, int H, int KV, int D, int S)
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool kv4_cache_ok(const ternaspmm_kv4* c) { return c && c->k && c->k_scale && c->v && c->v_scale && aligned16(c->k) && aligned16(c->v); }
 
-// Workgroups of the attention: sixteen rows of a kv head and a split each.
-long long kv4_workgroups(int B, int T, int H, int KV) { return static_cast<long long>(B) * KV * ((static_cast<long long>(T) * (H / KV) + 15) / 16); }
+// How the attention of one call is laid out: by 16 rows of a kv head and waves of their own (few rows: memory), or by 128 rows (many: matrix cores); tiles of
+// rows, and the parts that the slots are read in -- as many as fill the chip's 256 CUs while each keeps a step for every wave.
+struct Kv4Plan {
+    bool many;
+    int tiles, splits;
+};
+constexpr int kManyRows = 64;
+Kv4Plan kv4_plan(int B, int T, int H, int KV, int S)
+{
+    const int rows = T * (H / KV);
+    Kv4Plan p{rows > kManyRows, 0, 1};
+    const int tile = p.many ? kKv4Rows : 16, part = p.many ? 4 * kKv4Tile : kKv4Step * kKv4Waves;
+    p.tiles = (rows + tile - 1) / tile;
+    const long long fill = (p.many ? 256 : 512) / (static_cast<long long>(B) * KV * p.tiles), most = (S + part - 1) / part;
+    p.splits = static_cast<int>(std::min(std::max(fill, 1ll), std::min<long long>(most, kMaxSplits)));
+    return p;
+}
 
 template <bool STEP>
 int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, hipStream_t st)
 {
-    const int rows = a.T * (a.H / a.KV);
-    a.tiles = (rows + 15) / 16;
-    const long long groups = static_cast<long long>(a.B) * a.KV * a.splits, grid = (groups + 7) / 8 * 8 * a.tiles;
-    if (grid >= 1ll << 31) return -1;
-    auto kernel = D == 128 ? terna_kv4_attention_kernel<128, STEP, true> : terna_kv4_attention_kernel<64, STEP, true>;
-    if constexpr (STEP) {
-        if (!adjacent) kernel = D == 128 ? terna_kv4_attention_kernel<128, true, false> : terna_kv4_attention_kernel<64, true, false>;
+    const Kv4Plan plan = kv4_plan(a.B, a.T, a.H, a.KV, a.S);
+    a.tiles = plan.tiles;
+    a.splits = a.partial ? plan.splits : 1;
+    const long long groups = static_cast<long long>(a.B) * a.KV * a.splits;
+    if (!STEP && plan.many) {
+        const long long grid = 8 * groups * ((a.tiles + 7) / 8);
+        if (grid >= 1ll << 31) return -1;
+        const int lds = D == 128 ? Kv4PrefillLds<128>::kBytes : Kv4PrefillLds<64>::kBytes;
+        auto kernel = D == 128 ? terna_kv4_prefill_kernel<128> : terna_kv4_prefill_kernel<64>;
+        if (lds > kPlainLds - 4096) allow_dynamic_lds(kernel, lds, "hipFuncSetAttribute(4-bit attention)", __LINE__);
+        launch(kernel, dim3(grid), dim3(512), lds, st, a);
+    } else {
+        const long long grid = (groups + 7) / 8 * 8 * a.tiles;
+        if (grid >= 1ll << 31) return -1;
+        auto kernel = D == 128 ? terna_kv4_attention_kernel<128, STEP, true> : terna_kv4_attention_kernel<64, STEP, true>;
+        if constexpr (STEP) {
+            if (!adjacent) kernel = D == 128 ? terna_kv4_attention_kernel<128, true, false> : terna_kv4_attention_kernel<64, true, false>;
+        }
+        launch(kernel, dim3(grid), dim3(64 * kKv4Waves), 0, st, a);
     }
-    launch(kernel, dim3(grid), dim3(64 * kKv4Waves), 0, st, a);
     if (a.splits > 1)
         launch(D == 128 ? terna_kv4_merge_kernel<128> : terna_kv4_merge_kernel<64>, dim3(a.B * a.T * a.H), dim3(D), 0, st, a.partial, a.pos, a.out, a.T, a.H, a.splits,
                a.per_seq);
@@ -54,12 +81,7 @@ extern "C" {
 int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S)
 {
     if (!kv4_shape_ok(B, T, H, KV, D, S)) return -1;
-    // as many as give the 256 CUs two workgroups each, while each keeps a step for every wave
-    const long long wgs = kv4_workgroups(B, T, H, KV);
-    const int most = (S + kKv4Step * kKv4Waves - 1) / (kKv4Step * kKv4Waves);
-    long long splits = 512 / wgs;
-    splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
-    return static_cast<int>(splits < most ? splits : most);
+    return kv4_plan(B, T, H, KV, S).splits;
 }
 
 long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S)
@@ -108,7 +130,6 @@ int ternaspmm_kv4_attention(const terna_bf16* q, const ternaspmm_kv4* cache, con
 {
     if (!kv4_shape_ok(B, T, H, KV, D, S) || !kv4_cache_ok(cache) || !q || !pos || !out || !aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
     Kv4Attention a{};
-    a.splits = workspace ? ternaspmm_kv4_splits(B, T, H, KV, D, S) : 1;
     a.q = q, a.k = cache->k, a.k_scale = cache->k_scale, a.v = cache->v, a.v_scale = cache->v_scale, a.pos = pos, a.out = out, a.partial = static_cast<float*>(workspace);
     a.B = B, a.T = T, a.H = H, a.KV = KV, a.S = S, a.per_seq = per_sequence != 0;
     a.scale = scale * static_cast<float>(M_LOG2E);
@@ -122,7 +143,6 @@ int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* po
         !aligned16(qkv) || !aligned16(out) || !aligned16(workspace))
         return -1;
     Kv4Attention a{};
-    a.splits = workspace ? ternaspmm_kv4_splits(B, 1, H, KV, D, S) : 1;
     a.q = qkv, a.k = cache->k, a.k_scale = cache->k_scale, a.v = cache->v, a.v_scale = cache->v_scale, a.pos = pos, a.out = out, a.partial = static_cast<float*>(workspace);
     a.frequency = frequency, a.amplitude = amplitude, a.row = row, a.pairs = pairs;
     a.B = B, a.T = 1, a.H = H, a.KV = KV, a.S = S, a.per_seq = per_sequence != 0;

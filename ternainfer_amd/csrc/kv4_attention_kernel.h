@@ -24,6 +24,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKv4Waves = 4;
 constexpr int kKv4Step = 32;                   // slots of a wave's step
+constexpr float kKv4Held = -26.0f;             // a row's largest probability is held at 2^-26: sums over 2^25 slots of the largest values stay finite
 
 struct Kv4Attention {
     const uint16_t* q;                         // [B][H][T][D]; STEP: rows of `row` elements as terna_kv4_store_kernel takes them
@@ -231,10 +232,11 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // a row that has seen nothing yet: exp(-inf - 0) = 0
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
         m_run = m_new;
+        const float shift = m_use - kKv4Held;
         float sum = 0.0f, back[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(p[e] - m_use);
+            p[e] = __builtin_amdgcn_exp2f(p[e] - shift);
             sum += p[e];
         }
         l_run = l_run * alpha + sum;

@@ -69,9 +69,12 @@ def random_cache(batch, kv, slots, dim, seed, device="cuda"):
 def attention(q, pos, cache, scale):
     """q bf16 [B, H, T, D] -> (out float64 [B, T, H, D], tolerance).  The tolerance: the output's rounding, and (2 ds + 2^-15 + n 2^-24) sum p |v|, where
     ds = (D + 4) 2^-24 scale max sum |q| |k| bounds a score's error (a sum of D products in fp32) -- it enters numerator and denominator --, 2^-15 the
-    exponential's and the two-bf16 probabilities', n 2^-24 the sums over n slots.  Below the normal numbers nothing is promised: a probability, its two parts and
-    their products may each lose 2^-126 absolutely (the sum they are divided by is at least 1 where one key has the maximum), n slots n 2^-124 max |v|."""
+    exponential's and the two-bf16 probabilities', n 2^-24 the sums over n slots.  Below the normal numbers nothing is promised: a probability and its two parts
+    may each lose 2^-126 absolutely where the largest is held at 2^-26 (so that no sum of the largest values overflows): of it 2^-100, n slots n 2^-98 max |v|.
+    More than 64 rows of a kv head: probabilities in fp16, 2^-11 relative, and 2^-37 absolutely below 2^-26 of the largest (2^-25, held at 2^12)."""
     b, h, t, d = q.shape
+    many = t * (h // cache[0].shape[1]) > 64
+    rounding, below = (2.0 ** -11 + 2.0 ** -15, 2.0 ** -37) if many else (2.0 ** -15, 2.0 ** -98)
     k, v = values(cache[0], cache[1]), values(cache[2], cache[3])
     kv, s = k.shape[1:3]
     at = pos if pos.dim() == 2 else pos[None].expand(b, t)
@@ -91,8 +94,8 @@ def attention(q, pos, cache, scale):
                 p = torch.softmax((key * x).sum(-1) * scale, 0)
                 out[i, n, j] = (p[:, None] * value).sum(0)
                 ds = (d + 4) * HALF_FP32 * abs(scale) * float((key.abs() * x.abs()).sum(-1).max())
-                tol[i, n, j] = HALF_BF16 * out[i, n, j].abs() + (2 * ds + 2.0 ** -15 + (last + 1) * HALF_FP32) * (p[:, None] * value.abs()).sum(0) \
-                    + (last + 1) * 2.0 ** -124 * value.abs().nan_to_num(0.0).max()
+                tol[i, n, j] = HALF_BF16 * out[i, n, j].abs() + (2 * ds + rounding + (last + 1) * HALF_FP32) * (p[:, None] * value.abs()).sum(0) \
+                    + (last + 1) * below * value.abs().nan_to_num(0.0).max()
     return out, tol
 
 

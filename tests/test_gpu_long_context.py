@@ -325,6 +325,36 @@ def test_attention_of_large_and_of_one_dominating_score():
         _attend(q.abs(), pos, peaked)
 
 
+@pytest.mark.parametrize("t", [1, 9, 120])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_with_any_scale(t, d):
+    cache = T.Kv4Cache(*P.random_cache(2, 2, 150, d, 72))
+    q = _randn((2, 4, t, d), 73)
+    pos = torch.arange(t, device="cuda") + 150 - t
+    for scale in (0.0, -0.3, 1e-30, 4.0):
+        _attend(q, pos, cache, scale)
+
+
+@pytest.mark.parametrize("t", [1, 9, 120])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_over_scales_from_end_to_end(t, d):
+    """Values whose scales reach over the whole range of the format, and one such slot among ordinary ones."""
+    cache = T.Kv4Cache(*P.random_cache(1, 2, 300, d, 74))
+    q = _randn((1, 4, t, d), 75)
+    pos = torch.arange(t, device="cuda") + 300 - t
+    for low, high in ((2, 253), (104, 141), (100, 108), (138, 144)):
+        wide = T.Kv4Cache(*(c.clone() for c in cache))
+        wide.v_scale.copy_(torch.randint(low, high, cache.v_scale.shape, generator=_gen(76), device="cuda", dtype=torch.uint8))
+        _attend(q, pos, wide)
+    for byte in (2, 103, 104, 140, 141, 250):
+        one = T.Kv4Cache(*(c.clone() for c in cache))
+        one.v_scale[0, 1, 77, 0] = byte
+        _attend(q, pos, one)
+    low = T.Kv4Cache(*(c.clone() for c in cache))
+    low.k_scale.copy_(torch.randint(2, 128, cache.k_scale.shape, generator=_gen(77), device="cuda", dtype=torch.uint8))
+    _attend(q, pos, low)
+
+
 def test_caches_of_more_than_two_gigabytes():
     """Offsets beyond 2^31: the last sequence's rows."""
     b, kv, slots, d = 3, 8, 1 << 21, 128
