@@ -702,7 +702,7 @@ int ternaspmm_rotary(const void* x, const long long* x_strides, void* out, const
 /* A key/value cache in 4 bits: codes [B][KV][S][D / 2] and scale bytes [B][KV][S][D / 32].  A code is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign, the
  * even dimension in the lower half of a byte) and stands for code * 2^(byte - 127) of its 32 dimensions' scale byte: the smallest exponent e in
  * -125 .. 125 with max |x| <= 7 * 2^e, codes rounded to nearest (ties to even) and held to 6; byte 255 -- one of the 32 was NaN or infinite -- stands
- * for NaN.  Codes 16-byte aligned; D 64 or 128; S <= 2^25. */
+ * for NaN.  Codes 16-byte aligned, scale bytes 4; D 64 or 128; S <= 2^25. */
 typedef struct ternaspmm_kv4 {
     uint8_t *k, *k_scale, *v, *v_scale;
 } ternaspmm_kv4;

@@ -15,43 +15,78 @@ using namespace terna;
 
 namespace {
 
-constexpr int kMaxSplits = 128;
-
 bool kv4_shape_ok(int B, int T, int H, int KV, int D, int S)
 {
     return B >= 1 && T >= 1 && H >= 1 && KV >= 1 && H % KV == 0 && (D == 64 || D == 128) && S >= 1 && S <= 1 << 25 && H <= 4096 &&
            static_cast<long long>(B) * T <= 1 << 24 && static_cast<long long>(B) * T * H <= 1 << 28;
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool kv4_cache_ok(const ternaspmm_kv4* c) { return c && c->k && c->k_scale && c->v && c->v_scale && aligned16(c->k) && aligned16(c->v); }
+bool kv4_cache_ok(const ternaspmm_kv4* c) { return c && c->k && c->k_scale && c->v && c->v_scale && aligned16(c->k) && aligned16(c->v) &&
+                                                           ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3) == 0; }
 
 // How the attention of one call is laid out: by 16 rows of a kv head and waves of their own (few rows: memory), or by 128 rows (many: matrix cores); tiles of
-// rows, and the parts that the slots are read in -- as many as fill the chip's 256 CUs while each keeps a step for every wave.
+// rows, and the parts that the slots are read in.  By the times that the two take as a function of the sizes (us, from 110 measured shapes, graphs of 24 launches;
+// causal ones included, whose rows see half of what is counted here):
+//   few    a workgroup 4.2 + 0.63 a round of its four waves alone on its CU, 4.5 + 1.1 with a second one (64 dimensions: a fourth) beside it
+//   many   a workgroup 9 + 1.75 a step of its two groups (128 slots), one to a CU
+//   parts  2 for the launch that joins them, and their numerators written and read at 3 TB/s
+// Measured, few / many: 8 x 16 tokens, 4096 slots 17 / 22; 1 x 32, 32768 31 / 29; 8 x 64, 4096 55 / 41; prompts 1 x 400 14.2 / 14.9, 4 x 200 15.5 / 12.0, 1 x 1024 34.6 / 22.6;
+// parts of 1 x 1 token, 1024 slots 9.3 in one, 7.7 in four, 32768 17.2 in 102 of them; 1 x 384 tokens in one 6.1, in three 7.8.
 struct Kv4Plan {
     bool many;
-    int tiles, splits;
+    int tiles, splits, waves;
 };
-constexpr int kManyRows = 64;
-Kv4Plan kv4_plan(int B, int T, int H, int KV, int S)
+Kv4Plan kv4_plan(int B, int T, int H, int KV, int D, int S)
 {
-    const int rows = T * (H / KV);
-    Kv4Plan p{rows > kManyRows, 0, 1};
-    const int tile = p.many ? kKv4Rows : 16, part = p.many ? 4 * kKv4Tile : kKv4Step * kKv4Waves;
-    p.tiles = (rows + tile - 1) / tile;
-    const long long fill = (p.many ? 256 : 512) / (static_cast<long long>(B) * KV * p.tiles), most = (S + part - 1) / part;
-    p.splits = static_cast<int>(std::min(std::max(fill, 1ll), std::min<long long>(most, kMaxSplits)));
+    const long long rows = static_cast<long long>(T) * (H / KV), heads = static_cast<long long>(B) * KV;
+    const float all_rows = static_cast<float>(rows) * static_cast<float>(heads);
+    const long long steps = (S + kKv4Step - 1) / kKv4Step, tiles_few = (rows + 15) / 16, tiles_many = (rows + kKv4Rows - 1) / kKv4Rows;
+    auto joined = [&](long long n) { return n == 1 ? 0.0f : 2.0f + all_rows * static_cast<float>(8 * D * n) * (1.0f / 3e6f); };
+    auto few = [&](long long n) {
+        const float wgs = static_cast<float>(heads * tiles_few * n), rounds = static_cast<float>((steps + 4 * n - 1) / (4 * n));
+        return std::max(1.0f, wgs / (D == 64 ? 1024.0f : 512.0f)) * (wgs <= 256.0f ? 4.2f + 0.63f * rounds : 4.5f + 1.1f * rounds) + joined(n);
+    };
+    auto many = [&](long long n) {
+        const float wgs = static_cast<float>(heads * tiles_many * n), rounds = static_cast<float>((steps + 4 * n - 1) / (4 * n));
+        return (wgs <= 256.0f ? 1.0f : wgs / 256.0f + 0.5f) * (9.0f + 1.75f * rounds) + joined(n);
+    };
+    Kv4Plan p{false, static_cast<int>(tiles_few), 1, 4};
+    float best = few(1);
+    const long long most = std::min<long long>({kKv4MaxSplits, (steps + 3) / 4, 512 / (heads * tiles_few)});
+    // the next count of parts that saves a round
+    auto next = [&](long long n) { const long long rounds = (steps + 4 * n - 1) / (4 * n); return rounds <= 1 ? kKv4MaxSplits + 1ll : (steps + 4 * rounds - 5) / (4 * rounds - 4); };
+    for (long long n = next(1); n <= most; n = next(n))
+        if (const float time = few(n); time < best) best = time, p.splits = static_cast<int>(n);
+    // (in one part, a workgroup to a CU and a long way: eight waves instead of four, 3 x 16 tokens and 1528 slots 15.2 -> 12.0)
+    if (p.splits == 1 && heads * tiles_few <= 256 && steps > 32) p.waves = 8;
+    if (rows <= 32) return p;
+    const long long most_many = std::min<long long>({kKv4MaxSplits, steps / 8, 256 / (heads * tiles_many)});
+    for (long long n = 1; n <= std::max(1ll, most_many); n = next(n))
+        if (const float time = many(n); time < best) best = time, p = Kv4Plan{true, static_cast<int>(tiles_many), static_cast<int>(n), 8};
     return p;
+}
+
+template <int D, bool STEP>
+void launch_kv4_few(const Kv4Attention& a, int waves, int adjacent, long long grid, hipStream_t st)
+{
+    auto kernel = waves == 8 ? terna_kv4_attention_kernel<D, STEP, true, 8> : terna_kv4_attention_kernel<D, STEP, true, 4>;
+    if constexpr (STEP) {
+        if (!adjacent) kernel = waves == 8 ? terna_kv4_attention_kernel<D, true, false, 8> : terna_kv4_attention_kernel<D, true, false, 4>;
+    }
+    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * waves), 0, st, a);
 }
 
 template <bool STEP>
 int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, hipStream_t st)
 {
-    const Kv4Plan plan = kv4_plan(a.B, a.T, a.H, a.KV, a.S);
+    const Kv4Plan plan = kv4_plan(a.B, a.T, a.H, a.KV, D, a.S);
     a.tiles = plan.tiles;
     a.splits = a.partial ? plan.splits : 1;
     const long long groups = static_cast<long long>(a.B) * a.KV * a.splits;
     if (!STEP && plan.many) {
-        const long long grid = 8 * groups * ((a.tiles + 7) / 8);
+        const int rounds = (a.tiles + 7) / 8;
+        a.parts = (a.tiles + rounds - 1) / rounds;
+        const long long grid = 8 * ((groups * a.parts + 7) / 8) * rounds;
         if (grid >= 1ll << 31) return -1;
         const int lds = D == 128 ? Kv4PrefillLds<128>::kBytes : Kv4PrefillLds<64>::kBytes;
         auto kernel = D == 128 ? terna_kv4_prefill_kernel<128> : terna_kv4_prefill_kernel<64>;
@@ -60,14 +95,11 @@ int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, h
     } else {
         const long long grid = (groups + 7) / 8 * 8 * a.tiles;
         if (grid >= 1ll << 31) return -1;
-        auto kernel = D == 128 ? terna_kv4_attention_kernel<128, STEP, true> : terna_kv4_attention_kernel<64, STEP, true>;
-        if constexpr (STEP) {
-            if (!adjacent) kernel = D == 128 ? terna_kv4_attention_kernel<128, true, false> : terna_kv4_attention_kernel<64, true, false>;
-        }
-        launch(kernel, dim3(grid), dim3(64 * kKv4Waves), 0, st, a);
+        if (D == 128) launch_kv4_few<128, STEP>(a, plan.waves, adjacent, grid, st);
+        else launch_kv4_few<64, STEP>(a, plan.waves, adjacent, grid, st);
     }
     if (a.splits > 1)
-        launch(D == 128 ? terna_kv4_merge_kernel<128> : terna_kv4_merge_kernel<64>, dim3(a.B * a.T * a.H), dim3(D), 0, st, a.partial, a.pos, a.out, a.T, a.H, a.splits,
+        launch(D == 128 ? terna_kv4_merge_kernel<128> : terna_kv4_merge_kernel<64>, dim3(a.B * a.T * a.H), dim3(256), 0, st, a.partial, a.pos, a.out, a.T, a.H, a.splits,
                a.per_seq);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die(who, e, __LINE__);
@@ -81,7 +113,7 @@ extern "C" {
 int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S)
 {
     if (!kv4_shape_ok(B, T, H, KV, D, S)) return -1;
-    return kv4_plan(B, T, H, KV, S).splits;
+    return kv4_plan(B, T, H, KV, D, S).splits;
 }
 
 long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S)

@@ -9,11 +9,11 @@
 //   * Keys: a lane holds a quarter of a row (one 16-byte load of a row of 128 dimensions) and its scale byte; the products run over the dimensions in
 //     the order in which the lanes hold them, for queries and keys alike.
 //   * Values: a lane holds 32 dimensions of a row, which share a scale; converted rows go through LDS (of the wave alone) and come back transposed.
-//   * Probabilities are split into two bf16 (16 bits: their error is 2^-17, below the rounding of the output); all sums are fp32.
+//   * Values and probabilities are fp16 (below), all sums fp32.  The running maximum is raised, and the output rescaled, only where it grows by more than 2^3.
 //   * A value scale of 255 (NaN) in a slot that a row does not see must not reach it through 0 * NaN: the first such slot of each 32 dimensions is
 //     kept and NaN given to the rows that see it; the products use the largest finite scale in its place.  So also whatever unwritten slots hold.
-// What bounds it: a long cache -- memory, 68 bytes a slot, kv head and side against about 1200 clocks of a wave a step; a short one -- the launch, two
-// trips to memory (position, cache) and the chain of one step.
+// What bounds it: a long cache -- memory (4 x 32768 slots, 5 kv heads: 79 MB in 23 us, 3.4 TB/s); a short one -- the launch, two trips to memory (position,
+// cache), then 0.63 us a step of a wave, a chain through LDS and two kinds of products (1 x 384 slots 6.1 us, 1 x 100 4.9).
 #pragma once
 
 #include "kv4_store_kernel.h"
@@ -21,10 +21,34 @@
 namespace terna {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kKv4Waves = 4;
 constexpr int kKv4Step = 32;                   // slots of a wave's step
 constexpr float kKv4Held = -26.0f;             // a row's largest probability is held at 2^-26: sums over 2^25 slots of the largest values stay finite
+
+// Values and probabilities in fp16: a value is a code times a power of two, exact in fp16 for scale bytes 104 .. 140 (2^-23 .. 2^13); probabilities keep 11 bits, held
+// at 2^12 for a row's running maximum -- up to 2^15 where a larger score has not raised it yet -- so that those 2^-26 of it are still normal numbers.  Any
+// other scale marks the workgroup, which starts again with bf16 values and probabilities in two bf16, the products twice.
+constexpr uint32_t kKv4HalfLow = 104, kKv4HalfHigh = 140;
+constexpr float kKv4HeldHalf = 12.0f, kKv4Growth = 3.0f;
+
+__device__ __forceinline__ u32x4 kv4_values_half(uint32_t codes, float scale)
+{
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
+}
+
+// (as an instruction: from fmaxf the compiler makes two, each behind one that quiets a NaN that no matrix product leaves)
+__device__ __forceinline__ float kv4_max3(float a, float b, float c)
+{
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+    return m;
+}
 
 struct Kv4Attention {
     const uint16_t* q;                         // [B][H][T][D]; STEP: rows of `row` elements as terna_kv4_store_kernel takes them
@@ -35,7 +59,7 @@ struct Kv4Attention {
     const double* frequency;                   // STEP
     double amplitude;
     long long row;
-    int B, T, H, KV, S, tiles, splits, per_seq, pairs;
+    int B, T, H, KV, S, tiles, splits, per_seq, pairs, parts;
     float scale;                               // times log2(e)
 };
 
@@ -46,14 +70,14 @@ __device__ __forceinline__ int kv4_piece(int row, int piece)
     return row * (2 * D) + ((piece ^ (D == 128 ? (row & 7) << 1 : (row & 6))) << 4);
 }
 
-template <int D, bool STEP, bool ADJACENT>
-__global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(Kv4Attention a)
+template <int D, bool STEP, bool ADJACENT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Attention a)
 {
-    constexpr int NW = kKv4Waves, DL = D / 4, KI = DL / 8, DT = D / 16, GROUPS = D / kKv4Group;
+    constexpr int DL = D / 4, KI = DL / 8, DT = D / 16, GROUPS = D / kKv4Group;
     constexpr int STAGE = kKv4Step * D * 2;                    // bytes of a wave's converted values
     __shared__ __align__(16) uint8_t smem[NW * STAGE];
     __shared__ float2 stat[NW][16];
-    __shared__ int first_broken[GROUPS];
+    __shared__ int first_broken[GROUPS], wide_scales;
     __shared__ __align__(16) uint32_t new_codes[2][D / 8];     // STEP: the new token's key and value
     __shared__ uint32_t new_scale[2][GROUPS];
     __shared__ float2 angles[STEP ? D / 2 : 1];
@@ -94,32 +118,39 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
         uint32_t k[2][KI], ks[2], vs[VL];
         u32x4 v[VL];
     };
+    // Requests end with the split: a step behind it -- two are always under way -- touches no memory and gets zeros.  (Not by a branch: where a load may
+    // or may not have been issued, the wait for one in front of it waits for both.)
+    const uint32_t in_reach = static_cast<uint32_t>(max(min(end * kKv4Step, a.S), 0));
+    const __amdgpu_buffer_rsrc_t rk = make_raw_buffer(kb, in_reach * (D / 2)), rks = make_raw_buffer(ksb, in_reach * GROUPS), rv = make_raw_buffer(vb, in_reach * (D / 2)),
+                                 rvs = make_raw_buffer(vsb, in_reach * GROUPS);
     auto load = [&](int step, Tile& x) __attribute__((always_inline)) {
         const int k0 = step * kKv4Step;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t at = min(k0 + 16 * j + qi, a.S - 1);
+            const int at = (k0 + qi) * (D / 2) + g * (DL / 2) + j * 16 * (D / 2);
             if constexpr (KI == 4) {
-                const u32x4 c = *reinterpret_cast<const u32x4*>(kb + at * (D / 2) + g * (DL / 2));
+                const u32x4 c = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, at, 0, 0));
 #pragma unroll
                 for (int i = 0; i < KI; ++i) x.k[j][i] = c[i];
             } else {
-                const u32x2 c = *reinterpret_cast<const u32x2*>(kb + at * (D / 2) + g * (DL / 2));
+                const u32x2 c = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, at, 0, 0));
                 x.k[j][0] = c.x;
                 x.k[j][1] = c.y;
             }
-            x.ks[j] = ksb[at * GROUPS + k_group];
+            x.ks[j] = __builtin_amdgcn_raw_buffer_load_b8(rks, (k0 + qi) * GROUPS + k_group + j * 16 * GROUPS, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-            const uint32_t at = min(k0 + i * (64 / GROUPS) + v_row, a.S - 1);
-            x.v[i] = *reinterpret_cast<const u32x4*>(vb + at * (D / 2) + v_group * 16);
-            x.vs[i] = vsb[at * GROUPS + v_group];
+            x.v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (k0 + v_row) * (D / 2) + v_group * 16 + i * (64 / GROUPS) * (D / 2), 0, 0));
+            x.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rvs, k0 * GROUPS + lane + i * 64, 0, 0);
         }
     };
-    int step = begin + wave;
-    Tile even, odd;
-    if (step < end) load(step, even);
+    Tile ring[3];                                              // the next two steps are under way: a trip to memory takes longer than a step
+    auto load_first = [&]() __attribute__((always_inline)) {
+        load(begin + wave, ring[0]);
+        load(begin + wave + NW, ring[1]);
+    };
+    load_first();
 
     // ---- queries: a lane's quarter of its row
     bf16x8 bq[KI];
@@ -128,6 +159,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
         const int last = p64 < 0 || outside ? -1 : static_cast<int>(p64);      // one token: the same in every lane
         for (int j = tid; j < a.pairs; j += 64 * NW) angles[j] = rotary_angle(a.pos[a.per_seq ? b : 0], a.frequency[j], a.amplitude);
         if (tid < GROUPS) first_broken[tid] = 0x7fffffff;
+        if (tid == 0) wide_scales = 0;
         __syncthreads();
         // the tile's query heads, then the new key and value: eight dimensions a thread; queries through LDS into the products' order
         constexpr int PIECES = D / 8;
@@ -164,7 +196,20 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
 #pragma unroll
         for (int i = 0; i < KI; ++i) bq[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(qrow + 8 * i));
         if (tid < GROUPS) first_broken[tid] = 0x7fffffff;
+        if (tid == 0) wide_scales = 0;
         __syncthreads();
+    }
+    // The scale's sign goes into the queries, a scale of 0 too (0 * -inf would unmask a slot): the largest score is then that of the largest product.
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+    if (a.scale <= 0.0f) {
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            float x[8];
+            RotaryVector<uint16_t>::unpack(__builtin_bit_cast(u32x4, bq[i]), x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= a.scale == 0.0f ? 0.0f : -1.0f;
+            bq[i] = __builtin_bit_cast(bf16x8, RotaryVector<uint16_t>::pack(x));
+        }
     }
     // STEP: the slot that this launch fills is read from what it was filled with
     auto patch = [&](int step, Tile& x) __attribute__((always_inline)) {
@@ -191,91 +236,136 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
     const int vrow = 4 * g + (qi >> 2);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) va[dt] = kv4_piece<D>(vrow, 2 * dt + ((qi & 3) >> 1)) + 8 * (qi & 1);
-    f32x4 o[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = -INFINITY, l_run = 0.0f;
-    int broken = 0x7fffffff;                                   // this lane's 32 dimensions
-
-    auto work = [&](int step, Tile& x) __attribute__((always_inline)) {
-        const int k0 = step * kKv4Step;
-        // values -> bf16 rows in LDS
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-            const int row = i * (64 / GROUPS) + v_row;
-            if (x.vs[i] == kKv4Broken) broken = min(broken, min(k0 + row, a.S - 1));
-            const float scale = __uint_as_float(min(x.vs[i], kKv4MaxByte) << 23);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) *reinterpret_cast<u32x4*>(stage + kv4_piece<D>(row, v_group * 4 + n)) = kv4_values(x.v[i][n], scale);
-        }
-        // scores of keys 16 j + 4 g + v
-        f32x4 s[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const float scale = __uint_as_float(x.ks[j] << 23);
-#pragma unroll
-            for (int i = 0; i < KI; ++i)
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv4_values(x.k[j][i], scale)), bq[i], s[j], 0, 0, 0);
-        }
-        float p[8], top = -INFINITY;
-        if (k0 + kKv4Step <= n_full) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = s[e >> 2][e & 3] * a.scale;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = k0 + 16 * (e >> 2) + 4 * g + (e & 3) <= my_last ? s[e >> 2][e & 3] * a.scale : -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, p[e]);
-        const float m_new = fmaxf(m_run, cross_row_reduce<true>(top));
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // a row that has seen nothing yet: exp(-inf - 0) = 0
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-        m_run = m_new;
-        const float shift = m_use - kKv4Held;
-        float sum = 0.0f, back[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(p[e] - shift);
-            sum += p[e];
-        }
-        l_run = l_run * alpha + sum;
-        const u32x4 hi = RotaryVector<uint16_t>::pack(p);
-        RotaryVector<uint16_t>::unpack(hi, back);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] -= back[e];
-        const bf16x8 p_hi = __builtin_bit_cast(bf16x8, hi), p_lo = __builtin_bit_cast(bf16x8, RotaryVector<uint16_t>::pack(p));
-        // outputs: dims 16 dt + 4 g + v of row qi
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            using Tr = s16x4 __attribute__((address_space(3)))*;
-            const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(stage + va[dt])));
-            const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(stage + va[dt] + 16 * 2 * D)));
-            const bf16x8 values = __builtin_bit_cast(bf16x8, u32x4{a0.x, a0.y, a1.x, a1.y});
-            o[dt] *= alpha;
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, p_hi, o[dt], 0, 0, 0);
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, p_lo, o[dt], 0, 0, 0);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
     const int new_step = STEP && n_keys > 0 && !outside ? (n_keys - 1) / kKv4Step : -1;
-    while (step < end) {
-        if (step + NW < end) load(step + NW, odd);
-        if (STEP && step == new_step) patch(step, even);
-        work(step, even);
-        step += NW;
-        if (step >= end) break;
-        if (step + NW < end) load(step + NW, even);
-        if (STEP && step == new_step) patch(step, odd);
-        work(step, odd);
-        step += NW;
+    f32x4 o[DT];
+    float m_run, l_run;
+    int broken = 0x7fffffff;                                   // this lane's 32 dimensions
+    bool wide = false;
+    // All steps of the wave, with values and probabilities in fp16 (HALF) or with bf16 values and probabilities in two bf16.
+    auto pass = [&](auto in_half) __attribute__((always_inline)) {
+        constexpr bool HALF = decltype(in_half)::value;
+        constexpr float HELD = HALF ? kKv4HeldHalf : kKv4Held, GROWTH = HALF ? kKv4Growth : 0.0f;
+        auto work = [&](int step, Tile& x) __attribute__((always_inline)) {
+            const int k0 = step * kKv4Step;
+            // values -> rows in LDS
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int row = i * (64 / GROUPS) + v_row;
+                uint32_t byte = x.vs[i];
+                // one test for what is rare: NaN, slots that nobody sees and what they hold, scales that fp16 has no room for
+                if (k0 + kKv4Step > n_keys || __any(byte < kKv4HalfLow || byte > kKv4HalfHigh)) {
+                    if (k0 + row >= n_keys) byte = 127u;
+                    if (byte == kKv4Broken) {
+                        broken = min(broken, k0 + row);
+                        byte = 127u;
+                    }
+                    if (HALF) wide |= byte < kKv4HalfLow || byte > kKv4HalfHigh;
+                    byte = min(byte, HALF ? kKv4HalfHigh : kKv4MaxByte);
+                }
+                const float vs = __uint_as_float(byte << 23);
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    *reinterpret_cast<u32x4*>(stage + kv4_piece<D>(row, v_group * 4 + n)) = HALF ? kv4_values_half(x.v[i][n], vs) : kv4_values(x.v[i][n], vs);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // scores of keys 16 j + 4 g + v
+            f32x4 s[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                const float ks = __uint_as_float(x.ks[j] << 23);
+#pragma unroll
+                for (int i = 0; i < KI; ++i)
+                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv4_values(x.k[j][i], ks)), bq[i], s[j], 0, 0, 0);
+            }
+            // the transposed values, requested in front of the softmax: left to itself the compiler reads each where it is used, eight trips to LDS in a row
+            u32x4 values[DT];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                using Tr = s16x4 __attribute__((address_space(3)))*;
+                const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(stage + va[dt])));
+                const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(stage + va[dt] + 16 * 2 * D)));
+                values[dt] = u32x4{a0.x, a0.y, a1.x, a1.y};
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (k0 + kKv4Step > n_full) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k0 + 16 * (e >> 2) + 4 * g + (e & 3) > my_last) s[e >> 2][e & 3] = -INFINITY;
+            }
+            float top = kv4_max3(kv4_max3(s[0][0], s[0][1], s[0][2]), kv4_max3(s[0][3], s[1][0], s[1][1]), kv4_max3(s[1][2], s[1][3], s[1][3]));
+            top = cross_row_reduce<true>(top) * scale;
+            if (__any(top > m_run + GROWTH)) {
+                const float m_new = fmaxf(m_run, top);
+                const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));       // (a row that has seen nothing yet: exp(-inf))
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+            }
+            const float shift = HELD - (m_run == -INFINITY ? 0.0f : m_run);
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[e >> 2][e & 3], scale, shift));
+            // outputs: dims 16 dt + 4 g + v of row qi
+            if constexpr (HALF) {
+                u32x4 packed;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x2 pair = __builtin_convertvector((f32x2{p[2 * e], p[2 * e + 1]}), f16x2);
+                    packed[e] = __builtin_bit_cast(uint32_t, pair);
+                    l_run = __builtin_amdgcn_fdot2(pair, f16x2{1, 1}, l_run, false);
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, values[dt]), __builtin_bit_cast(f16x8, packed), o[dt], 0, 0, 0);
+            } else {
+                float back[8];
+                const u32x4 hi = RotaryVector<uint16_t>::pack(p);
+                RotaryVector<uint16_t>::unpack(hi, back);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    l_run += p[e];
+                    back[e] = p[e] - back[e];
+                }
+                const bf16x8 p_hi = __builtin_bit_cast(bf16x8, hi), p_lo = __builtin_bit_cast(bf16x8, RotaryVector<uint16_t>::pack(back));
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, values[dt]), p_hi, o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, values[dt]), p_lo, o[dt], 0, 0, 0);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        };
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run = -INFINITY;
+        l_run = 0.0f;
+        int step = begin + wave;
+        while (step < end) {
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                load(step + 2 * NW, ring[(n + 2) % 3]);
+                if (STEP && step == new_step) patch(step, ring[n]);
+                work(step, ring[n]);
+                step += NW;
+                if (step >= end) break;
+            }
+        }
+        l_run = cross_row_reduce<false>(l_run);
+        m_run -= HELD;                                         // what the probabilities are relative to: the splits of a row may differ in it
+    };
+    pass(std::true_type{});
+    if (wide) wide_scales = 1;
+    __syncthreads();
+    if (wide_scales) {                                         // (all have read it behind the barrier; nobody writes it again)
+        load_first();
+        pass(std::false_type{});
     }
 
-    // ---- the four waves
-    l_run = cross_row_reduce<false>(l_run);
+    // ---- the waves
     if (broken != 0x7fffffff) atomicMin(&first_broken[v_group], broken);      // a minimum: any order
     if (g == 0) stat[wave][qi] = float2{m_run, l_run};
     __syncthreads();
@@ -291,7 +381,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
         *reinterpret_cast<f32x4*>(numerators + qi * D + ((16 * dt + 4 * g) ^ ((qi & 7) << 2))) = o[dt];
     }
     __syncthreads();
-    // a thread: eight dimensions of a row, four waves' numerators
+    // a thread: eight dimensions of a row, the waves' numerators
     constexpr int PIECES = D / 8;
     for (int i = tid; i < 16 * PIECES; i += 64 * NW) {
         const int n = i / PIECES, d = (i & (PIECES - 1)) * 8, rr = tile * 16 + n;
@@ -332,27 +422,44 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void terna_kv4_attention_kernel(
     }
 }
 
-// The splits of a row: one workgroup of D threads.  Their order is fixed, so is the result.
+// The splits of a row: four waves, each every fourth split, D / 64 dimensions a lane.  Their order is fixed, so is the result.
+constexpr int kKv4MaxSplits = 128;             // two a lane
 template <int D>
-__global__ __launch_bounds__(D) void terna_kv4_merge_kernel(const float* __restrict__ partial, const long long* __restrict__ pos, uint16_t* __restrict__ out, int T, int H,
-                                                            int splits, int per_seq)
+__global__ __launch_bounds__(256) void terna_kv4_merge_kernel(const float* __restrict__ partial, const long long* __restrict__ pos, uint16_t* __restrict__ out, int T, int H,
+                                                              int splits, int per_seq)
 {
-    const int row = blockIdx.x, d = threadIdx.x;
-    const int token = row / H, t = token % T;
-    const float* o = partial + static_cast<size_t>(row) * splits * D + d;
+    constexpr int V = D / 64;
+    __shared__ float part[4][D];
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float2* stat = reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * splits * D) + static_cast<size_t>(row) * splits;
+    const float2 none{-INFINITY, 0.0f}, s0 = lane < splits ? stat[lane] : none, s1 = lane + 64 < splits ? stat[lane + 64] : none;
+    const float* o = partial + static_cast<size_t>(row) * splits * D + V * lane;
+    float first[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) first[v] = wave < splits ? o[static_cast<size_t>(wave) * D + v] : 0.0f;
+    const int token = row / H, t = token % T;
     const long long p = pos[per_seq ? token : t];
-    float m = -INFINITY;
-    for (int i = 0; i < splits; ++i) m = fmaxf(m, stat[i].x);
+    float m = fmaxf(s0.x, s1.x);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     const float m_use = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, x = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < splits; ++i) {
-        const float w = __builtin_amdgcn_exp2f(stat[i].x - m_use);
-        l += stat[i].y * w;
-        x += o[static_cast<size_t>(i) * D] * w;
+    const float w0 = __builtin_amdgcn_exp2f(s0.x - m_use), w1 = __builtin_amdgcn_exp2f(s1.x - m_use);
+    float l = s0.y * w0 + s1.y * w1;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = wave < splits ? first[v] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w0), wave)) : 0.0f;
+    for (int i = wave + 4; i < splits; i += 4) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(i < 64 ? w0 : w1), i & 63));
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] += o[static_cast<size_t>(i) * D + v] * w;
     }
-    out[static_cast<size_t>(row) * D + d] = float_to_bf16_bits(p < 0 ? 0.0f : x / l);
+#pragma unroll
+    for (int v = 0; v < V; ++v) part[wave][V * lane + v] = x[v];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < D) out[static_cast<size_t>(row) * D + d] = float_to_bf16_bits(p < 0 ? 0.0f : ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) / l);
 }
 
 }  // namespace terna

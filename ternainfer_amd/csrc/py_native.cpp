@@ -1014,8 +1014,8 @@ struct Kv4 {
             refuse("%s: a cache has heads of 64 or 128 dimensions and 1 to 2^25 slots", who);
         for (int i = 0; i < 4; ++i) {
             const std::array<int64_t, 4> want{batch, kv, slots, i & 1 ? dim / 32 : dim / 2};
-            if (t[i]->scalar_type() != at::kByte || t[i]->sizes() != at::IntArrayRef(want) || !t[i]->is_contiguous() || !(i & 1 || aligned16(*t[i])))
-                refuse("%s: the cache is contiguous uint8: codes [B, KV, S, D / 2] from a multiple of 16 bytes on, scales [B, KV, S, D / 32]", who);
+            if (t[i]->scalar_type() != at::kByte || t[i]->sizes() != at::IntArrayRef(want) || !t[i]->is_contiguous() || (reinterpret_cast<uintptr_t>(t[i]->const_data_ptr()) & (i & 1 ? 3 : 15)) != 0)
+                refuse("%s: the cache is contiguous uint8: codes [B, KV, S, D / 2] from a multiple of 16 bytes on, scales [B, KV, S, D / 32] from one of 4", who);
             check_device(who, "the cache", *t[i], *t[0]);
         }
         c = ternaspmm_kv4{data<uint8_t>(t[0]), data<uint8_t>(t[1]), data<uint8_t>(t[2]), data<uint8_t>(t[3])};

@@ -69,12 +69,11 @@ def random_cache(batch, kv, slots, dim, seed, device="cuda"):
 def attention(q, pos, cache, scale):
     """q bf16 [B, H, T, D] -> (out float64 [B, T, H, D], tolerance).  The tolerance: the output's rounding, and (2 ds + 2^-15 + n 2^-24) sum p |v|, where
     ds = (D + 4) 2^-24 scale max sum |q| |k| bounds a score's error (a sum of D products in fp32) -- it enters numerator and denominator --, 2^-15 the
-    exponential's and the two-bf16 probabilities', n 2^-24 the sums over n slots.  Below the normal numbers nothing is promised: a probability and its two parts
+    exponential's and that of probabilities in two bf16, n 2^-24 the sums over n slots.  Below the normal numbers nothing is promised: a probability and its two parts
     may each lose 2^-126 absolutely where the largest is held at 2^-26 (so that no sum of the largest values overflows): of it 2^-100, n slots n 2^-98 max |v|.
-    More than 64 rows of a kv head: probabilities in fp16, 2^-11 relative, and 2^-37 absolutely below 2^-26 of the largest (2^-25, held at 2^12)."""
+    Probabilities in fp16: 2^-11 relative in numerator and denominator each, and 2^-37 absolutely below 2^-26 of the largest (2^-25, held at 2^12)."""
     b, h, t, d = q.shape
-    many = t * (h // cache[0].shape[1]) > 64
-    rounding, below = (2.0 ** -11 + 2.0 ** -15, 2.0 ** -37) if many else (2.0 ** -15, 2.0 ** -98)
+    rounding, below = 2 * 2.0 ** -11 + 2.0 ** -15, 2.0 ** -37
     k, v = values(cache[0], cache[1]), values(cache[2], cache[3])
     kv, s = k.shape[1:3]
     at = pos if pos.dim() == 2 else pos[None].expand(b, t)
