@@ -110,7 +110,7 @@ PROTOTYPES = {
     "ternaspmm_kv4_workspace_bytes": ([_ci] * 6, ctypes.c_longlong),
     "ternaspmm_kv4_attention": ([_vp, _vp, _vp, _ci, _vp, _vp] + [_ci] * 6 + [ctypes.c_float, _vp], _ci),
     "ternaspmm_kv4_step": ([_vp, ctypes.c_longlong, _vp, _ci, _vp, _ci, ctypes.c_double, _vp, _vp, _vp] + [_ci] * 5 + [ctypes.c_float, _ci, _vp], _ci),
-    "ternaspmm_token_logprobs_workspace_bytes": ([_ci] * 3, ctypes.c_longlong),
+    "ternaspmm_token_logprobs_workspace_bytes": ([_ci] * 4, ctypes.c_longlong),
     "ternaspmm_token_logprobs": ([_vp, ctypes.c_longlong, _ci] + [_vp] * 5 + [_ci, _vp, _ci, _ci, _vp], _ci),
     "ternaspmm_version": ([], ctypes.c_char_p),
 }

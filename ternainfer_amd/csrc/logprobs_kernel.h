@@ -6,15 +6,20 @@
 // way, in a fixed order.  fp32 throughout: differences are formed before they are scaled, and the terms of -inf are held to exp(-1e4) = 0 so that
 // 0 * inf does not arise.
 //
-// Alternatives without a second pass over everything.  Elements are in order by (value, lower index first) as 64-bit keys; NaN below all.  A thread's
-// pieces have a best one, by value and the first piece that holds it.  If T is a bound that k of the threads' bests reach, k elements reach T, so the k
-// best elements do, and they lie with the threads whose best reaches T: those alone read their pieces again (about k / 256 of the row, from
-// the L2), elements that reach T go to LDS, and the k best of these are found by counting.  The order in which they arrive there does not matter.
-// T comes by bisection over the keys' bits, which ends as soon as exactly k reach it (10 - 15 rounds where values differ).
+// Alternatives without a second pass over everything.  Elements are in order by (value, lower index first) as 64-bit keys; NaN below all.  Sixteen lanes' pieces
+// are a block of 256 contiguous bytes, whose largest value goes to LDS (four permutations and a store for about 80 other instructions).  If T is a bound that
+// k blocks' bests reach, k elements reach T, so the k best elements do, and they lie in blocks whose best reaches T: those alone are read again, elements
+// that reach T go to LDS, and the k best of these are found by counting.  The order in which they arrive there does not matter.
+// T is the k-th best of 64 (for k > 32: of 256) bests of blocks taken together, by bisection over the keys' bits, a ballot a bit, which ends as soon as exactly
+// k reach it (10 - 15 rounds where values differ); about 1.2 k blocks reach it.  Elements go to LDS in one sweep; only where they are more than it holds are
+// they taken again in rounds, with the best k kept from each to the next.  (Blocks and not, say, the pieces of a thread: those are 4 KB apart, and the
+// second reading of the few that matter took three quarters of the row's lines, 17 us of 70 for 1024 x 128256.)
 //
 // What bounds it: many rows -- memory (vector work: 11 issue slots an element against 64 a clock and CU); one row -- two launches (the row split over
 // workgroups, then merged), a trip to memory each and the selection of the alternatives.
 #pragma once
+
+#include <type_traits>
 
 #include "terna_common.h"
 
@@ -25,6 +30,7 @@ constexpr int kLogprobMaxTop = 64;
 constexpr int kLogprobBatch = 2048;            // elements that one round over the pieces can add
 constexpr int kLogprobSlack = 512;             // kept between rounds
 constexpr int kLogprobKeys = kLogprobBatch + kLogprobSlack;
+constexpr int kLogprobBlocks = 2048;           // of a workgroup: 16 pieces each
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef unsigned long long key64;
@@ -50,6 +56,21 @@ __device__ __forceinline__ LogprobStats logprob_join(const LogprobStats& a, cons
     const float fa = __builtin_amdgcn_exp2f(da * kLog2e), fb = __builtin_amdgcn_exp2f(db * kLog2e);
     return {m, a.s * fa + b.s * fb, fa * (a.t + a.s * da) + fb * (b.t + b.s * db)};
 }
+
+// over the wave, in every lane: quads and rows by permutations within 16 lanes, then rows
+template <typename Op>
+__device__ __forceinline__ float logprob_row(float v, Op op)
+{
+    auto dpp = [](float x, auto control) {
+        return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), decltype(control)::value, 0xf, 0xf, true));
+    };
+    v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));                // lanes 1 0 3 2
+    v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));                // lanes 2 3 0 1
+    v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));               // the row's halves mirrored
+    return op(v, dpp(v, std::integral_constant<int, 0x140>{}));            // the row mirrored
+}
+__device__ __forceinline__ float logprob_wave_max(float v) { return cross_row_reduce<true>(logprob_row(v, [](float a, float b) { return fmaxf(a, b); })); }
+__device__ __forceinline__ float logprob_wave_sum(float v) { return cross_row_reduce<false>(logprob_row(v, [](float a, float b) { return a + b; })); }
 
 template <typename T>
 struct LogprobVector;
@@ -84,31 +105,28 @@ __device__ __forceinline__ int logprob_count(const key64* keys, int n, key64 bou
     for (int i = 0; i < n; i += 64) count += __popcll(__ballot(i + lane < n && keys[i + lane] >= bound));
     return count;
 }
-// A bound that `want` of the keys reach and no more (keys differ), or 0 where there are no more than that.  One wave; 4 keys a lane at most are
-// held in registers while they are counted.
+// A bound that `want` of the wave's keys, one a lane, reach and no more (keys differ); 0 where no more than that are not 0.
+__device__ __forceinline__ key64 logprob_bound64(key64 mine, int want)
+{
+    key64 bound = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const key64 next = bound | 1ull << bit;
+        const int count = __popcll(__ballot(mine >= next));
+        if (count >= want) bound = next;
+        if (count == want) break;
+    }
+    return bound;
+}
+// The same for n keys in LDS, or 0 where there are no more than `want`.  One wave.
 __device__ __forceinline__ key64 logprob_bound(const key64* keys, int n, int want, int lane)
 {
     if (n <= want) return 0;
     key64 bound = 0;
-    if (n <= 256) {
-        key64 mine[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mine[i] = 64 * i + lane < n ? keys[64 * i + lane] : 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const key64 next = bound | 1ull << bit;
-            int count = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) count += __popcll(__ballot(mine[i] >= next));
-            if (count >= want) bound = next;
-            if (count == want) break;
-        }
-    } else {
-        for (int bit = 63; bit >= 0; --bit) {
-            const key64 next = bound | 1ull << bit;
-            const int count = logprob_count(keys, n, next, lane);
-            if (count >= want) bound = next;
-            if (count == want) break;
-        }
+    for (int bit = 63; bit >= 0; --bit) {
+        const key64 next = bound | 1ull << bit;
+        const int count = logprob_count(keys, n, next, lane);
+        if (count >= want) bound = next;
+        if (count == want) break;
     }
     return bound;
 }
@@ -130,7 +148,12 @@ __device__ __forceinline__ int logprob_compact(key64* keys, int n, key64 bound, 
 // The `top` best of n keys, best first, into `sorted` (zeros where there are fewer).  One wave; keys is changed.
 __device__ __forceinline__ void logprob_best(key64* keys, int n, int top, key64* sorted, int lane)
 {
-    if (n > 64) n = logprob_compact(keys, n, logprob_bound(keys, n, top, lane), lane);
+    if (n > 64) {
+        key64 most = 0;                                                    // `top` lanes' best ones reach the bound: so do `top` keys, and few more
+        for (int i = lane; i < n; i += 64) most = most > keys[i] ? most : keys[i];
+        n = logprob_compact(keys, n, logprob_bound64(most, top), lane);
+        if (n > 64) n = logprob_compact(keys, n, logprob_bound(keys, n, top, lane), lane);
+    }
     const key64 mine = lane < n ? keys[lane] : 0;
     int rank = 0;
     for (int i = 0; i < n; ++i) {
@@ -166,13 +189,10 @@ __device__ __forceinline__ void logprob_results(const LogprobArgs& a, int row, c
 // (m, s, t) of the workgroup's threads, in every thread
 __device__ __forceinline__ LogprobStats logprob_join_all(LogprobStats s, LogprobStats* part)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const LogprobStats other{__shfl_xor(s.m, off), __shfl_xor(s.s, off), __shfl_xor(s.t, off)};
-        s = lane & off ? logprob_join(other, s) : logprob_join(s, other);
-    }
-    if (lane == 0) part[threadIdx.x >> 6] = s;
+    const float m = logprob_wave_max(s.m), use = m == -INFINITY ? 0.0f : m;
+    const float down = max_keep_nan(s.m - use, -1e4f), f = __builtin_amdgcn_exp2f(down * kLog2e);
+    const LogprobStats wave{m, logprob_wave_sum(s.s * f), logprob_wave_sum(f * __fmaf_rn(s.s, down, s.t))};
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = wave;
     __syncthreads();
     return logprob_join(logprob_join(part[0], part[1]), logprob_join(part[2], part[3]));
 }
@@ -185,7 +205,8 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
     __shared__ key64 keys[kLogprobKeys];
     __shared__ key64 sorted[kLogprobMaxTop];
     __shared__ LogprobStats part[kLogprobThreads / 64];
-    __shared__ int chosen[kLogprobThreads];
+    __shared__ float best[kLogprobBlocks];
+    __shared__ uint16_t chosen[kLogprobBlocks];
     __shared__ key64 bound_of;
     __shared__ int count_of, chosen_count;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -199,23 +220,27 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
     const int begin = split * share, end = min(begin + share, all);
     const int inside_from = lead ? 1 : 0, inside_to = (lead + a.V) / N;    // pieces of the row's elements alone
 
+    const int rounds = max(0, (end - begin + kLogprobThreads - 1) / kLogprobThreads), blocks = max(0, (end - begin + 15) / 16);
     LogprobStats s{-INFINITY, 0.0f, 0.0f};
-    int best = begin + tid;                                                // the first piece with the thread's maximum
-    auto take = [&](int piece, const u32x4& v) __attribute__((always_inline)) {
+    auto take = [&](int round, const u32x4& v) __attribute__((always_inline)) {            // (all lanes, for the blocks' sake)
+        const int piece = begin + round * kLogprobThreads + tid;
         float x[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) x[e] = Vec::at(v, e);
-        if (piece < inside_from || piece >= inside_to) {
+        if (piece < inside_from || piece >= min(inside_to, end)) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int at = piece * N + e - lead;
-                if (at < 0 || at >= a.V) x[e] = -INFINITY;
+                if (at < 0 || at >= a.V || piece >= end) x[e] = -INFINITY;
             }
         }
         float top = x[0];
 #pragma unroll
         for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-        if (top > s.m) best = piece;
+        if (a.top > 0) {
+            const float block = logprob_row(top, [](float p, float q) { return fmaxf(p, q); });
+            if ((tid & 15) == 0 && piece < end) best[(piece - begin) >> 4] = block;
+        }
         const float m = fmaxf(s.m, top), use = m == -INFINITY ? 0.0f : m;
         const float down = max_keep_nan(s.m - use, -1e4f), f = __builtin_amdgcn_exp2f(down * kLog2e);
         float sum = 0.0f, weighted = 0.0f;
@@ -229,46 +254,60 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
         s.s = __fmaf_rn(s.s, f, sum);
         s.m = m;
     };
-    int at = begin + tid;
     {
         u32x4 now[AHEAD], next[AHEAD];
-        auto fetch = [&](u32x4* to, int from) __attribute__((always_inline)) {
+        auto fetch = [&](u32x4* to, int round) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) to[i] = pieces[min(from + i * kLogprobThreads, all - 1)];
+            for (int i = 0; i < AHEAD; ++i) to[i] = pieces[min(begin + (round + i) * kLogprobThreads + tid, all - 1)];
         };
-        constexpr int ROUND = AHEAD * kLogprobThreads;
-        if (at < end) fetch(now, at);
-        while (at + ROUND - kLogprobThreads < end) {                       // whole rounds
-            fetch(next, at + ROUND);
+        int round = 0;
+        if (rounds > 0) fetch(now, 0);
+        for (; round + AHEAD <= rounds; round += AHEAD) {
+            fetch(next, round + AHEAD);
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) take(at + i * kLogprobThreads, now[i]);
-            at += ROUND;
+            for (int i = 0; i < AHEAD; ++i) take(round + i, now[i]);
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) now[i] = next[i];
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-            if (at + i * kLogprobThreads < end) take(at + i * kLogprobThreads, now[i]);
+            if (round + i < rounds) take(round + i, now[i]);
     }
-    const bool any = begin + tid < end;
-    const key64 mine = any ? static_cast<key64>(logprob_order(s.m)) << 32 | static_cast<uint32_t>(~best) : 0;
     s = logprob_join_all(s, part);
 
     const int in_range = max(0, min(end * N - lead, a.V) - max(begin * N - lead, 0));       // elements of this split
     const int want = min(a.top, in_range);
     if (a.top > 0) {
-        keys[tid] = mine;
-        if (tid == 0) count_of = 0;
-        __syncthreads();
+        if (tid == 0) count_of = 0;                                        // (`best` is whole behind the barrier in logprob_join_all)
+        auto block_key = [&](int block) __attribute__((always_inline)) {
+            return static_cast<key64>(logprob_order(best[block])) << 32 | static_cast<uint32_t>(~block);
+        };
         if (tid < 64) {
-            const key64 b = want > 0 ? logprob_bound(keys, kLogprobThreads, want, lane) : 0;
-            int n = 0;
+            key64 b = 0;
+            if (want > 32) {
+                key64 most[4] = {0, 0, 0, 0};
+                for (int i = 0; i < blocks; i += 256)
 #pragma unroll
-            for (int i = 0; i < kLogprobThreads / 64; ++i) {
-                const key64 k = keys[64 * i + lane];
-                const bool in = k != 0 && k >= b;
+                    for (int n = 0; n < 4; ++n)
+                        if (i + 64 * n + lane < blocks) most[n] = max(most[n], block_key(i + 64 * n + lane));
+                for (int bit = 63; bit >= 0; --bit) {
+                    const key64 next = b | 1ull << bit;
+                    int count = 0;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) count += __popcll(__ballot(most[n] >= next));
+                    if (count >= want) b = next;
+                    if (count == want) break;
+                }
+            } else if (want > 0) {
+                key64 most = 0;
+                for (int i = lane; i < blocks; i += 64) most = max(most, block_key(i));
+                b = logprob_bound64(most, want);
+            }
+            int n = 0;
+            for (int i = 0; i < blocks; i += 64) {
+                const bool in = i + lane < blocks && block_key(i + lane) >= b;
                 const key64 mask = __ballot(in);
-                if (in) chosen[n + __popcll(mask & ((1ull << lane) - 1))] = 64 * i + lane;
+                if (in) chosen[n + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(i + lane);
                 n += __popcll(mask);
             }
             if (lane == 0) bound_of = b, chosen_count = n;
@@ -276,25 +315,48 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
         __syncthreads();
         key64 bound = bound_of;
         int owners = chosen_count;
-        const int rounds = (end - begin + kLogprobThreads - 1) / kLogprobThreads;           // pieces a thread
-        for (int attempt = 0; attempt < 2; ++attempt) {
-            // attempt 1, only where NaN made a thread's best no element: everything again, bound by nothing
-            for (int from = 0; from < owners * rounds; from += kLogprobThreads) {
-                const int i = from + tid, owner = i / rounds, piece = begin + (i - owner * rounds) * kLogprobThreads + (owner < owners ? (attempt ? owner : chosen[owner]) : 0);
-                if (owner < owners && piece < end) {
-                    const u32x4 v = pieces[piece];
+        auto piece_of = [&](int i, bool everybody) __attribute__((always_inline)) {         // -1: none
+            const int n = i >> 4, piece = n < owners ? begin + (everybody ? n : chosen[n]) * 16 + (i & 15) : end;
+            return piece < end ? piece : -1;
+        };
+        auto offer = [&](int piece, const u32x4& v) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const int index = piece * N + e - lead;
-                        const uint32_t order = logprob_order(Vec::at(v, e));
-                        if (index >= 0 && index < a.V && (static_cast<key64>(order) << 32 | static_cast<uint32_t>(~piece)) >= bound)
-                            keys[atomicAdd(&count_of, 1)] = static_cast<key64>(order) << 32 | static_cast<uint32_t>(~index);
-                    }
+            for (int e = 0; e < N; ++e) {
+                const int index = piece * N + e - lead;
+                const uint32_t order = logprob_order(Vec::at(v, e));
+                if (index >= 0 && index < a.V && (static_cast<key64>(order) << 32 | static_cast<uint32_t>(~((piece - begin) >> 4))) >= bound) {
+                    const int at = atomicAdd(&count_of, 1);
+                    if (at < kLogprobKeys) keys[at] = static_cast<key64>(order) << 32 | static_cast<uint32_t>(~index);
                 }
+            }
+        };
+        for (int from = 0; from < owners * 16; from += AHEAD * kLogprobThreads) {
+            int piece[AHEAD];
+            u32x4 v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                piece[i] = piece_of(from + i * kLogprobThreads + tid, false);
+                v[i] = pieces[max(piece[i], 0)];
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (piece[i] >= 0) offer(piece[i], v[i]);
+        }
+        __syncthreads();
+        // Again in rounds where LDS did not hold them, and without a bound where NaN made a block's best no element.
+        if (count_of > kLogprobKeys || count_of < want) {
+            const bool everybody = count_of < want;
+            __syncthreads();
+            if (tid == 0) count_of = 0;
+            if (everybody) bound = 0, owners = blocks;
+            __syncthreads();
+            for (int from = 0; from < owners * 16; from += kLogprobThreads) {
+                const int piece = piece_of(from + tid, everybody);
+                if (piece >= 0) offer(piece, pieces[piece]);
                 __syncthreads();
                 const int have = count_of;
                 __syncthreads();                                           // (all have read it before the next round counts on)
-                if (have > kLogprobSlack && from + kLogprobThreads < owners * rounds) {      // room for the next round: only the best stay
+                if (have > kLogprobSlack && from + kLogprobThreads < owners * 16) {      // room for the next round: only the best stay
                     if (tid < 64) {
                         const int n = logprob_compact(keys, have, logprob_bound(keys, have, want, lane), lane);
                         if (lane == 0) count_of = n;
@@ -302,12 +364,6 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
                     __syncthreads();
                 }
             }
-            if (count_of >= want) break;                                   // uniform: nobody writes it any more
-            __syncthreads();
-            if (tid == 0) count_of = 0;
-            bound = 0;
-            owners = kLogprobThreads;
-            __syncthreads();
         }
         if (tid < 64) logprob_best(keys, count_of, a.top, sorted, lane);
         __syncthreads();
