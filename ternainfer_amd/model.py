@@ -11,6 +11,9 @@ linear); RoPE + KV-cache write, single-token attention, the multi-token attentio
 pass, the LM head of a decode step and greedy sampling are library kernels too (the prompt pass projects
 its last rows through the LM head with a PyTorch-ROCm matmul); one decode step is captured in a HIP graph, as
 generate.py:204-224 does.
+
+Next to the bf16 cache, of up to 8192 slots for the kernels, stands one in 4 bits of any length (`Transformer.make_cache(..., bits=4)`), and
+`Transformer.score` gives the log probabilities of the tokens of a text.
 """
 from __future__ import annotations
 
@@ -25,6 +28,7 @@ from . import _lib
 from .linear import (EPILOGUE_GATE, EPILOGUE_RESIDUAL, argmax_rows, attention_merge_rmsnorm_linear_packed, fused_linear, get_global_workspace, greedy_step,
                      greedy_step_state, interleave_gate_up, lm_head, prompt_inputs, quant_from_stats, quant_input, row_stats, relu2_mul_rmsnorm_linear_packed, relu2_mul_rmsnorm_quant, step_inputs,
                      repack_weight, rmsnorm_linear_packed, rmsnorm_quant)
+from .long_context import Kv4Cache, TokenLogprobs, kv4_attention, kv4_step, kv4_store, rotary_frequencies, token_logprobs
 
 
 @dataclass
@@ -38,6 +42,7 @@ class ModelArgs:                      # model.py:23-34
     norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     rope_adjacent: bool = True        # pairs (2j, 2j+1), rope_padded's default (model.py:221-229); False = (j, j + D/2)
+    rope_scaling: Optional[dict] = None     # for contexts longer than the trained one: see long_context.rotary_frequencies
 
     @property
     def head_dim(self) -> int:
@@ -208,7 +213,15 @@ class Block:
         n = self.w13.n
         return rows > 16 and n != 3840 and (self.w13.ws_num == 1 or n % 256 == 0)
 
-    def forward_chain(self, x, stats, cache_k, cache_v, pos_idx, cos, sin, attn_ws, next_norm, split=False):
+    def attend_kv4(self, qkv, pos_idx, cache, inv_freq, amplitude):
+        """RoPE, cache write and attention over a cache in 4 bits: rows qkv [B*T, (H + 2 KV) D] -> [B*T, H D]."""
+        a = self.args
+        how = dict(amplitude=amplitude, adjacent=a.rope_adjacent)
+        if qkv.shape[0] == cache.k.shape[0]:
+            return kv4_step(qkv, pos_idx, inv_freq, cache, a.n_heads, **how)
+        return kv4_attention(kv4_store(qkv, pos_idx, inv_freq, cache, a.n_heads, **how), pos_idx, cache)
+
+    def forward_chain(self, x, stats, cache_k, cache_v, pos_idx, cos, sin, attn_ws, next_norm, split=False, kv4=None):
         """One new token per sequence (up to 16 sequences), the linears chained through producer-side norm statistics:
         `x` is the residual stream INCLUDING the previous block's FFN output and `stats` its partials under this block's
         attention_norm (None: the first block, which takes them inside).  Every linear's epilogue leaves what the next
@@ -217,7 +230,9 @@ class Block:
         partials under `next_norm` (the next block's attention_norm).  Returns (stream, partials).
         `split`: the producers are the same, but the norm + quantisation in front of QKV, gate+up and the down projection
         is a launch of its own from the partials (quant_from_stats: element-wise, no reduction over the row) and the
-        linears take the quantised rows -- for row counts at which every workgroup repeating that work costs more."""
+        linears take the quantised rows -- for row counts at which every workgroup repeating that work costs more.
+        `kv4` (cache, inv_freq, amplitude): the cache is one in 4 bits, whose `k` and `v` are given as cache_k and cache_v; cos, sin and attn_ws
+        are not read."""
         a = self.args
         bsz = cache_k.shape[0]
         lib = self.wqkv.lib
@@ -279,7 +294,9 @@ class Block:
                 r = fused_linear(o, self.attn_sub_norm, a.norm_eps, self.wo.packed, self.wo.ws, self.wo.ws_num, self.wo.n, self.wo.k, **o_kw)
         else:
             o_stats = None
-            if self.prefetch is not None:
+            if kv4 is not None:
+                o = self.attend_kv4(qkv, pos_idx, *kv4)
+            elif self.prefetch is not None:
                 o = torch.empty((bsz, a.n_heads * a.head_dim), dtype=torch.bfloat16, device=x.device)
                 ptrs, sizes, units, count = self.prefetch
                 lib.ternaspmm_rope_decode_attention_prefetch(
@@ -331,11 +348,12 @@ class Block:
         note("w2", r)
         return r[0], r[1]
 
-    def forward(self, x, pending, cache_k, cache_v, pos_idx, cos, sin, mask, attn_ws=None):
+    def forward(self, x, pending, cache_k, cache_v, pos_idx, cos, sin, mask, attn_ws=None, kv4=None):
         """x [B*T, dim] (T new tokens per sequence) and `pending`, the previous block's FFN output that
         has not been added to the stream yet (None for the first block): the add is part of this
         block's first fused kernel.  cache_* [B, n_kv, S, hd]; pos_idx int64 [T] cache slots shared by the
         sequences, or [B, T] with cos / sin [B*T, hd/2]: every sequence at its own positions (generate.py:253-262).
+        `kv4`: as in forward_chain; mask is not read either.
         Returns (stream, pending) for the next block; pending None where the down projection has added its output to the stream."""
         a = self.args
         bsz = cache_k.shape[0]
@@ -343,7 +361,7 @@ class Block:
         per_seq = int(pos_idx.dim() == 2)
         one_token = mask is None           # the caller's rule: fused, one new token, a head size the kernel has
         # more rows than _norm_linear's one-launch forms take: the launches of the block as one native call
-        if x.shape[0] > 8 and self.fused and self.act == "int8" and self.capture is None and \
+        if x.shape[0] > 8 and self.fused and self.act == "int8" and self.capture is None and kv4 is None and \
                 (mask is KERNEL_ATTENTION or (one_token and self.prefetch is None)):
             wqkv, wo, w13, w2 = self.wqkv, self.wo, self.w13, self.w2
             return _lib.native().block(
@@ -357,7 +375,9 @@ class Block:
         native = _lib.native()
         attend = (qkv, cos, sin, pos_idx, cache_k, cache_v, a.n_heads, a.head_dim, a.head_dim ** -0.5, int(a.rope_adjacent))
         deferred = one_token and isinstance(attn_ws, tuple)
-        if deferred:
+        if kv4 is not None:
+            o = self.attend_kv4(qkv, pos_idx, *kv4)
+        elif deferred:
             # the cache prefix of every head split over several workgroups that leave partial results; the O
             # projection's prologue merges them (one sequence; else a merge launch): the launch boundary is the synchronisation
             # (no prefetch regions here: this launch is shorter than the prefetch of the following weights would be --
@@ -397,7 +417,7 @@ class Block:
             else:
                 cache_k.index_copy_(2, pos_idx, k)
                 cache_v.index_copy_(2, pos_idx, v)
-        if not one_token and mask is not KERNEL_ATTENTION:
+        if not one_token and mask is not KERNEL_ATTENTION and kv4 is None:
             kk = cache_k.repeat_interleave(rep, dim=1)
             vv = cache_v.repeat_interleave(rep, dim=1)
             o = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
@@ -525,10 +545,22 @@ class Transformer:
         tables = getattr(self, "_rope_tables", None)
         if tables is None or tables[0] != key:
             a = self.args
+            if a.rope_scaling is not None:
+                inv, amplitude = rotary_frequencies(a.head_dim, a.rope_theta, a.rope_scaling, dev)
+                ang = torch.arange(max_seq, device=dev, dtype=torch.float64)[:, None] * inv[None, :]
+                self._rope_tables = (key, (torch.stack([ang.cos(), ang.sin()], dim=1) * amplitude).float().contiguous())
+                return self._rope_tables[1]
             inv = 1.0 / (a.rope_theta ** (torch.arange(0, a.head_dim, 2, device=dev, dtype=torch.float32) / a.head_dim))
             ang = torch.arange(max_seq, device=dev, dtype=torch.float32)[:, None] * inv[None, :]
             self._rope_tables = tables = (key, torch.stack([ang.cos(), ang.sin()], dim=1).contiguous())
         return tables[1]
+
+    def rope_frequencies(self, dev):
+        """(inv_freq, amplitude) of the rotary positions, as the 4-bit cache's kernels take them; kept: a captured step holds the pointer."""
+        held = getattr(self, "_rope_frequencies", None)
+        if held is None or held[0].device != dev:
+            self._rope_frequencies = held = rotary_frequencies(self.args.head_dim, self.args.rope_theta, self.args.rope_scaling, dev)
+        return held
 
     def attention_partial(self, bsz: int, max_seq: int, single_split: bool = False):
         """(buffer, splits) for the decode step whose attention leaves the merge of its splits to the consumer of its
@@ -585,8 +617,17 @@ class Transformer:
         return _lib.native().decode_step(tokens, pos_idx.reshape(-1), self.tok_embeddings, self.rope_tables(max_seq, tokens.device), a.n_heads, a.head_dim,
                                          a.head_dim ** -0.5, a.norm_eps, splits, blocks)
 
-    def make_cache(self, bsz: int, max_seq: int):
+    def make_cache(self, bsz: int, max_seq: int, bits: int = 16):
+        """The key/value cache of every block, for bsz sequences of max_seq tokens.  bits=4: `Kv4Cache`s, 4.25 bits a value and any length (heads of 64 or
+        128 dimensions, up to 16 query heads each); it needs the fused kernels, and a step is its launches, never one (whole_step).
+        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 653 and
+        994, of 8192 1067 and 1077, of 131072 1941 in 4; 8 of 1528 1132 and 1295, of 8192 1725 and 1747; 16 of 8192 2657 and 2113; 32 of 8192 4387 and
+        3188.  A prompt of 8192 tokens 30.8 and 27.8 ms, of 32768 222 in 4."""
         a = self.args
+        if bits == 4:
+            return [Kv4Cache.empty(bsz, a.n_kv_heads, max_seq, a.head_dim, self.tok_embeddings.device) for _ in range(a.n_layers)]
+        if bits != 16:
+            raise ValueError(f"make_cache: 4 or 16 bits, not {bits}")
         shape = (bsz, a.n_kv_heads, max_seq, a.head_dim)
         dev = self.tok_embeddings.device
         return [(torch.zeros(shape, dtype=torch.bfloat16, device=dev), torch.zeros(shape, dtype=torch.bfloat16, device=dev))
@@ -598,21 +639,40 @@ class Transformer:
         of the last new token -- of new token last_idx[b] of sequence b when `last_idx` (int64 [B]) is given: the
         prompt pass of prompts padded to one length.  `trace`, if given, is called after every block as
         trace(index, stream_in, pending_in, stream_out, pending_out) (layer-by-layer checks against a golden)."""
+        bsz, t = tokens.shape
+        x, pending = self.stream(tokens, cache, pos_idx, trace, last_idx is None)
+        if last_idx is not None:                                              # padded prompts: each sequence's own last token
+            pick = torch.arange(bsz, device=tokens.device) * t + last_idx
+            x, pending = x.index_select(0, pick), None if pending is None else pending.index_select(0, pick)
+        elif t > 1:                                                           # only the last new token feeds the head
+            x, pending = (None if y is None else y.view(bsz, t, self.args.dim)[:, -1].contiguous() for y in (x, pending))
+        return self.head(x, pending, bsz)
+
+    def stream(self, tokens, cache, pos_idx, trace=None, whole=True):
+        """The residual stream [B*T, dim] behind the last block, and the part of it that has not been added yet (or None): what `forward` projects.
+        `whole`: a single-token step may be one launch."""
         a = self.args
         bsz, t = tokens.shape
         max_seq = cache[0][0].shape[2]
         dev = tokens.device
         mask = None
-        kernels_fit = self.layers[0].fused and a.head_dim in (64, 128) and max_seq <= 8192 and tokens.is_cuda
+        four = isinstance(cache[0], Kv4Cache)
+        if four and not (self.layers[0].fused and tokens.is_cuda):
+            raise ValueError("a cache in 4 bits: only with the fused kernels, on a GPU")
+        kv4 = self.rope_frequencies(dev) if four else None
+        kernels_fit = self.layers[0].fused and a.head_dim in (64, 128) and (four or max_seq <= 8192) and tokens.is_cuda
         one_launch_attention = kernels_fit and t == 1
         # one new token for a few sequences: the linears chained through producer-side norm statistics (forward_chain)
         chain = one_launch_attention and self.layers[0].act == "int8" and bsz <= max(self.chain_rows, self.split_rows) and getattr(self, "chain", True) and self.chain_supported()
         stats = None
-        if chain and trace is None and last_idx is None:
+        if chain and trace is None and whole and not four:
             x = self.whole_step(tokens, cache, pos_idx, max_seq)
             if x is not None:                                                 # the blocks of the step in one launch
-                return self.head(x, None, bsz)
-        if chain and getattr(self, "step_inputs", True):
+                return x, None
+        if four:                                                              # no tables: the kernels form the angles
+            cos = sin = None
+            x = self.tok_embeddings[tokens.reshape(-1)]
+        elif chain and getattr(self, "step_inputs", True):
             # embedding rows, their partials under the first block's norm and the RoPE rows of the positions: one launch
             x, stats, cos, sin = step_inputs(tokens, pos_idx.reshape(-1), self.tok_embeddings, self.rope_tables(max_seq, dev), self.layers[0].attention_norm)
         elif kernels_fit and getattr(self, "step_inputs", True) and a.dim % 8 == 0:
@@ -621,14 +681,16 @@ class Transformer:
             rows = self.rope_tables(max_seq, dev).index_select(0, pos_idx.reshape(-1))   # fp32 [T | B*T, 2, head_dim / 2]
             cos, sin = rows[:, 0].contiguous(), rows[:, 1].contiguous()       # views when one row
             x = self.tok_embeddings[tokens.reshape(-1)]
-        if kernels_fit and t > 1 and getattr(self, "kernel_prefill_attention", True):
+        if four:
+            pass
+        elif kernels_fit and t > 1 and getattr(self, "kernel_prefill_attention", True):
             mask = KERNEL_ATTENTION
         elif not one_launch_attention:
             # causal over cache slots: new token at slot p sees slots <= p
             seen = torch.arange(max_seq, device=dev) <= pos_idx[..., None]    # [T | B, T][S]
             mask = seen[:, None] if pos_idx.dim() == 2 else seen[None, None]
         pending = None
-        attn_ws = self.attention_workspace(bsz) if one_launch_attention else None     # layers run one after another: shared
+        attn_ws = self.attention_workspace(bsz) if one_launch_attention and not four else None     # layers run one after another: shared
         split = chain and bsz > self.chain_rows
         # Split attention whose merge is left to its consumer: always for one sequence (the O projection's prologue merges); for more, where the
         # attention is shorter by more than the merge launch costs.  That launch also norms and quantises the O projection's rows, which unsplit
@@ -639,36 +701,63 @@ class Transformer:
         # on, where both are level: 14 at 384 1320 -> 1217 and 1409 -> 1240, 16 at 384 1331 -> 1227 and 1415 -> 1249, 20 at 512 1654 -> 1466 and 1712 ->
         # 1516.  `split_merge_quant`: the split form of 9 to 16 sequences whatever the length.
         short = 256 if bsz * a.n_heads > 256 else 512 if chain and bsz > 4 else self.defer_above
-        if one_launch_attention and self.layers[0].act == "int8" and (bsz == 1 or max_seq > short):
+        if four:
+            pass
+        elif one_launch_attention and self.layers[0].act == "int8" and (bsz == 1 or max_seq > short):
             attn_ws = self.attention_partial(bsz, max_seq) or attn_ws
         elif split and getattr(self, "split_merge_quant", False):
             attn_ws = self.attention_partial(bsz, max_seq, single_split=True) or attn_ws
-        for index, (layer, (ck, cv)) in enumerate(zip(self.layers, cache)):
+        for index, (layer, held) in enumerate(zip(self.layers, cache)):
             x_in, pending_in = x, pending
+            ck, cv = (held.k, held.v) if four else held
+            in4 = (held, *kv4) if four else None
             if chain:
                 nxt = self.layers[index + 1].attention_norm if index + 1 < len(self.layers) else self.norm
-                x, stats = layer.forward_chain(x, stats, ck, cv, pos_idx, cos, sin, attn_ws, nxt, split=split)
+                x, stats = layer.forward_chain(x, stats, ck, cv, pos_idx, cos, sin, attn_ws, nxt, split=split, kv4=in4)
             else:
-                x, pending = layer.forward(x, pending, ck, cv, pos_idx, cos, sin, mask, attn_ws)
+                x, pending = layer.forward(x, pending, ck, cv, pos_idx, cos, sin, mask, attn_ws, kv4=in4)
             if trace is not None:
                 trace(index, x_in, pending_in, x, pending)
-        if last_idx is not None:                                              # padded prompts: each sequence's own last token
-            pick = torch.arange(bsz, device=dev) * t + last_idx
-            x, pending = x.index_select(0, pick), None if pending is None else pending.index_select(0, pick)
-        elif t > 1:                                                           # only the last new token feeds the head
-            x, pending = x.view(bsz, t, a.dim)[:, -1].contiguous(), None if pending is None else pending.view(bsz, t, a.dim)[:, -1].contiguous()
-        return self.head(x, pending, bsz)
+        return x, pending
 
     def head(self, x, pending, bsz):
         """Logits of the rows x (+ pending): last residual add, final norm, LM head."""
         a = self.args
-        if self.layers[0].fused and x.is_cuda:                                # last residual add + final norm: one launch
-            x, _ = rmsnorm_quant(x, self.norm, a.norm_eps, residual=pending, quant=False)     # (pending None: the stream has it)
-        else:
-            x = rms_norm(x + pending, self.norm, a.norm_eps)
+        x = self.final_norm(x, pending)
         if x.is_cuda and bsz <= 16 and a.dim % 32 == 0 and bsz * (2 * a.dim + 16) <= 160 * 1024:
             return lm_head(x, self.tok_embeddings)                            # tied LM head (model.py:367): one HBM-bound pass
         return F.linear(x, self.tok_embeddings)
+
+    def final_norm(self, x, pending):
+        """The rows that the LM head takes: last residual add and final norm."""
+        a = self.args
+        if self.layers[0].fused and x.is_cuda:                                # one launch
+            return rmsnorm_quant(x, self.norm, a.norm_eps, residual=pending, quant=False)[0]     # (pending None: the stream has it)
+        return rms_norm(x + pending, self.norm, a.norm_eps)
+
+    score_rows = 1024              # rows of logits that `score` holds at a time (1024 x 128256 in bf16: 263 MB)
+
+    @torch.inference_mode()
+    def score(self, tokens: torch.Tensor, lens: Optional[torch.Tensor] = None, top: int = 0, kv_bits: int = 16) -> TokenLogprobs:
+        """Log probabilities of the tokens of a text under the model, in one pass over it: tokens int64 [B, T] -> `TokenLogprobs` whose fields are
+        [B, T - 1] (and [B, T - 1, top]), entry i for token i + 1 after tokens 0 .. i.  `lens` (int64 [B], each 1 .. T): the texts have different lengths
+        and are padded to T with any token; the log probabilities of padding are NaN."""
+        a = self.args
+        bsz, t = tokens.shape
+        if t < 2:
+            raise ValueError("score: a text of at least two tokens")
+        if lens is not None and tuple(lens.shape) != (bsz,):
+            raise ValueError("score: one length a text")
+        dev = tokens.device
+        x, pending = self.stream(tokens[:, :-1].contiguous(), self.make_cache(bsz, t - 1, kv_bits), torch.arange(t - 1, device=dev), whole=False)
+        targets = tokens[:, 1:].contiguous()
+        if lens is not None:
+            targets = targets.masked_fill(torch.arange(1, t, device=dev) >= lens.to(dev)[:, None], -1)
+        targets, h = targets.view(-1), self.final_norm(x, pending)
+        parts = [token_logprobs(F.linear(h[i:i + self.score_rows], self.tok_embeddings), targets[i:i + self.score_rows], top)
+                 for i in range(0, h.shape[0], self.score_rows)]
+        join = lambda field: None if field[0] is None else torch.cat(field).view(bsz, t - 1, *field[0].shape[1:])
+        return TokenLogprobs(*map(join, zip(*parts)))
 
 
 def _greedy_steps(step, count: int, use_graph: bool) -> float:
@@ -696,16 +785,19 @@ def _greedy_steps(step, count: int, use_graph: bool) -> float:
 
 
 @torch.inference_mode()
-def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use_graph: bool = True, prompt_lens=None):
+def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use_graph: bool = True, prompt_lens=None, kv_bits: int = 16,
+                  logprobs: Optional[int] = None):
     """Prefill `prompt` [B, P], then `gen_tokens` greedy steps.  Returns (tokens [B, gen_tokens],
     prefill seconds, decode seconds).  The decode step (model forward + argmax + position bump) is
     captured once and replayed (`_greedy_steps`).
     `prompt_lens` (int64 [B], each 1 .. P): the prompts have different lengths and are padded to P with any token
     (generate.py:244-262): sequence b's first generated token comes from its prompt token prompt_lens[b] - 1, and
     its n-th decode step runs at cache slot prompt_lens[b] + n -- every sequence at its own position.  A padding token's
-    cache rows are overwritten by the decode steps before any query can see them."""
+    cache rows are overwritten by the decode steps before any query can see them.
+    `kv_bits` 4: the cache in 4 bits (Transformer.make_cache).  `logprobs` (0 .. 64): a fourth result, the `TokenLogprobs` of the generated tokens,
+    [B, gen_tokens], with so many alternatives each."""
     bsz, plen = prompt.shape
-    cache = model.make_cache(bsz, plen + gen_tokens)
+    cache = model.make_cache(bsz, plen + gen_tokens, kv_bits)
     slots = torch.arange(plen, device="cuda")
     ragged = prompt_lens is not None
     if ragged:
@@ -721,11 +813,28 @@ def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use
     out = torch.empty((bsz, gen_tokens), dtype=torch.int64, device="cuda")
     out[:, 0:1] = tok
     state = greedy_step_state(bsz)
+    history = None
+    if logprobs is not None:
+        first = token_logprobs(logits, tok.view(-1), logprobs)
+        # (the last step's token is behind the generated ones: a column of its own, as the token itself finds no room in `out`)
+        history = TokenLogprobs(*[None if f is None else f.new_empty((bsz, gen_tokens + 1, *f.shape[1:])) for f in first])
+
+    def note(scores, index):                                                  # index int64 [1]: on the device, a captured step's own
+        for kept, f in zip(history, scores):
+            if kept is not None:
+                kept.index_copy_(1, index, f[:, None])
+
+    if history is not None:
+        note(first, counters[1:2] - 1)
 
     def step():                                                               # the forward has read tok by the time it changes
-        greedy_step(model.forward(tok, cache, pos), tok, out, counters, state)
+        step_logits = model.forward(tok, cache, pos)
+        greedy_step(step_logits, tok, out, counters, state)
+        if history is not None:                                               # (the counter is one past the token just stored)
+            note(token_logprobs(step_logits, tok.view(-1), logprobs), counters[1:2] - 1)
         if ragged:
             pos.add_(1)
 
     seconds = _greedy_steps(step, gen_tokens, use_graph)
-    return out, ev[0].elapsed_time(ev[1]) * 1e-3, seconds
+    result = out, ev[0].elapsed_time(ev[1]) * 1e-3, seconds
+    return result if history is None else (*result, TokenLogprobs(*[None if f is None else f[:, :gen_tokens] for f in history]))

@@ -150,3 +150,26 @@ def test_python_functions_refuse_tensors_that_are_not_on_the_gpu():
             call()
     with pytest.raises(TypeError):
         T.token_logprobs([1.0])
+
+
+def test_the_model_refuses_what_its_cache_does_not_take():
+    from ternainfer_amd.model import ModelArgs, Transformer
+    model = Transformer.__new__(Transformer)
+    model.args = ModelArgs(dim=256, n_layers=2, n_heads=4, n_kv_heads=2)
+    model.tok_embeddings = torch.zeros((10, 256), dtype=torch.bfloat16)
+    assert [tuple(t.shape) for t in model.make_cache(2, 9, bits=4)[1]] == [(2, 2, 9, 32), (2, 2, 9, 2)] * 2
+    assert [tuple(t.shape) for t in model.make_cache(2, 9)[1]] == [(2, 2, 9, 64)] * 2
+    for bits in (0, 8, "4"):
+        with pytest.raises(ValueError):
+            model.make_cache(2, 9, bits=bits)
+    model.args.n_heads = 8                       # heads of 32 dimensions
+    with pytest.raises(ValueError):
+        model.make_cache(2, 9, bits=4)
+    model.args.n_heads = 4
+    layer = type("Layer", (), {"fused": True})()
+    model.layers = [layer]
+    with pytest.raises(ValueError):              # no GPU
+        model.forward(torch.zeros((2, 1), dtype=torch.int64), model.make_cache(2, 9, bits=4), torch.arange(1))
+    for tokens, lens in ((torch.zeros((2, 1), dtype=torch.int64), None), (torch.zeros((2, 4), dtype=torch.int64), torch.ones(3))):
+        with pytest.raises(ValueError):
+            model.score(tokens, lens)
