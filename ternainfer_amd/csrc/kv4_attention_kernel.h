@@ -30,8 +30,9 @@ constexpr float kKv4Held = -26.0f;             // a row's largest probability is
 
 // Values and probabilities in fp16: a value is a code times a power of two, exact in fp16 for scale bytes 104 .. 140 (2^-23 .. 2^13); probabilities keep 11 bits, held
 // at 2^12 for a row's running maximum -- up to 2^15 where a larger score has not raised it yet -- so that those 2^-26 of it are still normal numbers.  Any
-// other scale marks the workgroup, which starts again with bf16 values and probabilities in two bf16, the products twice.
+// other scale of a group that is not all zeros marks the workgroup, which starts again with bf16 values and probabilities in two bf16, the products twice.
 constexpr uint32_t kKv4HalfLow = 104, kKv4HalfHigh = 140;
+constexpr uint32_t kKv4Magnitudes = 0x77777777u;           // the bits of eight codes that make them no zeros
 constexpr float kKv4HeldHalf = 12.0f, kKv4Growth = 3.0f;
 
 __device__ __forceinline__ u32x4 kv4_values_half(uint32_t codes, float scale)
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
                         broken = min(broken, k0 + row);
                         byte = 127u;
                     }
-                    if (HALF) wide |= byte < kKv4HalfLow || byte > kKv4HalfHigh;
+                    if (HALF) wide |= (byte < kKv4HalfLow || byte > kKv4HalfHigh) && ((x.v[i][0] | x.v[i][1] | x.v[i][2] | x.v[i][3]) & kKv4Magnitudes) != 0;
                     byte = min(byte, HALF ? kKv4HalfHigh : kKv4MaxByte);
                 }
                 const float vs = __uint_as_float(byte << 23);

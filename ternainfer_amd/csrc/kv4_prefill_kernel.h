@@ -193,7 +193,10 @@ __device__ __forceinline__ bool kv4_prefill(const Kv4Attention& a, uint8_t* smem
             byte = 127u;
         }
         if (HALF) {
-            wide |= byte < kKv4HalfLow || byte > kKv4HalfHigh;
+            uint32_t codes = v_codes[0];
+#pragma unroll
+            for (int i = 1; i < WORDS; ++i) codes |= v_codes[i];
+            wide |= (byte < kKv4HalfLow || byte > kKv4HalfHigh) && (codes & kKv4Magnitudes) != 0;
             byte = min(byte, kKv4HalfHigh);
         } else {
             byte = min(byte, kKv4MaxByte);

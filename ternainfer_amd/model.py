@@ -620,9 +620,9 @@ class Transformer:
     def make_cache(self, bsz: int, max_seq: int, bits: int = 16):
         """The key/value cache of every block, for bsz sequences of max_seq tokens.  bits=4: `Kv4Cache`s, 4.25 bits a value and any length (heads of 64 or
         128 dimensions, up to 16 query heads each); it needs the fused kernels, and a step is its launches, never one (whole_step).
-        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 653 and
-        994, of 8192 1067 and 1077, of 131072 1941 in 4; 8 of 1528 1132 and 1295, of 8192 1725 and 1747; 16 of 8192 2657 and 2113; 32 of 8192 4387 and
-        3188.  A prompt of 8192 tokens 30.8 and 27.8 ms, of 32768 222 in 4."""
+        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 651 and
+        898, of 8192 1066 and 1010, of 131072 1516 in 4; 8 of 1528 1129 and 1214, of 8192 1724 and 1442; 16 of 8192 2660 and 1717; 32 of 8192 4427 and
+        2393.  A prompt of 2048 tokens 6.3 and 6.8 ms, of 8192 28.9 and 26.2, of 32768 200 in 4."""
         a = self.args
         if bits == 4:
             return [Kv4Cache.empty(bsz, a.n_kv_heads, max_seq, a.head_dim, self.tok_embeddings.device) for _ in range(a.n_layers)]

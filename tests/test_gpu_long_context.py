@@ -350,6 +350,14 @@ def test_attention_over_scales_from_end_to_end(t, d):
         one = T.Kv4Cache(*(c.clone() for c in cache))
         one.v_scale[0, 1, 77, 0] = byte
         _attend(q, pos, one)
+    # groups of zeros, as the store leaves them: the smallest scale, codes 0 and -0; alone and with one of another value among them
+    zeros = T.Kv4Cache(*(c.clone() for c in cache))
+    for slot in (0, 5, 31, 150, 299):
+        zeros.v[0, :, slot] = 0x80 if slot % 2 else 0x08
+        zeros.v_scale[0, :, slot] = 2
+    _attend(q, pos, zeros)
+    zeros.v[0, 0, 150, 3] = 0x70
+    _attend(q, pos, zeros)
     low = T.Kv4Cache(*(c.clone() for c in cache))
     low.k_scale.copy_(torch.randint(2, 128, cache.k_scale.shape, generator=_gen(77), device="cuda", dtype=torch.uint8))
     _attend(q, pos, low)
