@@ -730,7 +730,7 @@ int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* po
 /* Of M rows of V logits (bf16, or fp32; `row` elements apart): logprob fp32 [M] of targets int64 [M] (NaN for one outside [0, V); both may be NULL),
  * entropy fp32 [M] in nats, and the `top` (0 .. 64, at most V) largest: ids int64 [M][top], by value, equal values by lower index, NaN last, with
  * their log probabilities.  A row with NaN or +inf, or of -inf alone, has no distribution: its probabilities and entropy are NaN.
- * V up to 2^22.  workspace: ternaspmm_token_logprobs_workspace_bytes, 8-byte aligned; NULL: slower for few rows, not taken for V above 262000 (fp32: 131000). */
+ * V up to 2^19.  workspace: ternaspmm_token_logprobs_workspace_bytes, 4-byte aligned; NULL: slower for few rows. */
 long long ternaspmm_token_logprobs_workspace_bytes(int M, int V, int fp32, int top);
 int ternaspmm_token_logprobs(const void* logits, long long row, int fp32, const long long* targets, float* logprob, float* entropy, long long* top_ids,
                              float* top_logprobs, int top, void* workspace, int M, int V, terna_stream stream);

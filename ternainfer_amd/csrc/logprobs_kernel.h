@@ -7,16 +7,19 @@
 // 0 * inf does not arise.
 //
 // Alternatives without a second pass over everything.  Elements are in order by (value, lower index first) as 64-bit keys; NaN below all.  Sixteen lanes' pieces
-// are a block of 256 contiguous bytes, whose largest value goes to LDS (four permutations and a store for about 80 other instructions).  If T is a bound that
-// k blocks' bests reach, k elements reach T, so the k best elements do, and they lie in blocks whose best reaches T: those alone are read again, elements
-// that reach T go to LDS, and the k best of these are found by counting.  The order in which they arrive there does not matter.
+// are a block of 256 contiguous bytes -- a wave's, 1024 bytes, where those would be more than LDS has room for --, whose largest value is kept (four permutations
+// and a store for about 80 other instructions).  If T is a bound that k blocks' bests reach, k elements reach T, so the k best elements do, and they lie in
+// blocks whose best reaches T: those alone are read again, elements that reach T go to LDS, and the k best of these are found by counting.  The order in
+// which they arrive there does not matter.  Where a row is split, the launch that merges its parts does this, once a row (each part finding its own k best
+// first: 8 rows of 128256 with 20 alternatives 18.2 us, so 13.5).  Bests and the bound they give are every wave's work: with one wave's, one row took 11.8 us, so 9.3.
 // T is the k-th best of 64 (for k > 32: of 256) bests of blocks taken together, by bisection over the keys' bits, a ballot a bit, which ends as soon as exactly
 // k reach it (10 - 15 rounds where values differ); about 1.2 k blocks reach it.  Elements go to LDS in one sweep; only where they are more than it holds are
 // they taken again in rounds, with the best k kept from each to the next.  (Blocks and not, say, the pieces of a thread: those are 4 KB apart, and the
 // second reading of the few that matter took three quarters of the row's lines, 17 us of 70 for 1024 x 128256.)
 //
-// What bounds it: many rows -- memory (vector work: 11 issue slots an element against 64 a clock and CU); one row -- two launches (the row split over
-// workgroups, then merged), a trip to memory each and the selection of the alternatives.
+// What bounds it: many rows -- memory (1024 x 128256 in bf16, 263 MB: 49.7 us without alternatives, 5.3 TB/s; the blocks' bests 7 more, 20 alternatives 4 more;
+// two pieces a thread ahead: 4 were 3 us slower, 1 12); one row -- two launches (the row split over workgroups, then merged), a trip to memory each (5.1 us)
+// and the selection of the alternatives (4.2).
 #pragma once
 
 #include <type_traits>
@@ -30,7 +33,7 @@ constexpr int kLogprobMaxTop = 64;
 constexpr int kLogprobBatch = 2048;            // elements that one round over the pieces can add
 constexpr int kLogprobSlack = 512;             // kept between rounds
 constexpr int kLogprobKeys = kLogprobBatch + kLogprobSlack;
-constexpr int kLogprobBlocks = 2048;           // of a workgroup: 16 pieces each
+constexpr int kLogprobBlocks = 2056;           // of a row
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef unsigned long long key64;
@@ -93,9 +96,33 @@ struct LogprobArgs {
     float *logprob, *entropy;                  // [M]
     long long* top_ids;                        // [M][top]
     float* top_logprobs;
-    void* partial;                             // splits > 1: key64 [M][splits][top], then LogprobStats [M][splits]
+    float* partial;                            // splits > 1: LogprobStats [M][splits], then, where top > 0, the blocks' bests fp32 [M][blocks]
     long long ld;
-    int M, V, top, splits;
+    int M, V, top, splits, blocks, shift;      // a block: 2^shift pieces, 16 or 64
+};
+
+// The row as whole 16-byte pieces, its own first and last elements somewhere in the first and last of them: a piece that holds an element of the row lies in
+// the allocation that does.
+template <typename T>
+struct LogprobRow {
+    static constexpr int N = LogprobVector<T>::N;
+    const u32x4* pieces;
+    int lead, all;
+    __device__ __forceinline__ LogprobRow(const LogprobArgs& a, int row)
+    {
+        const T* first = static_cast<const T*>(a.logits) + row * a.ld;
+        lead = static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / sizeof(T));
+        pieces = reinterpret_cast<const u32x4*>(first - lead);
+        all = (lead + a.V + N - 1) / N;
+    }
+};
+
+struct LogprobSelection {
+    key64 keys[kLogprobKeys];
+    key64 sorted[kLogprobMaxTop], most[kLogprobThreads];
+    float best[kLogprobBlocks];
+    uint16_t chosen[kLogprobBlocks];
+    int count, chosen_count;
 };
 
 // How many of `n` keys in LDS reach `bound`: one wave.
@@ -197,30 +224,113 @@ __device__ __forceinline__ LogprobStats logprob_join_all(LogprobStats s, Logprob
     return logprob_join(logprob_join(part[0], part[1]), logprob_join(part[2], part[3]));
 }
 
+// The row's a.top best elements into h.sorted, from the blocks' bests in h.best (behind a barrier).  The whole workgroup.
+template <typename T>
+__device__ __forceinline__ void logprob_select(const LogprobArgs& a, const LogprobRow<T>& x, LogprobSelection& h)
+{
+    using Vec = LogprobVector<T>;
+    constexpr int N = Vec::N, AHEAD = 2;
+    const int tid = threadIdx.x, lane = tid & 63, size = 1 << a.shift, blocks = (x.all + size - 1) >> a.shift;
+    if (tid == 0) h.count = 0, h.chosen_count = 0;
+    auto block_key = [&](int block) __attribute__((always_inline)) {
+        return static_cast<key64>(logprob_order(h.best[block])) << 32 | static_cast<uint32_t>(~block);
+    };
+    key64 bound = 0;
+    for (int i = tid; i < blocks; i += kLogprobThreads) bound = max(bound, block_key(i));
+    h.most[tid] = bound;
+    __syncthreads();
+    key64 most[4];                                                         // (every wave finds the bound for itself)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) most[n] = h.most[64 * n + lane];
+    if (a.top > 32) {
+        bound = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const key64 next = bound | 1ull << bit;
+            int count = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) count += __popcll(__ballot(most[n] >= next));
+            if (count >= a.top) bound = next;
+            if (count == a.top) break;
+        }
+    } else {
+        bound = logprob_bound64(max(max(most[0], most[1]), max(most[2], most[3])), a.top);
+    }
+    for (int i = tid; i < blocks; i += kLogprobThreads)
+        if (block_key(i) >= bound) h.chosen[atomicAdd(&h.chosen_count, 1)] = static_cast<uint16_t>(i);
+    __syncthreads();
+    int owners = h.chosen_count;
+    auto piece_of = [&](int i, bool everybody) __attribute__((always_inline)) {             // -1: none
+        const int n = i >> a.shift, piece = n < owners ? (everybody ? n : h.chosen[n]) << a.shift | (i & (size - 1)) : x.all;
+        return piece < x.all ? piece : -1;
+    };
+    auto offer = [&](int piece, const u32x4& v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int index = piece * N + e - x.lead;
+            const uint32_t order = logprob_order(Vec::at(v, e));
+            if (index >= 0 && index < a.V && (static_cast<key64>(order) << 32 | static_cast<uint32_t>(~(piece >> a.shift))) >= bound) {
+                const int at = atomicAdd(&h.count, 1);
+                if (at < kLogprobKeys) h.keys[at] = static_cast<key64>(order) << 32 | static_cast<uint32_t>(~index);
+            }
+        }
+    };
+    for (int from = 0; from < owners << a.shift; from += AHEAD * kLogprobThreads) {
+        int piece[AHEAD];
+        u32x4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            piece[i] = piece_of(from + i * kLogprobThreads + tid, false);
+            v[i] = x.pieces[max(piece[i], 0)];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (piece[i] >= 0) offer(piece[i], v[i]);
+    }
+    __syncthreads();
+    // Again in rounds where LDS did not hold them, and without a bound where NaN made a block's best no element.
+    if (h.count > kLogprobKeys || h.count < a.top) {
+        const bool everybody = h.count < a.top;
+        __syncthreads();
+        if (tid == 0) h.count = 0;
+        if (everybody) bound = 0, owners = blocks;
+        __syncthreads();
+        for (int from = 0; from < owners << a.shift; from += kLogprobThreads) {
+            const int piece = piece_of(from + tid, everybody);
+            if (piece >= 0) offer(piece, x.pieces[piece]);
+            __syncthreads();
+            const int have = h.count;
+            __syncthreads();                                               // (all have read it before the next round counts on)
+            if (have > kLogprobSlack && from + kLogprobThreads < owners << a.shift) {      // room for the next round: only the best stay
+                if (tid < 64) {
+                    const int n = logprob_compact(h.keys, have, logprob_bound(h.keys, have, a.top, lane), lane);
+                    if (lane == 0) h.count = n;
+                }
+                __syncthreads();
+            }
+        }
+    }
+    if (tid < 64) logprob_best(h.keys, h.count, a.top, h.sorted, lane);
+    __syncthreads();
+}
+
 template <typename T>
 __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(LogprobArgs a)
 {
     using Vec = LogprobVector<T>;
-    constexpr int N = Vec::N, AHEAD = 4;
-    __shared__ key64 keys[kLogprobKeys];
-    __shared__ key64 sorted[kLogprobMaxTop];
+    constexpr int N = Vec::N, AHEAD = 2;
+    __shared__ LogprobSelection h;
     __shared__ LogprobStats part[kLogprobThreads / 64];
-    __shared__ float best[kLogprobBlocks];
-    __shared__ uint16_t chosen[kLogprobBlocks];
-    __shared__ key64 bound_of;
-    __shared__ int count_of, chosen_count;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
-    // The row as whole 16-byte pieces, its own first and last elements somewhere in the first and last of them: a piece that holds an element of the
-    // row lies in the allocation that does.
-    const T* first = static_cast<const T*>(a.logits) + row * a.ld;
-    const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / sizeof(T));
-    const u32x4* pieces = reinterpret_cast<const u32x4*>(first - lead);
-    const int all = (lead + a.V + N - 1) / N, share = (all + a.splits - 1) / a.splits;
+    const LogprobRow<T> line(a, row);
+    const int lead = line.lead, all = line.all;
+    const u32x4* pieces = line.pieces;
+    const int share = ((all + a.splits - 1) / a.splits + 63) & ~63;        // whole blocks
     const int begin = split * share, end = min(begin + share, all);
     const int inside_from = lead ? 1 : 0, inside_to = (lead + a.V) / N;    // pieces of the row's elements alone
+    float* bests = a.partial + 3 * static_cast<size_t>(a.M) * a.splits + static_cast<size_t>(row) * a.blocks;
 
-    const int rounds = max(0, (end - begin + kLogprobThreads - 1) / kLogprobThreads), blocks = max(0, (end - begin + 15) / 16);
+    const int rounds = max(0, (end - begin + kLogprobThreads - 1) / kLogprobThreads);
     LogprobStats s{-INFINITY, 0.0f, 0.0f};
     auto take = [&](int round, const u32x4& v) __attribute__((always_inline)) {            // (all lanes, for the blocks' sake)
         const int piece = begin + round * kLogprobThreads + tid;
@@ -238,8 +348,9 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
 #pragma unroll
         for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
         if (a.top > 0) {
-            const float block = logprob_row(top, [](float p, float q) { return fmaxf(p, q); });
-            if ((tid & 15) == 0 && piece < end) best[(piece - begin) >> 4] = block;
+            float block = logprob_row(top, [](float p, float q) { return fmaxf(p, q); });
+            if (a.shift == 6) block = cross_row_reduce<true>(block);
+            if ((tid & ((1 << a.shift) - 1)) == 0 && piece < end) (a.splits > 1 ? bests : h.best)[piece >> a.shift] = block;
         }
         const float m = fmaxf(s.m, top), use = m == -INFINITY ? 0.0f : m;
         const float down = max_keep_nan(s.m - use, -1e4f), f = __builtin_amdgcn_exp2f(down * kLog2e);
@@ -274,129 +385,31 @@ __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_kernel(Logprob
             if (round + i < rounds) take(round + i, now[i]);
     }
     s = logprob_join_all(s, part);
-
-    const int in_range = max(0, min(end * N - lead, a.V) - max(begin * N - lead, 0));       // elements of this split
-    const int want = min(a.top, in_range);
-    if (a.top > 0) {
-        if (tid == 0) count_of = 0;                                        // (`best` is whole behind the barrier in logprob_join_all)
-        auto block_key = [&](int block) __attribute__((always_inline)) {
-            return static_cast<key64>(logprob_order(best[block])) << 32 | static_cast<uint32_t>(~block);
-        };
-        if (tid < 64) {
-            key64 b = 0;
-            if (want > 32) {
-                key64 most[4] = {0, 0, 0, 0};
-                for (int i = 0; i < blocks; i += 256)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        if (i + 64 * n + lane < blocks) most[n] = max(most[n], block_key(i + 64 * n + lane));
-                for (int bit = 63; bit >= 0; --bit) {
-                    const key64 next = b | 1ull << bit;
-                    int count = 0;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) count += __popcll(__ballot(most[n] >= next));
-                    if (count >= want) b = next;
-                    if (count == want) break;
-                }
-            } else if (want > 0) {
-                key64 most = 0;
-                for (int i = lane; i < blocks; i += 64) most = max(most, block_key(i));
-                b = logprob_bound64(most, want);
-            }
-            int n = 0;
-            for (int i = 0; i < blocks; i += 64) {
-                const bool in = i + lane < blocks && block_key(i + lane) >= b;
-                const key64 mask = __ballot(in);
-                if (in) chosen[n + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(i + lane);
-                n += __popcll(mask);
-            }
-            if (lane == 0) bound_of = b, chosen_count = n;
-        }
-        __syncthreads();
-        key64 bound = bound_of;
-        int owners = chosen_count;
-        auto piece_of = [&](int i, bool everybody) __attribute__((always_inline)) {         // -1: none
-            const int n = i >> 4, piece = n < owners ? begin + (everybody ? n : chosen[n]) * 16 + (i & 15) : end;
-            return piece < end ? piece : -1;
-        };
-        auto offer = [&](int piece, const u32x4& v) __attribute__((always_inline)) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int index = piece * N + e - lead;
-                const uint32_t order = logprob_order(Vec::at(v, e));
-                if (index >= 0 && index < a.V && (static_cast<key64>(order) << 32 | static_cast<uint32_t>(~((piece - begin) >> 4))) >= bound) {
-                    const int at = atomicAdd(&count_of, 1);
-                    if (at < kLogprobKeys) keys[at] = static_cast<key64>(order) << 32 | static_cast<uint32_t>(~index);
-                }
-            }
-        };
-        for (int from = 0; from < owners * 16; from += AHEAD * kLogprobThreads) {
-            int piece[AHEAD];
-            u32x4 v[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                piece[i] = piece_of(from + i * kLogprobThreads + tid, false);
-                v[i] = pieces[max(piece[i], 0)];
-            }
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                if (piece[i] >= 0) offer(piece[i], v[i]);
-        }
-        __syncthreads();
-        // Again in rounds where LDS did not hold them, and without a bound where NaN made a block's best no element.
-        if (count_of > kLogprobKeys || count_of < want) {
-            const bool everybody = count_of < want;
-            __syncthreads();
-            if (tid == 0) count_of = 0;
-            if (everybody) bound = 0, owners = blocks;
-            __syncthreads();
-            for (int from = 0; from < owners * 16; from += kLogprobThreads) {
-                const int piece = piece_of(from + tid, everybody);
-                if (piece >= 0) offer(piece, pieces[piece]);
-                __syncthreads();
-                const int have = count_of;
-                __syncthreads();                                           // (all have read it before the next round counts on)
-                if (have > kLogprobSlack && from + kLogprobThreads < owners * 16) {      // room for the next round: only the best stay
-                    if (tid < 64) {
-                        const int n = logprob_compact(keys, have, logprob_bound(keys, have, want, lane), lane);
-                        if (lane == 0) count_of = n;
-                    }
-                    __syncthreads();
-                }
-            }
-        }
-        if (tid < 64) logprob_best(keys, count_of, a.top, sorted, lane);
-        __syncthreads();
+    if (a.splits > 1) {
+        if (tid == 0) reinterpret_cast<LogprobStats*>(a.partial)[static_cast<size_t>(row) * a.splits + split] = s;
+        return;
     }
-    if (a.splits == 1) {
-        logprob_results<T>(a, row, s, sorted);
-    } else {
-        const size_t slot = static_cast<size_t>(row) * a.splits + split;
-        key64* to = static_cast<key64*>(a.partial);
-        if (tid < a.top) to[slot * a.top + tid] = sorted[tid];
-        if (tid == 0) reinterpret_cast<LogprobStats*>(to + static_cast<size_t>(a.M) * a.splits * a.top)[slot] = s;
-    }
+    if (a.top > 0) logprob_select(a, line, h);                             // (h.best is whole behind the barrier in logprob_join_all)
+    logprob_results<T>(a, row, s, h.sorted);
 }
 
-// The splits of a row.
+// The splits of a row, and its alternatives.
 template <typename T>
 __global__ __launch_bounds__(kLogprobThreads) void terna_logprobs_merge_kernel(LogprobArgs a)
 {
-    __shared__ key64 keys[kLogprobKeys];
-    __shared__ key64 sorted[kLogprobMaxTop];
+    __shared__ LogprobSelection h;
     __shared__ LogprobStats part[kLogprobThreads / 64];
-    const int tid = threadIdx.x, row = blockIdx.x, n = a.splits * a.top;
-    const key64* from = static_cast<const key64*>(a.partial) + static_cast<size_t>(row) * n;
-    const LogprobStats* stats = reinterpret_cast<const LogprobStats*>(static_cast<const key64*>(a.partial) + static_cast<size_t>(a.M) * n) + static_cast<size_t>(row) * a.splits;
-    for (int i = tid; i < n; i += kLogprobThreads) keys[i] = from[i];
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const LogprobRow<T> line(a, row);
     LogprobStats s{-INFINITY, 0.0f, 0.0f};
-    if (tid < a.splits) s = stats[tid];
-    s = logprob_join_all(s, part);
+    if (tid < a.splits) s = reinterpret_cast<const LogprobStats*>(a.partial)[static_cast<size_t>(row) * a.splits + tid];
     if (a.top > 0) {
-        if (tid < 64) logprob_best(keys, n, a.top, sorted, tid);
-        __syncthreads();
+        const float* bests = a.partial + 3 * static_cast<size_t>(a.M) * a.splits + static_cast<size_t>(row) * a.blocks;
+        for (int i = tid; i < (line.all + (1 << a.shift) - 1) >> a.shift; i += kLogprobThreads) h.best[i] = bests[i];
     }
-    logprob_results<T>(a, row, s, sorted);
+    s = logprob_join_all(s, part);
+    if (a.top > 0) logprob_select(a, line, h);
+    logprob_results<T>(a, row, s, h.sorted);
 }
 
 }  // namespace terna

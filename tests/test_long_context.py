@@ -92,8 +92,8 @@ def test_splits_and_workspaces():
         assert 1 <= splits <= 128 and (splits - 1) * 32 < s
         assert lib.ternaspmm_kv4_workspace_bytes(*shape) == (0 if splits == 1 else 4 * b * t * h * splits * (d + 2))
     logprobs = lib.ternaspmm_token_logprobs_workspace_bytes
-    assert logprobs(0, 10, 0, 0) == -1 and logprobs(1, 10, 0, 11) == -1 and logprobs(1, 100, 0, 65) == -1 and logprobs(1, (1 << 22) + 1, 0, 0) == -1
-    assert logprobs(2048, 128256, 0, 20) == 0 and logprobs(1, 128256, 0, 5) > 0 and logprobs(2048, 1 << 20, 0, 20) > 0 and logprobs(2048, 200000, 1, 0) > 0
+    assert logprobs(0, 10, 0, 0) == -1 and logprobs(1, 10, 0, 11) == -1 and logprobs(1, 100, 0, 65) == -1 and logprobs(1, (1 << 19) + 1, 0, 0) == -1
+    assert logprobs(2048, 128256, 0, 20) == 0 and logprobs(1, 128256, 0, 5) > 0 and logprobs(2048, 1 << 19, 0, 20) == 0 and logprobs(20, 200000, 1, 0) > 0
 
 
 class _Kv4(ctypes.Structure):
@@ -136,7 +136,7 @@ def test_c_entry_points_refuse_before_they_enqueue():
     names = "logits row fp32 targets logprob entropy ids lps top work M V stream".split()
     good = dict(logits=p(64), row=10, fp32=0, targets=p(64), logprob=p(64), entropy=p(64), ids=p(64), lps=p(64), top=3, work=None, M=1, V=10, stream=None)
     refused("ternaspmm_token_logprobs", names, good, [*({n: None} for n in ("logits", "logprob", "entropy", "ids", "lps")), dict(top=-1), dict(top=11), dict(top=65, V=100), dict(M=0), dict(V=0),
-                                                      dict(logits=p(65)), dict(logits=p(66), fp32=1), dict(work=p(68)), dict(row=-1), dict(V=300000, row=300000), dict(V=140000, row=140000, fp32=1)])
+                                                      dict(logits=p(65)), dict(logits=p(66), fp32=1), dict(work=p(66)), dict(row=-1), dict(V=(1 << 19) + 1)])
 
 
 def test_python_functions_refuse_tensors_that_are_not_on_the_gpu():
