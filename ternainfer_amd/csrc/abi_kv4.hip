@@ -130,7 +130,9 @@ int ternaspmm_kv4_store(const terna_bf16* qkv, long long row, const long long* p
         return -1;
     RotaryShape s{T, H, D, pairs, per_sequence != 0, B * T, 1, amplitude};
     const int steps = (H + 2 * KV) * (D / 8);
-    while (2 * s.tokens_a_group * pairs <= kRotaryMaxAngles && s.tokens_a_group * steps < 4 * kRotaryThreads && s.tokens / (2 * s.tokens_a_group) >= 512 &&
+    // Tokens a workgroup: as for ternaspmm_rotary; half pairs, whose pieces are read twice, twice as many (us, 4 x 8192 tokens of 30 heads adjacent 91.2, with
+    // twice as many 96.5; 2 x 4096 of 48 half 49.1, with half as many 52.9).
+    while (2 * s.tokens_a_group * pairs <= kRotaryMaxAngles && (adjacent ? 2 : 1) * s.tokens_a_group * steps <= 4 * kRotaryThreads && s.tokens / (2 * s.tokens_a_group) >= 512 &&
            (T == 1 || 2 * s.tokens_a_group <= T))
         s.tokens_a_group *= 2;
     const int groups = (s.tokens + s.tokens_a_group - 1) / s.tokens_a_group;
@@ -149,9 +151,10 @@ int ternaspmm_kv4_rows(const ternaspmm_kv4* cache, const long long* pos, int per
                        terna_stream stream)
 {
     if (!kv4_shape_ok(B, T, KV, KV, D, S) || !kv4_cache_ok(cache) || !pos || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) return -1;
-    const long long groups = static_cast<long long>(B) * T * KV * (D / kKv4Group);
-    launch(terna_kv4_rows_kernel, dim3(static_cast<unsigned>((2 * groups + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), cache->k, cache->k_scale, cache->v,
-           cache->v_scale, pos, k_out, v_out, T, KV, S, D, per_sequence != 0, groups);
+    // two steps a thread, and no fewer workgroups than the CUs; a group has at most T tokens of them where T > 1
+    const int tokens = B * T, most = T > 1 ? T : tokens, tokens_a_group = std::max(1, std::min({512 / (2 * KV * (D / 8)), most, tokens / 512}));
+    launch(terna_kv4_rows_kernel, dim3((tokens + tokens_a_group - 1) / tokens_a_group), dim3(256), 0, static_cast<hipStream_t>(stream), cache->k, cache->k_scale, cache->v,
+           cache->v_scale, pos, k_out, v_out, T, KV, S, D, per_sequence != 0, tokens, tokens_a_group);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_kv4_rows", e, __LINE__);
     return 0;

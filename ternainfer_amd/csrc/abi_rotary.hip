@@ -37,10 +37,11 @@ int ternaspmm_rotary(const void* x, const long long* x_strides, void* out, const
     auto whole = [&](const void* p, const RotaryRows& r) { return ((reinterpret_cast<uintptr_t>(p) & 15) | ((r.batch | r.token | r.head) & (n - 1))) == 0; };
     const bool pieces = D % n == 0 && whole(x, in) && whole(out, to) && (adjacent || pairs % n == 0);
     RotaryShape s{T, H, D, pairs, per_sequence != 0, B * T, 1, amplitude};
-    // tokens a workgroup: as many as its angles have room for and give every thread about four pieces; where that leaves CUs without one, the
-    // heads of a token go to several workgroups
+    // Tokens a workgroup: as many as its angles have room for while a thread has no more than four pieces (us, 32768 tokens of one head of 128 dimensions in
+    // bf16: one token 25.5, so 10.5; of 25 heads, where this is one: 74.9, four 81.8).  Where that leaves CUs without a workgroup, the heads of a token
+    // go to several (one token of 200 heads 8.6, so 3.5).
     const long long steps = static_cast<long long>(H) * (pieces ? D / n : D - pairs);
-    while (2 * s.tokens_a_group * pairs <= kRotaryMaxAngles && s.tokens_a_group * steps < 4 * kRotaryThreads && s.tokens / (2 * s.tokens_a_group) >= 512 &&
+    while (2 * s.tokens_a_group * pairs <= kRotaryMaxAngles && 2 * s.tokens_a_group * steps <= 4 * kRotaryThreads && s.tokens / (2 * s.tokens_a_group) >= 512 &&
            (T == 1 || 2 * s.tokens_a_group <= T))
         s.tokens_a_group *= 2;
     const int groups = (s.tokens + s.tokens_a_group - 1) / s.tokens_a_group;

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
             const uint16_t* from = token + head * D;
             const u32x4 own = *reinterpret_cast<const u32x4*>(from + d);
             float x[8];
-            if (n <= heads) kv4_turn8<ADJACENT>(from, own, d, angles, a.pairs, x);
+            if (n <= heads) kv4_turn8<ADJACENT>(from, own, kv4_partner<ADJACENT>(from, own, d, a.pairs), d, angles, a.pairs, x);
             else RotaryVector<uint16_t>::unpack(own, x);
             if (n < heads) {
                 *reinterpret_cast<u32x4*>(smem + kv4_piece<D>(n, d / 8)) = RotaryVector<uint16_t>::pack(x);

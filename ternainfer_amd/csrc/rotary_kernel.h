@@ -6,7 +6,8 @@
 // What bounds it: memory -- a row is read once and written once.  A workgroup takes a few tokens with all their heads: the angles (a 64-bit
 // series, about 40 instructions) are computed once a token into LDS and serve every head; its rows are requested before that.  A thread moves
 // 16 bytes of a head at a time (half pairs: 16 bytes and their partners); rows that are no whole 16 bytes, or half pairs whose partners lie
-// across such a piece, take the kernel of one pair a thread.
+// across such a piece, take the kernel of one pair a thread (2 x 1920 x 25 heads of 128 dimensions in bf16: 11.5 us by pieces, 22.5 by pairs).
+// Measured: 4 x 8192 tokens of 25 heads of 128 dimensions in bf16 74.9 us, 5.6 TB/s; one token 3.4, which is the launch and two trips to memory.
 #pragma once
 
 #include "rotary_common.h"
