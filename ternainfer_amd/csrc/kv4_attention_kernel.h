@@ -125,10 +125,10 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
     const __amdgpu_buffer_rsrc_t rk = make_raw_buffer(kb, in_reach * (D / 2)), rks = make_raw_buffer(ksb, in_reach * GROUPS), rv = make_raw_buffer(vb, in_reach * (D / 2)),
                                  rvs = make_raw_buffer(vsb, in_reach * GROUPS);
     auto load = [&](int step, Tile& x) __attribute__((always_inline)) {
-        const int k0 = step * kKv4Step;
+        const uint32_t k0 = static_cast<uint32_t>(step) * kKv4Step;         // (requests behind the longest cache pass 2^31)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int at = (k0 + qi) * (D / 2) + g * (DL / 2) + j * 16 * (D / 2);
+            const uint32_t at = (k0 + qi) * (D / 2) + g * (DL / 2) + j * 16 * (D / 2);
             if constexpr (KI == 4) {
                 const u32x4 c = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, at, 0, 0));
 #pragma unroll

@@ -455,6 +455,45 @@ def test_c_entry_point_without_a_workspace():
     assert P.same_or_near(out.view(b, 1, h, d), want, tol) <= 0
 
 
+@pytest.mark.parametrize("t", [1, 48])
+def test_the_longest_cache(t):
+    """2^25 slots of two sequences: byte offsets beyond 2^32, requests beyond 2^31.  All slots are zeros but a few written ones, whose keys weigh against the
+    zeros' 2^25 times exp(0)."""
+    slots, h, d = 1 << 25, 4, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("9 GB of caches, with room to spare")
+    _say("the longest cache", t)
+    cache = T.Kv4Cache.empty(2, 1, slots, d)
+    inv, _ = T.rotary_frequencies(d)
+    written = torch.tensor([0, 5, 1 << 24, (1 << 24) + 77, slots - 100 - t, slots - 70 - t], device="cuda")
+    last = torch.arange(slots - t, slots, device="cuda")
+    unit = _randn((2, 1, d), 80) * 0.5
+    rows = torch.cat([_randn((2, 6 + t, h * d), 81), (unit + 0.1 * _randn((2, 6 + t, d), 82)).to(torch.bfloat16), _randn((2, 6 + t, d), 83)], -1).to(torch.bfloat16)
+    T.kv4_store(rows.view(-1, (h + 2) * d), torch.cat([written, last]), inv * 0, cache, h)
+    if t == 1:                                                                   # the same bits, by the step's own launch
+        again = T.kv4_step(rows[:, -1].contiguous(), last, inv * 0, cache, h)
+    keys, values = (x[:, :, 0].double() for x in T.kv4_rows(cache, torch.cat([written, last])))
+    assert (keys != 0).any(-1).all() and torch.isfinite(keys).all()
+    one_row = T.kv4_rows(cache, torch.tensor([6, slots - 60 - t], device="cuda"))
+    assert not one_row[0].any() and not one_row[1].any()                         # nothing went elsewhere nearby
+    q = (unit[:, None, :, :].expand(2, h, t, d) * 6 + _randn((2, h, t, d), 84)).to(torch.bfloat16)
+    scale = d ** -0.5
+    got = T.kv4_attention(q, last, cache, scale).view(2, t, h, d).double()
+    score = scale * q.double() @ keys.transpose(1, 2)[:, None]                   # [2, H, T, 6 + t]
+    seen = torch.arange(6 + t, device="cuda")[None] < 7 + torch.arange(t, device="cuda")[:, None]
+    weight = torch.where(seen, score.exp(), torch.zeros_like(score))
+    mass = (last + 1 - 7 - torch.arange(t, device="cuda")).double()[None, None, :, None] + weight.sum(-1, keepdim=True)
+    want = (weight @ values[:, None] / mass).transpose(1, 2)
+    # A wave or half row adds at most 2^25 / 128 slots one after the other (2^18 half steps of an fp32, in truth far fewer), several at a time: 2^-6 of the sum and
+    # of the numerators at most; fp16 probabilities 2^-11, scores of magnitude below 40 off by (128 + 4) 2^-24 40 < 2^-11.
+    tol = (2 * 2.0 ** -6) * (weight @ values.abs()[:, None] / mass).transpose(1, 2) + P.HALF_BF16 * want.abs() + 2.0 ** -40
+    assert P.same_or_near(got, want, tol) <= 0
+    assert want.abs().max() > 1e-3                                               # (the written slots weigh something)
+    if t == 1:
+        own = T.kv4_attention(rows[:, -1, :h * d].reshape(2, h, 1, d).contiguous(), last, cache)
+        assert torch.equal(again, own)
+
+
 # ---- log probabilities ---------------------------------------------------------------------------------------------------------------
 
 
