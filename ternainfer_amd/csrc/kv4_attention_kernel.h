@@ -12,8 +12,8 @@
 //   * Values and probabilities are fp16 (below), all sums fp32.  The running maximum is raised, and the output rescaled, only where it grows by more than 2^3.
 //   * A value scale of 255 (NaN) in a slot that a row does not see must not reach it through 0 * NaN: the first such slot of each 32 dimensions is
 //     kept and NaN given to the rows that see it; the products use the largest finite scale in its place.  So also whatever unwritten slots hold.
-// What bounds it: a long cache -- memory (4 x 32768 slots, 5 kv heads: 79 MB in 23 us, 3.4 TB/s); a short one -- the launch, two trips to memory (position,
-// cache), then 0.63 us a step of a wave, a chain through LDS and two kinds of products (1 x 384 slots 6.1 us, 1 x 100 4.9).
+// What bounds it: a long cache -- memory (4 x 32768 slots, 5 kv heads: 85 MB in 20 us, 4.2 TB/s, then 4 for the splits); a short one -- the launch, two trips to memory (position,
+// cache), then 0.63 us a step of a wave, a chain through LDS and two kinds of products (1 x 384 slots 6.4 us, 8 x 384 7.0).
 #pragma once
 
 #include "kv4_store_kernel.h"
@@ -423,7 +423,8 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
     }
 }
 
-// The splits of a row: four waves, each every fourth split, D / 64 dimensions a lane.  Their order is fixed, so is the result.
+// The splits of a row: four waves, each every fourth split, D / 64 dimensions a lane.  Their order is fixed, so is the result.  What bounds it: the launch and two
+// trips to memory -- eight splits are under way at a time (step and merge of 1 x 32768 slots in 43 splits 15.0 us with one, so 13.5; of 1 x 131072 29.0 and 25.5).
 constexpr int kKv4MaxSplits = 128;             // two a lane
 template <int D>
 __global__ __launch_bounds__(256) void terna_kv4_merge_kernel(const float* __restrict__ partial, const long long* __restrict__ pos, uint16_t* __restrict__ out, int T, int H,
@@ -435,9 +436,20 @@ __global__ __launch_bounds__(256) void terna_kv4_merge_kernel(const float* __res
     const float2* stat = reinterpret_cast<const float2*>(partial + static_cast<size_t>(gridDim.x) * splits * D) + static_cast<size_t>(row) * splits;
     const float2 none{-INFINITY, 0.0f}, s0 = lane < splits ? stat[lane] : none, s1 = lane + 64 < splits ? stat[lane + 64] : none;
     const float* o = partial + static_cast<size_t>(row) * splits * D + V * lane;
-    float first[V];
+    constexpr int AT_ONCE = 8;
+    float part_of[AT_ONCE][V];
+    auto fetch = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) first[v] = wave < splits ? o[static_cast<size_t>(wave) * D + v] : 0.0f;
+        for (int n = 0; n < AT_ONCE; ++n) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) part_of[n][v] = 0.0f;
+            if (from + 4 * n < splits) {                                   // (the same for the wave)
+#pragma unroll
+                for (int v = 0; v < V; ++v) part_of[n][v] = o[static_cast<size_t>(from + 4 * n) * D + v];
+            }
+        }
+    };
+    fetch(wave);
     const int token = row / H, t = token % T;
     const long long p = pos[per_seq ? token : t];
     float m = fmaxf(s0.x, s1.x);
@@ -450,11 +462,17 @@ __global__ __launch_bounds__(256) void terna_kv4_merge_kernel(const float* __res
     for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
     float x[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = wave < splits ? first[v] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w0), wave)) : 0.0f;
-    for (int i = wave + 4; i < splits; i += 4) {
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(i < 64 ? w0 : w1), i & 63));
+    for (int v = 0; v < V; ++v) x[v] = 0.0f;
+    for (int i = wave; i < splits; i += 4 * AT_ONCE) {
+        if (i != wave) fetch(i);
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[v] += o[static_cast<size_t>(i) * D + v] * w;
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int at = i + 4 * n;
+            if (at >= splits) break;
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(at < 64 ? w0 : w1), at & 63));
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] += part_of[n][v] * w;
+        }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) part[wave][V * lane + v] = x[v];
