@@ -562,6 +562,13 @@ class Transformer:
             self._rope_frequencies = held = rotary_frequencies(self.args.head_dim, self.args.rope_theta, self.args.rope_scaling, dev)
         return held
 
+    def no_rope_table(self, dev):
+        """What stands in for the tables where nobody reads them: one position (kept, as the frequencies are)."""
+        held = getattr(self, "_no_rope_table", None)
+        if held is None or held.device != dev:
+            self._no_rope_table = held = torch.zeros((1, 2, self.args.head_dim // 2), dtype=torch.float32, device=dev)
+        return held
+
     def attention_partial(self, bsz: int, max_seq: int, single_split: bool = False):
         """(buffer, splits) for the decode step whose attention leaves the merge of its splits to the consumer of its
         output (one sequence: the O projection's prologue; more: a merge launch), or None when that form does not apply
@@ -620,9 +627,9 @@ class Transformer:
     def make_cache(self, bsz: int, max_seq: int, bits: int = 16):
         """The key/value cache of every block, for bsz sequences of max_seq tokens.  bits=4: `Kv4Cache`s, 4.25 bits a value and any length (heads of 64 or
         128 dimensions, up to 16 query heads each); it needs the fused kernels, and a step is its launches, never one (whole_step).
-        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 651 and
-        898, of 8192 1066 and 1010, of 131072 1516 in 4; 8 of 1528 1129 and 1214, of 8192 1724 and 1442; 16 of 8192 2660 and 1717; 32 of 8192 4427 and
-        2393.  A prompt of 2048 tokens 6.3 and 6.8 ms, of 8192 28.9 and 26.2, of 32768 200 in 4."""
+        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 652 and
+        896, of 8192 1069 and 981, of 131072 1417 in 4; 8 of 1528 1132 and 1212, of 8192 1727 and 1443; 16 of 8192 2659 and 1726; 32 of 8192 4381 and
+        2412.  A prompt of 2048 tokens 6.6 and 6.7 ms, of 8192 29.5 and 27.0, of 32768 219 in 4."""
         a = self.args
         if bits == 4:
             return [Kv4Cache.empty(bsz, a.n_kv_heads, max_seq, a.head_dim, self.tok_embeddings.device) for _ in range(a.n_layers)]
@@ -669,16 +676,17 @@ class Transformer:
             x = self.whole_step(tokens, cache, pos_idx, max_seq)
             if x is not None:                                                 # the blocks of the step in one launch
                 return x, None
-        if four:                                                              # no tables: the kernels form the angles
-            cos = sin = None
-            x = self.tok_embeddings[tokens.reshape(-1)]
-        elif chain and getattr(self, "step_inputs", True):
+        # (4 bits: the kernels form the angles, and the rows that come out of a table of one position are not read)
+        table = self.no_rope_table(dev) if four else self.rope_tables(max_seq, dev)
+        if chain and getattr(self, "step_inputs", True):
             # embedding rows, their partials under the first block's norm and the RoPE rows of the positions: one launch
-            x, stats, cos, sin = step_inputs(tokens, pos_idx.reshape(-1), self.tok_embeddings, self.rope_tables(max_seq, dev), self.layers[0].attention_norm)
-        elif kernels_fit and getattr(self, "step_inputs", True) and a.dim % 8 == 0:
-            x, cos, sin = prompt_inputs(tokens, pos_idx, self.tok_embeddings, self.rope_tables(max_seq, dev))
+            x, stats, cos, sin = step_inputs(tokens, pos_idx.reshape(-1), self.tok_embeddings, table, self.layers[0].attention_norm)
+        elif kernels_fit and (four or getattr(self, "step_inputs", True)) and a.dim % 8 == 0:
+            x, cos, sin = prompt_inputs(tokens, pos_idx, self.tok_embeddings, table)
+        elif four:
+            raise ValueError("a cache in 4 bits: rows of a multiple of 8 elements")
         else:
-            rows = self.rope_tables(max_seq, dev).index_select(0, pos_idx.reshape(-1))   # fp32 [T | B*T, 2, head_dim / 2]
+            rows = table.index_select(0, pos_idx.reshape(-1))                 # fp32 [T | B*T, 2, head_dim / 2]
             cos, sin = rows[:, 0].contiguous(), rows[:, 1].contiguous()       # views when one row
             x = self.tok_embeddings[tokens.reshape(-1)]
         if four:

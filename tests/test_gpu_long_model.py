@@ -203,3 +203,14 @@ def test_what_a_cache_in_4_bits_does_not_take():
         model.forward(_tokens(1, 4), cache, torch.arange(4, device="cuda"))
     with pytest.raises(ValueError):
         model.make_cache(1, 8, bits=8)
+
+
+@torch.inference_mode()
+def test_tokens_outside_the_vocabulary_do_not_fault():
+    """As over the bf16 cache: a prompt's row of such a token is NaN, and nothing but it and those that see it."""
+    model = _model(0)
+    tokens = _tokens(2, 12, seed=25)
+    clean = model.forward(tokens, model.make_cache(2, 16, bits=4), torch.arange(12, device="cuda"))
+    tokens[1, 5] = 1 << 40
+    got = model.forward(tokens, model.make_cache(2, 16, bits=4), torch.arange(12, device="cuda"))
+    assert torch.equal(got[0], clean[0]) and torch.isnan(got[1]).all()
