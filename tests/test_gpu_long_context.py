@@ -666,3 +666,61 @@ def test_a_request_from_positions_to_scores_eager_and_captured():
             assert torch.equal(got, w), i
         for one, two in zip(eager, graphed):
             assert torch.equal(one, two)
+
+
+def test_calls_at_once_and_two_graphs():
+    """The same operators on two streams at the same time, eager and as two captured graphs replayed together: split launches keep to scratch of their own."""
+    h, kv, d, slots = 20, 5, 128, 4000
+    caches = [T.Kv4Cache(*P.random_cache(2, kv, slots, d, 320 + i)) for i in range(2)]
+    logits = [_randn((3, 60000), 330 + i, torch.float32) for i in range(2)]
+    q = [_randn((2, h, 1, d), 340 + i) for i in range(2)]
+    many = [_randn((2, h, 60, d), 350 + i) for i in range(2)]
+    last, inv = torch.tensor([slots - 1], device="cuda"), T.rotary_frequencies(d)[0]
+    span = torch.arange(slots - 60, slots, device="cuda")
+
+    def work(i):
+        return [T.kv4_attention(q[i], last, caches[i]), *T.token_logprobs(logits[i], last.expand(3), 20), T.kv4_attention(many[i], span, caches[i]),
+                T.rotary_embed(many[i], span[:h].repeat(2, 1), inv)]
+
+    want = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        got = [None, None]
+        for i, stream in enumerate(streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got[i] = work(i)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want[i]))
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, stream=streams[i]):
+            got[i] = work(i)
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                graphs[i].replay()
+        eager = work(0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want[i]))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[0]))
+
+
+@pytest.mark.parametrize("b,h,kv,d", [(300, 8, 8, 64), (257, 5, 1, 128), (1, 64, 2, 128), (2, 33, 1, 64)])
+def test_steps_of_many_sequences_and_of_many_heads(b, h, kv, d):
+    """More workgroups than CUs; more query heads than a tile has rows."""
+    _say("step", b, h, kv, d)
+    slots = 50
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 360))
+    twin = T.Kv4Cache(*(c.clone() for c in cache))
+    pos = torch.randint(-1, slots + 1, (b, 1), generator=_gen(361), device="cuda")
+    inv, _ = T.rotary_frequencies(d)
+    x = _randn((b, (h + 2 * kv) * d), 362)
+    got = T.kv4_step(x, pos, inv, cache, h)
+    q = T.kv4_store(x, pos, inv, twin, h)
+    assert all(torch.equal(one, two) for one, two in zip(cache, twin))
+    assert torch.equal(got.isnan(), T.kv4_attention(q, pos, twin).isnan())
+    _attend(q, pos, twin)
+    want, tol = P.attention(q, pos, twin, d ** -0.5)
+    assert P.same_or_near(got.view(b, 1, h, d), want, tol) <= 0
