@@ -4,8 +4,8 @@
 //
 // The rows of a kv head -- its G = H / KV query heads times the new tokens, row r = t * G + head -- are taken sixteen at a time, as the columns of the
 // matrix cores' 16x16x32 products.  A wave works alone on 32 slots at a time: codes -> bf16 in registers (the hardware conversion, two values an
-// instruction, the scale inside it: exact), scores, running maximum and sum, output; no wave waits for another until the end, where the four
-// of a workgroup and then the splits are merged.
+// instruction, the scale inside it: exact), scores, running maximum and sum, output; no wave waits for another until the end, where the four or
+// eight of a workgroup and then the splits are merged.
 //   * Keys: a lane holds a quarter of a row (one 16-byte load of a row of 128 dimensions) and its scale byte; the products run over the dimensions in
 //     the order in which the lanes hold them, for queries and keys alike.
 //   * Values: a lane holds 32 dimensions of a row, which share a scale; converted rows go through LDS (of the wave alone) and come back transposed.
