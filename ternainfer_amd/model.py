@@ -626,7 +626,7 @@ class Transformer:
 
     def make_cache(self, bsz: int, max_seq: int, bits: int = 16):
         """The key/value cache of every block, for bsz sequences of max_seq tokens.  bits=4: `Kv4Cache`s, 4.25 bits a value and any length (heads of 64 or
-        128 dimensions, up to 16 query heads each); it needs the fused kernels, and a step is its launches, never one (whole_step).
+        128 dimensions); it needs the fused kernels, and a step is its launches, never one (whole_step).
         For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 652 and
         896, of 8192 1069 and 981, of 131072 1417 in 4; 8 of 1528 1132 and 1212, of 8192 1727 and 1443; 16 of 8192 2659 and 1726; 32 of 8192 4381 and
         2412.  A prompt of 2048 tokens 6.6 and 6.7 ms, of 8192 29.5 and 27.0, of 32768 219 in 4."""
@@ -718,12 +718,12 @@ class Transformer:
         for index, (layer, held) in enumerate(zip(self.layers, cache)):
             x_in, pending_in = x, pending
             ck, cv = (held.k, held.v) if four else held
-            in4 = (held, *kv4) if four else None
+            in4 = dict(kv4=(held, *kv4)) if four else {}
             if chain:
                 nxt = self.layers[index + 1].attention_norm if index + 1 < len(self.layers) else self.norm
-                x, stats = layer.forward_chain(x, stats, ck, cv, pos_idx, cos, sin, attn_ws, nxt, split=split, kv4=in4)
+                x, stats = layer.forward_chain(x, stats, ck, cv, pos_idx, cos, sin, attn_ws, nxt, split=split, **in4)
             else:
-                x, pending = layer.forward(x, pending, ck, cv, pos_idx, cos, sin, mask, attn_ws, kv4=in4)
+                x, pending = layer.forward(x, pending, ck, cv, pos_idx, cos, sin, mask, attn_ws, **in4)
             if trace is not None:
                 trace(index, x_in, pending_in, x, pending)
         return x, pending

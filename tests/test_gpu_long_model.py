@@ -214,3 +214,18 @@ def test_tokens_outside_the_vocabulary_do_not_fault():
     tokens[1, 5] = 1 << 40
     got = model.forward(tokens, model.make_cache(2, 16, bits=4), torch.arange(12, device="cuda"))
     assert torch.equal(got[0], clean[0]) and torch.isnan(got[1]).all()
+
+
+@torch.inference_mode()
+def test_blocks_of_a_users_own_run_as_before(monkeypatch):
+    """A block whose methods know nothing of a cache in 4 bits is called without it."""
+    model = _model(0)
+    want = _prompt_and_steps(model, model.make_cache(2, 40), 2, 17, 2)
+    forward, chain = Block.forward, Block.forward_chain
+    monkeypatch.setattr(Block, "forward", lambda self, x, pending, cache_k, cache_v, pos_idx, cos, sin, mask, attn_ws=None:
+                        forward(self, x, pending, cache_k, cache_v, pos_idx, cos, sin, mask, attn_ws))
+    monkeypatch.setattr(Block, "forward_chain", lambda self, x, stats, cache_k, cache_v, pos_idx, cos, sin, attn_ws, next_norm, split=False:
+                        chain(self, x, stats, cache_k, cache_v, pos_idx, cos, sin, attn_ws, next_norm, split))
+    model.one_launch_step = False
+    got = _prompt_and_steps(model, model.make_cache(2, 40), 2, 17, 2)
+    assert all(torch.equal(one, two) for one, two in zip(got, want))
