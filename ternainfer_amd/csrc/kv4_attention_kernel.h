@@ -43,13 +43,9 @@ __device__ __forceinline__ u32x4 kv4_values_half(uint32_t codes, float scale)
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
 }
 
-// (as an instruction: from fmaxf the compiler makes two, each behind one that quiets a NaN that no matrix product leaves)
-__device__ __forceinline__ float kv4_max3(float a, float b, float c)
-{
-    float m;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
-    return m;
-}
+// NaN where one of them is: a row with such a score is NaN, whatever its maximum.  (IEEE 754-2019's maximum, one instruction.  From fmaxf the compiler makes two, each
+// behind one that quiets a NaN; and not inline assembly, in front of which it does not wait for the matrix products that are read here.)
+__device__ __forceinline__ float kv4_max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 struct Kv4Attention {
     const uint16_t* q;                         // [B][H][T][D]; STEP: rows of `row` elements as terna_kv4_store_kernel takes them
