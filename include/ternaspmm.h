@@ -716,7 +716,8 @@ int ternaspmm_kv4_store(const terna_bf16* qkv, long long row, const long long* p
 int ternaspmm_kv4_rows(const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* k_out, terna_bf16* v_out, int B, int T, int KV, int D, int S,
                        terna_stream stream);
 /* Attention over the cache: out bf16 [B * T][H * D], row (b, t) = softmax over the slots 0 .. pos of scale * q . k, times the values; q bf16
- * [B][H][T][D].  A negative position sees nothing: zeros.  One from S on: NaN.  Slots that a row does not see do not reach it, whatever they hold.
+ * [B][H][T][D].  A negative position sees nothing: zeros.  One from S on: NaN.  Slots that a row does not see do not reach it, whatever they hold
+ * (one that a row computed beside it sees may change its last bits: where a value's scale byte lies outside 104 .. 140 they are all computed with bf16 values).
  * workspace: ternaspmm_kv4_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for long caches of few rows.
  * ternaspmm_kv4_splits: the number of parts a row's slots are read in. */
 int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S);

@@ -9,7 +9,8 @@
 //   * Keys: a lane holds a quarter of a row (one 16-byte load of a row of 128 dimensions) and its scale byte; the products run over the dimensions in
 //     the order in which the lanes hold them, for queries and keys alike.
 //   * Values: a lane holds 32 dimensions of a row, which share a scale; converted rows go through LDS (of the wave alone) and come back transposed.
-//   * Values and probabilities are fp16 (below), all sums fp32.  The running maximum is raised, and the output rescaled, only where it grows by more than 2^3.
+//   * Values and probabilities are fp16 (below), all sums fp32.  The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own, so that a
+//     row's bits are the same whatever rows, real or padded, share its tile.
 //   * A value scale of 255 (NaN) in a slot that a row does not see must not reach it through 0 * NaN: the first such slot of each 32 dimensions is
 //     kept and NaN given to the rows that see it; the products use the largest finite scale in its place.  So also whatever unwritten slots hold.
 // What bounds it: a long cache -- memory (4 x 32768 slots, 5 kv heads: 85 MB in 20 us, 4.2 TB/s, then 4 for the splits); a short one -- the launch, two trips to memory (position,
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
             float top = kv4_max3(kv4_max3(s[0][0], s[0][1], s[0][2]), kv4_max3(s[0][3], s[1][0], s[1][1]), kv4_max3(s[1][2], s[1][3], s[1][3]));
             top = cross_row_reduce<true>(top) * scale;
             if (__any(top > m_run + GROWTH)) {
-                const float m_new = fmaxf(m_run, top);
+                const float m_new = top > m_run + GROWTH ? top : m_run;            // a row by its own growth alone: its bits do not hang on the rows beside it
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));       // (a row that has seen nothing yet: exp(-inf))
                 m_run = m_new;
                 l_run *= alpha;

@@ -13,7 +13,7 @@
 //   * Values and probabilities are fp16: a value is a code times a power of two, exact in fp16 for scale bytes 104 .. 140 (2^-23 .. 2^13); probabilities keep 11 bits,
 //     held at 2^12 for a row's maximum (up to 2^15 by what follows) so that those 2^-26 of it are still normal numbers.  A tile with any other scale
 //     marks its workgroup, which starts again with bf16 values and probabilities in two bf16 -- the products twice.
-//   * A row's running maximum is raised, and the output rescaled, only where it grows by more than 2^3.
+//   * A row's running maximum is raised, and the output rescaled, only where it grows by more than 2^3 itself.
 // Scales that stand for NaN and slots that a row does not see: as in kv4_attention_kernel.h.
 #pragma once
 
@@ -285,7 +285,7 @@ __device__ __forceinline__ bool kv4_prefill(const Kv4Attention& a, uint8_t* smem
         float top = kv4_max3(kv4_max3(tops[0], tops[1], tops[2]), tops[3], -INFINITY);
         top = halves_reduce<true>(top) * scale;
         if (__any(top > m_run + GROWTH)) {
-            const float m_new = fmaxf(m_run, top);
+            const float m_new = top > m_run + GROWTH ? top : m_run;            // a row by its own growth alone: its bits do not hang on the rows beside it
             const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
             m_run = m_new;
             l_run *= alpha;

@@ -724,3 +724,40 @@ def test_steps_of_many_sequences_and_of_many_heads(b, h, kv, d):
     _attend(q, pos, twin)
     want, tol = P.attention(q, pos, twin, d ** -0.5)
     assert P.same_or_near(got.view(b, 1, h, d), want, tol) <= 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t,h,kv", [(1, 8, 1), (3, 5, 1), (4, 20, 5), (40, 8, 2), (120, 4, 1), (200, 8, 2)])
+def test_a_row_does_not_depend_on_the_rows_beside_it(t, h, kv, d):
+    """Bit for bit: other queries, and other keys and values in slots that it does not see (with scales that fp16 has room for), in both layouts."""
+    _say("rows beside", t, h, kv, d)
+    slots = 900
+    cache = T.Kv4Cache(*P.random_cache(1, kv, slots, d, 390))
+    pos = 600 + torch.arange(t, device="cuda")
+    q = _randn((1, h, t, d), 391)
+    want = T.kv4_attention(q, pos, cache).view(t, h, d)
+    for seed, factor in ((392, 1.0), (393, 30.0), (394, 300.0)):
+        other = (_randn(q.shape, seed) * factor).to(torch.bfloat16)
+        even = torch.arange(h, device="cuda") % 2 == 0
+        mixed = torch.where(even[None, :, None, None], q, other)
+        assert torch.equal(T.kv4_attention(mixed, pos, cache).view(t, h, d)[:, even], want[:, even])
+        if t > 1:
+            first = t // 2
+            mixed = torch.cat([q[:, :, :first], other[:, :, first:]], 2)
+            later = T.Kv4Cache(*(c.clone() for c in cache))
+            for c, fresh in zip(later, P.random_cache(1, kv, slots, d, seed)):
+                c[:, :, 600 + first:] = fresh[:, :, 600 + first:]
+            later.k_scale[:, :, 600 + first::7] = 135
+            assert torch.equal(T.kv4_attention(mixed, pos, later).view(t, h, d)[:first], want[:first])
+
+
+@pytest.mark.parametrize("b,h,kv,d,slots", [(2, 300, 1, 128, 20000), (3, 23, 1, 128, 700), (2, 40, 2, 64, 2000)])
+def test_step_is_store_and_attention_where_a_tile_has_few_rows(b, h, kv, d, slots):
+    """The last tile of a kv head's query heads: what fills up its sixteen rows does not count."""
+    _say("step", b, h, kv, d, slots)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 395))
+    pos = torch.randint(slots // 2, slots, (b, 1), generator=_gen(396), device="cuda")
+    inv, _ = T.rotary_frequencies(d)
+    x = _randn((b, (h + 2 * kv) * d), 397) * 3
+    got = T.kv4_step(x, pos, inv, cache, h)
+    assert torch.equal(got, T.kv4_attention(T.kv4_store(x, pos, inv, cache, h), pos, cache))
