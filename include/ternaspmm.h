@@ -724,7 +724,8 @@ int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S);
 long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S);
 int ternaspmm_kv4_attention(const terna_bf16* q, const ternaspmm_kv4* cache, const long long* pos, int per_sequence, terna_bf16* out, void* workspace, int B, int T, int H,
                             int KV, int D, int S, float scale, terna_stream stream);
-/* One new token per sequence: ternaspmm_kv4_store and ternaspmm_kv4_attention in one launch (two with splits), their bits; T = 1. */
+/* One new token per sequence: ternaspmm_kv4_store and ternaspmm_kv4_attention in one launch (two with splits), their bits; T = 1.  More than 32 query heads
+ * a kv head may take the launches of the two instead; the queries then go through the workspace. */
 int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
                        const ternaspmm_kv4* cache, terna_bf16* out, void* workspace, int B, int H, int KV, int D, int S, float scale, int adjacent, terna_stream stream);
 

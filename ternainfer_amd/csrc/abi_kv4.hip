@@ -1,4 +1,4 @@
-// C ABI of the 4-bit key/value cache: store, rows of it, attention of few query rows, the single-token step (kv4_*_kernel.h).
+// C ABI of the 4-bit key/value cache: store, rows of it, attention of few and of many query rows, the single-token step (kv4_*_kernel.h).
 // Declarations: include/ternaspmm.h.
 #include <hip/hip_runtime.h>
 
@@ -9,6 +9,7 @@
 
 #include "../../include/ternaspmm.h"
 #include "host_util.h"
+#include "kv4_plan.h"
 #include "kv4_prefill_kernel.h"
 
 using namespace terna;
@@ -24,54 +25,6 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 bool kv4_cache_ok(const ternaspmm_kv4* c) { return c && c->k && c->k_scale && c->v && c->v_scale && aligned16(c->k) && aligned16(c->v) &&
                                                            ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3) == 0; }
 
-// How the attention of one call is laid out: by 16 rows of a kv head and waves of their own (few rows: memory), or by 128 rows (many: matrix cores); tiles of
-// rows, and the parts that the slots are read in.  By the times that the two take as a function of the sizes (us, from 110 measured shapes, graphs of 24 launches;
-// causal ones included, whose rows see half of what is counted here):
-//   few    a workgroup 4.2 + 0.63 a round of its four waves alone on its CU, 4.5 + 1.1 with a second one (64 dimensions: a fourth) beside it; one of eight waves
-//          is as two beside each other in half the parts (one token of 32 sequences, 1528 slots: 14.9 in three parts of four waves, 13.3 in one of eight)
-//   many   a workgroup 9 + 1.75 a step of its two groups (128 slots), one to a CU
-//   parts  2 for the launch that joins them, and their numerators written and read at 3 TB/s
-// Measured, few / many: 8 x 16 tokens, 4096 slots 17 / 22; 1 x 32, 32768 31 / 29; 8 x 64, 4096 55 / 41; prompts 1 x 400 14.2 / 14.9, 4 x 200 15.5 / 12.0, 1 x 1024 34.6 / 22.6;
-// parts of 1 x 1 token, 1024 slots 9.3 in one, 7.7 in four, 32768 17.2 in 102 of them; 1 x 384 tokens in one 6.1, in three 7.8.
-struct Kv4Plan {
-    bool many;
-    int tiles, splits, waves;
-};
-Kv4Plan kv4_plan(int B, int T, int H, int KV, int D, int S)
-{
-    const long long rows = static_cast<long long>(T) * (H / KV), heads = static_cast<long long>(B) * KV;
-    const float all_rows = static_cast<float>(rows) * static_cast<float>(heads);
-    const long long steps = (S + kKv4Step - 1) / kKv4Step, tiles_few = (rows + 15) / 16, tiles_many = (rows + kKv4Rows - 1) / kKv4Rows;
-    auto joined = [&](long long n) { return n == 1 ? 0.0f : 2.0f + all_rows * static_cast<float>(8 * D * n) * (1.0f / 3e6f); };
-    auto rounds = [&](long long n, int waves) { return static_cast<float>((steps + waves * n - 1) / (waves * n)); };
-    auto few = [&](long long n) {
-        const float wgs = static_cast<float>(heads * tiles_few * n);
-        return std::max(1.0f, wgs / (D == 64 ? 1024.0f : 512.0f)) * (wgs <= 256.0f ? 4.2f + 0.63f * rounds(n, 4) : 4.5f + 1.1f * rounds(n, 4)) + joined(n);
-    };
-    auto few_of_eight = [&](long long n) { return 4.5f + 1.1f * rounds(n, 8) + joined(n); };
-    auto many = [&](long long n) {
-        const float wgs = static_cast<float>(heads * tiles_many * n);
-        return (wgs <= 256.0f ? 1.0f : wgs / 256.0f + 0.5f) * (9.0f + 1.75f * rounds(n, 4)) + joined(n);
-    };
-    // the next count of parts that saves a round
-    auto next = [&](long long n, int waves) {
-        const long long r = (steps + waves * n - 1) / (waves * n);
-        return r <= 1 ? kKv4MaxSplits + 1ll : (steps + waves * (r - 1) - 1) / (waves * (r - 1));
-    };
-    Kv4Plan p{false, static_cast<int>(tiles_few), 1, 4};
-    float best = few(1);
-    const long long most = std::min<long long>({kKv4MaxSplits, (steps + 3) / 4, 512 / (heads * tiles_few)}), most_of_eight = std::min(most, 256 / (heads * tiles_few));
-    for (long long n = next(1, 4); n <= most; n = next(n, 4))
-        if (const float time = few(n); time < best) best = time, p.splits = static_cast<int>(n);
-    for (long long n = 1; n <= most_of_eight; n = next(n, 8))
-        if (const float time = few_of_eight(n); time < best - 0.25f) best = time, p.splits = static_cast<int>(n), p.waves = 8;
-    if (rows <= 32) return p;
-    const long long most_many = std::min<long long>({kKv4MaxSplits, steps / 8, 256 / (heads * tiles_many)});
-    for (long long n = 1; n <= std::max(1ll, most_many); n = next(n, 4))
-        if (const float time = many(n); time < best) best = time, p = Kv4Plan{true, static_cast<int>(tiles_many), static_cast<int>(n), 8};
-    return p;
-}
-
 template <int D, bool STEP>
 void launch_kv4_few(const Kv4Attention& a, int waves, int adjacent, long long grid, hipStream_t st)
 {
@@ -86,10 +39,12 @@ template <bool STEP>
 int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, hipStream_t st)
 {
     const Kv4Plan plan = kv4_plan(a.B, a.T, a.H, a.KV, D, a.S);
-    a.tiles = plan.tiles;
     a.splits = a.partial ? plan.splits : 1;
+    // (one token without a workspace by few rows, so that a step, which has no room there for turned queries, is the same)
+    const bool many = !STEP && plan.many && (a.T > 1 || a.partial);
+    a.tiles = kv4_tiles(static_cast<long long>(a.T) * (a.H / a.KV), many);
     const long long groups = static_cast<long long>(a.B) * a.KV * a.splits;
-    if (!STEP && plan.many) {
+    if (many) {
         const int rounds = (a.tiles + 7) / 8;
         a.parts = (a.tiles + rounds - 1) / rounds;
         const long long grid = 8 * ((groups * a.parts + 7) / 8) * rounds;
@@ -112,6 +67,9 @@ int launch_kv4_attention(const char* who, Kv4Attention a, int D, int adjacent, h
     return 0;
 }
 
+// Of the workspace of one new token: the queries that a step by many rows stores in front of the parts.
+long long kv4_query_bytes(int B, int T, int H, int KV, int D, int S) { return T == 1 && kv4_plan(B, T, H, KV, D, S).many ? 2ll * B * H * D : 0; }
+
 }  // namespace
 
 extern "C" {
@@ -124,8 +82,9 @@ int ternaspmm_kv4_splits(int B, int T, int H, int KV, int D, int S)
 
 long long ternaspmm_kv4_workspace_bytes(int B, int T, int H, int KV, int D, int S)
 {
-    const int splits = ternaspmm_kv4_splits(B, T, H, KV, D, S);
-    return splits < 0 ? -1 : splits == 1 ? 0 : 4ll * B * T * H * splits * (D + 2);
+    if (!kv4_shape_ok(B, T, H, KV, D, S)) return -1;
+    const int splits = kv4_plan(B, T, H, KV, D, S).splits;
+    return kv4_query_bytes(B, T, H, KV, D, S) + (splits == 1 ? 0 : 4ll * B * T * H * splits * (D + 2));
 }
 
 int ternaspmm_kv4_store(const terna_bf16* qkv, long long row, const long long* pos, int per_sequence, const double* frequency, int pairs, double amplitude,
@@ -183,6 +142,13 @@ int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* po
     if (!kv4_shape_ok(B, 1, H, KV, D, S) || !kv4_cache_ok(cache) || !qkv || !pos || !frequency || !out || pairs < 1 || 2 * pairs > D || row < (H + 2ll * KV) * D || (row & 7) ||
         !aligned16(qkv) || !aligned16(out) || !aligned16(workspace))
         return -1;
+    // The kernel of many rows takes queries that are turned, and keys that lie in the cache: two launches or three (us, against the step's own kernel, 128 sequences
+    // of 128 query heads and a kv head: 40 slots 16.0 / 25.0, 512 21.3 / 31.9, 4096 65.8 / 90.5; 96 of 48, 6000 slots 58.6 / 60.7).
+    if (const long long queries = workspace ? kv4_query_bytes(B, 1, H, KV, D, S) : 0; queries > 0) {
+        terna_bf16* q = static_cast<terna_bf16*>(workspace);
+        if (ternaspmm_kv4_store(qkv, row, pos, per_sequence, frequency, pairs, amplitude, q, cache, B, 1, H, KV, D, S, adjacent, stream) != 0) return -1;
+        return ternaspmm_kv4_attention(q, cache, pos, per_sequence, out, static_cast<uint8_t*>(workspace) + queries, B, 1, H, KV, D, S, scale, stream);
+    }
     Kv4Attention a{};
     a.q = qkv, a.k = cache->k, a.k_scale = cache->k_scale, a.v = cache->v, a.v_scale = cache->v_scale, a.pos = pos, a.out = out, a.partial = static_cast<float*>(workspace);
     a.frequency = frequency, a.amplitude = amplitude, a.row = row, a.pairs = pairs;

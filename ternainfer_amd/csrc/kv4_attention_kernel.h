@@ -17,6 +17,7 @@
 // cache), then 0.63 us a step of a wave, a chain through LDS and two kinds of products (1 x 384 slots 6.4 us, 8 x 384 7.0).
 #pragma once
 
+#include "kv4_plan.h"
 #include "kv4_store_kernel.h"
 
 namespace terna {
@@ -26,7 +27,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kKv4Step = 32;                   // slots of a wave's step
 constexpr float kKv4Held = -26.0f;             // a row's largest probability is held at 2^-26: sums over 2^25 slots of the largest values stay finite
 
 // Values and probabilities in fp16: a value is a code times a power of two, exact in fp16 for scale bytes 104 .. 140 (2^-23 .. 2^13); probabilities keep 11 bits, held
@@ -422,7 +422,6 @@ __global__ __launch_bounds__(64 * NW, 2) void terna_kv4_attention_kernel(Kv4Atte
 
 // The splits of a row: four waves, each every fourth split, D / 64 dimensions a lane.  Their order is fixed, so is the result.  What bounds it: the launch and two
 // trips to memory -- eight splits are under way at a time (step and merge of 1 x 32768 slots in 43 splits 15.0 us with one, so 13.5; of 1 x 131072 29.0 and 25.5).
-constexpr int kKv4MaxSplits = 128;             // two a lane
 template <int D>
 __global__ __launch_bounds__(256) void terna_kv4_merge_kernel(const float* __restrict__ partial, const long long* __restrict__ pos, uint16_t* __restrict__ out, int T, int H,
                                                               int splits, int per_seq)

@@ -21,7 +21,6 @@
 
 namespace terna {
 
-constexpr int kKv4Rows = 128;                  // query rows of a workgroup
 constexpr int kKv4Tile = 64;                   // slots of a tile
 
 template <int D>

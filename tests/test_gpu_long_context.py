@@ -761,3 +761,58 @@ def test_step_is_store_and_attention_where_a_tile_has_few_rows(b, h, kv, d, slot
     x = _randn((b, (h + 2 * kv) * d), 397) * 3
     got = T.kv4_step(x, pos, inv, cache, h)
     assert torch.equal(got, T.kv4_attention(T.kv4_store(x, pos, inv, cache, h), pos, cache))
+
+
+# Query heads of one kv head enough for the layout of many rows, in one part and in several, with parts whose rows are an odd number.
+MANY_HEADS = [(128, 128, 1, 128, 40), (256, 64, 1, 128, 128), (96, 48, 1, 128, 6000), (48, 96, 2, 128, 5600), (8, 71, 1, 64, 32768), (1, 568, 8, 64, 32768), (4, 128, 1, 64, 32768),
+              (2, 300, 1, 128, 20000)]
+
+
+@pytest.mark.parametrize("b,h,kv,d,slots", MANY_HEADS)
+def test_steps_of_many_query_heads_a_kv_head(b, h, kv, d, slots):
+    """Every head against 64 bits; outputs and cache are those of kv4_store and kv4_attention, bit for bit."""
+    _say("step of many heads", b, h, kv, d, slots)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 370))
+    twin = T.Kv4Cache(*(c.clone() for c in cache))
+    pos = torch.randint(slots // 2, slots, (b, 1), generator=_gen(371), device="cuda")
+    if b > 2:
+        pos[0], pos[1] = -1, slots
+    inv, _ = T.rotary_frequencies(d)
+    x = _randn((b, (h + 2 * kv) * d), 372)
+    got = T.kv4_step(x, pos, inv, cache, h, adjacent=False)
+    q = T.kv4_store(x, pos, inv, twin, h, adjacent=False)
+    want = _attend(q, pos, twin)
+    assert all(torch.equal(one, two) for one, two in zip(cache, twin))
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("b,h,kv,d,slots", [(96, 48, 1, 128, 6000), (8, 71, 1, 64, 32768)])
+def test_a_captured_step_of_many_query_heads(b, h, kv, d, slots):
+    """Replayed with eager work between, and without a workspace."""
+    _say("captured step of many heads", b, h, kv, d, slots)
+    cache = T.Kv4Cache(*P.random_cache(b, kv, slots, d, 380))
+    twin = T.Kv4Cache(*(c.clone() for c in cache))
+    pos = torch.randint(slots // 2, slots - 8, (b, 1), generator=_gen(381), device="cuda")
+    now, inv = pos.clone(), T.rotary_frequencies(d)[0]
+    steps = [_randn((b, (h + 2 * kv) * d), 382 + i) for i in range(4)]
+    x = steps[0].clone()
+    T.kv4_step(x, now, inv, T.Kv4Cache(*(c.clone() for c in cache)), h)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = T.kv4_step(x, now, inv, cache, h)
+    for i, rows in enumerate(steps):
+        x.copy_(rows)
+        now.copy_(pos + i)
+        want = T.kv4_step(rows, pos + i, inv, twin, h)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want) and all(torch.equal(one, two) for one, two in zip(cache, twin)), i
+    lib = _lib.load()
+    out = torch.empty((b, h * d), dtype=torch.bfloat16, device="cuda")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    c = ctypes.byref(_Kv4(*(t.data_ptr() for t in cache)))
+    assert lib.ternaspmm_kv4_step(x.data_ptr(), x.shape[1], now.data_ptr(), 1, inv.data_ptr(), inv.numel(), 1.0, c, out.data_ptr(), None, b, h, kv, d, slots, d ** -0.5, 1, stream) == 0
+    q = T.kv4_store(x, now, inv, twin, h)
+    want, tol = P.attention(q, now, twin, d ** -0.5)
+    assert P.same_or_near(out.view(b, 1, h, d), want, tol) <= 0
