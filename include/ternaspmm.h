@@ -695,14 +695,16 @@ int ternaspmm_probe_barrier(void* state, int workgroups, int rounds, unsigned fi
  * elements, the last contiguous; out likewise, or x itself with x's strides; no other overlap.  pos int64 [T] ([B][T] with per_sequence); frequency
  * float64 [pairs], radians a position.  Pair j = dimensions (2j, 2j + 1) when adjacent, else (j, j + pairs); (a, b) becomes
  * (a cos - b sin, b cos + a sin), cos and sin of pos * frequency[j] (formed in 64 bits) times amplitude.  Dimensions from 2 * pairs on are copied.
- * 2 * pairs <= D <= 1024, H <= 65535. */
+ * 2 * pairs <= D <= 1024, H <= 65535, and fewer than 2^24 workgroups: B * T < 2^24, and up to 2^30 where a workgroup takes several tokens (heads of few pieces,
+ * T not below their number unless it is 1). */
 int ternaspmm_rotary(const void* x, const long long* x_strides, void* out, const long long* out_strides, int fp32, const long long* pos, int per_sequence,
                      const double* frequency, int pairs, double amplitude, int B, int T, int H, int D, int adjacent, terna_stream stream);
 
 /* A key/value cache in 4 bits: codes [B][KV][S][D / 2] and scale bytes [B][KV][S][D / 32].  A code is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign, the
  * even dimension in the lower half of a byte) and stands for code * 2^(byte - 127) of its 32 dimensions' scale byte: the smallest exponent e in
  * -125 .. 125 with max |x| <= 7 * 2^e, codes rounded to nearest (ties to even) and held to 6; byte 255 -- one of the 32 was NaN or infinite -- stands
- * for NaN.  Codes 16-byte aligned, scale bytes 4; D 64 or 128; S <= 2^25. */
+ * for NaN.  Codes 16-byte aligned, scale bytes 4; D 64 or 128; S <= 2^25.  Of a call: B * T <= 2^24, B * T * H <= 2^28, and fewer than 2^24 workgroups (the attention has
+ * one for every 16 query rows of a kv head). */
 typedef struct ternaspmm_kv4 {
     uint8_t *k, *k_scale, *v, *v_scale;
 } ternaspmm_kv4;
@@ -732,7 +734,7 @@ int ternaspmm_kv4_step(const terna_bf16* qkv, long long row, const long long* po
 /* Of M rows of V logits (bf16, or fp32; `row` elements apart): logprob fp32 [M] of targets int64 [M] (NaN for one outside [0, V); both may be NULL),
  * entropy fp32 [M] in nats, and the `top` (0 .. 64, at most V) largest: ids int64 [M][top], by value, equal values by lower index, NaN last, with
  * their log probabilities.  A row with NaN or +inf, or of -inf alone, has no distribution: its probabilities and entropy are NaN.
- * V up to 2^19.  workspace: ternaspmm_token_logprobs_workspace_bytes, 4-byte aligned; NULL: slower for few rows. */
+ * V up to 2^19, M below 2^24.  workspace: ternaspmm_token_logprobs_workspace_bytes, 4-byte aligned; NULL: slower for few rows. */
 long long ternaspmm_token_logprobs_workspace_bytes(int M, int V, int fp32, int top);
 int ternaspmm_token_logprobs(const void* logits, long long row, int fp32, const long long* targets, float* logprob, float* entropy, long long* top_ids,
                              float* top_logprobs, int top, void* workspace, int M, int V, terna_stream stream);

@@ -14,7 +14,7 @@ namespace {
 
 bool logprobs_shape_ok(int M, int V, int top)
 {
-    return M >= 1 && M <= 1 << 24 && V >= 1 && V <= 1 << 19 && top >= 0 && top <= kLogprobMaxTop && top <= V;
+    return M >= 1 && launch_fits(M, kLogprobThreads) && V >= 1 && V <= 1 << 19 && top >= 0 && top <= kLogprobMaxTop && top <= V;
 }
 
 // Workgroups of a row: enough that the rows together give every CU two, while each keeps two pieces a thread.
@@ -53,10 +53,8 @@ int ternaspmm_token_logprobs(const void* logits, long long row, int fp32, const 
     const int shift = logprobs_shift(V, fp32);
     LogprobArgs a{logits, targets, logprob, entropy, top_ids, top_logprobs, static_cast<float*>(workspace), row, M, V, top, workspace ? logprobs_splits(M, V) : 1,
                   logprobs_blocks(V, fp32, shift), shift};
-    const long long grid = static_cast<long long>(M) * a.splits;
-    if (grid >= 1ll << 31) return -1;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    launch(fp32 ? terna_logprobs_kernel<float> : terna_logprobs_kernel<uint16_t>, dim3(static_cast<unsigned>(grid)), dim3(kLogprobThreads), 0, st, a);
+    launch(fp32 ? terna_logprobs_kernel<float> : terna_logprobs_kernel<uint16_t>, dim3(M * a.splits), dim3(kLogprobThreads), 0, st, a);
     if (a.splits > 1) launch(fp32 ? terna_logprobs_merge_kernel<float> : terna_logprobs_merge_kernel<uint16_t>, dim3(M), dim3(kLogprobThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_token_logprobs", e, __LINE__);

@@ -45,6 +45,7 @@ int ternaspmm_rotary(const void* x, const long long* x_strides, void* out, const
            (T == 1 || 2 * s.tokens_a_group <= T))
         s.tokens_a_group *= 2;
     const int groups = (s.tokens + s.tokens_a_group - 1) / s.tokens_a_group;
+    if (!launch_fits(groups, kRotaryThreads)) return -1;
     int slices = 1;
     while (slices < 64 && groups * slices < 512 && 2 * slices * kRotaryThreads <= s.tokens_a_group * steps) slices *= 2;
     const dim3 grid(groups, slices);

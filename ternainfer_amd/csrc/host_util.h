@@ -80,6 +80,9 @@ void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t
     }, values);
 }
 
+// A launch has fewer than 2^32 threads along a dimension of its grid.
+inline bool launch_fits(long long workgroups, int threads) { return workgroups * threads < 1ll << 32; }
+
 // Launches with more dynamic LDS than this need the opt-in below.
 constexpr int kPlainLds = 64 * 1024;
 

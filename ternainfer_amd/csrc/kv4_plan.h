@@ -28,7 +28,7 @@ inline int kv4_tiles(long long rows, bool many)
 // parts of 1 x 1 token, 1024 slots 9.3 in one, 7.7 in four, 32768 17.2 in 102 of them; 1 x 384 tokens in one 6.1, in three 7.8.
 struct Kv4Plan {
     bool many;
-    int splits, waves;
+    int splits, waves;                         // waves: of few rows
 };
 inline Kv4Plan kv4_plan(int B, int T, int H, int KV, int D, int S)
 {
@@ -61,7 +61,7 @@ inline Kv4Plan kv4_plan(int B, int T, int H, int KV, int D, int S)
     if (rows <= 32) return p;
     const long long most_many = std::min<long long>({kKv4MaxSplits, steps / 8, 256 / (heads * tiles_many)});
     for (long long n = 1; n <= std::max(1ll, most_many); n = next(n, 4))
-        if (const float time = many(n); time < best) best = time, p = Kv4Plan{true, static_cast<int>(n), 8};
+        if (const float time = many(n); time < best) best = time, p = Kv4Plan{true, static_cast<int>(n), 4};
     return p;
 }
 

@@ -996,7 +996,7 @@ TERNA_FUNCTION(rotary_embed, 6)
     const int rc = lib.ternaspmm_rotary(rows.const_data_ptr(), in_strides, out.mutable_data_ptr(), out_strides, x.scalar_type() == at::kFloat, pos.data(), pos.each,
                                         frequency.data(), frequency.pairs(), amplitude, b, t, h, d, adjacent, stream());
     unlocked.end();
-    if (rc != 0) refuse("%s: the library refused the launch", who);
+    if (rc != 0) refuse("%s: more tokens than a launch has room for: fewer than 2^24, or than 2^24 groups of several", who);
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -1157,7 +1157,7 @@ TERNA_FUNCTION(token_logprobs, 3)
     if (logits.dim() != 2 || (logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)) refuse("%s: logits are bfloat16 or float32 [M, V]", who);
     check_device(who, "logits", logits, logits);
     const int64_t m = logits.size(0), v = logits.size(1);
-    if (v < 1 || v > 1 << 19 || m > 1 << 24) refuse("%s: 1 to 2^19 logits in at most 2^24 rows", who);
+    if (v < 1 || v > 1 << 19 || m >= 1 << 24) refuse("%s: 1 to 2^19 logits in fewer than 2^24 rows", who);
     if (top < 0 || top > 64 || top > v) refuse("%s: top is 0 to 64 and at most V", who);
     if (targets != nullptr) {
         if (targets->scalar_type() != at::kLong || targets->dim() != 1 || targets->size(0) != m) refuse("%s: targets are int64 [M]", who);

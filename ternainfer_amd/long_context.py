@@ -68,7 +68,7 @@ def rotary_embed(x: torch.Tensor, pos: torch.Tensor, inv_freq: torch.Tensor, *, 
     """Rotary positions on x [B, T, H, D] (bfloat16 or float32, any strides: a view of a fused projection's rows takes queries and keys in one
     call).  pos int64 [T] or [B, T]; inv_freq float64 [pairs] (`rotary_frequencies`).  Pair j of a head -- dimensions 2j and 2j + 1 when
     `adjacent`, else j and j + pairs -- turns by pos * inv_freq[j], an angle formed in 64 bits; the dimensions from 2 * pairs on stay.
-    `out`: x itself, or rows that share no memory with it."""
+    `out`: x itself, or rows that share no memory with it.  Fewer than 2^24 tokens (more where a workgroup takes several: few heads, or T = 1)."""
     return _lib.native().rotary_embed(x, pos, inv_freq, amplitude, adjacent, out)
 
 
@@ -127,5 +127,5 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
     """Of every row of logits [M, V] (bfloat16 or float32, rows any distance apart): the log probability of its token in `targets` (int64 [M]; NaN
     for one outside the vocabulary, as -1 for padding), the entropy, and the `top` (at most 64) likeliest tokens -- equal logits by lower index,
-    NaN last -- with theirs.  One pass over the logits.  A row with NaN or +inf, or of -inf alone, has NaN for its probabilities and entropy."""
+    NaN last -- with theirs.  One pass over the logits; V up to 2^19, M below 2^24.  A row with NaN or +inf, or of -inf alone, has NaN for its probabilities and entropy."""
     return TokenLogprobs(*_lib.native().token_logprobs(logits, targets, top))

@@ -816,3 +816,49 @@ def test_a_captured_step_of_many_query_heads(b, h, kv, d, slots):
     q = T.kv4_store(x, now, inv, twin, h)
     want, tol = P.attention(q, now, twin, d ** -0.5)
     assert P.same_or_near(out.view(b, 1, h, d), want, tol) <= 0
+
+
+# ---- the most that a launch has room for ---------------------------------------------------------------------------------------------
+
+
+def test_the_most_rows_of_log_probabilities():
+    m = (1 << 24) - 1
+    _say("log probabilities of", m)
+    logits = _randn((m, 2), 400)
+    got = T.token_logprobs(logits, torch.ones(m, dtype=torch.int64, device="cuda"), 1)
+    a, b = logits.double().unbind(-1)
+    peak, gap = torch.maximum(a, b), (a - b).abs()
+    lse = torch.log1p((-gap).exp())
+    # differences below 16 in fp32, an exponential and a logarithm: the same bound as for few logits above
+    for value, want in ((got.logprob, b - peak - lse), (got.top_logprobs[:, 0], -lse), (got.entropy, lse + gap * (-gap).exp() / (1 + (-gap).exp()))):
+        assert ((value.double() - want).abs() <= 40 * 2.0 ** -23 * (1 + want.abs())).all()
+    assert torch.equal(got.top_ids[:, 0], (b > a).long())
+    with pytest.raises(ValueError, match="token_logprobs"):
+        T.token_logprobs(logits[:1].expand(m + 1, 2))
+
+
+def test_the_most_tokens_of_rotary_positions():
+    b = 1 << 23
+    _say("rotary of", 3 * b)
+    x, pos = _randn((b, 3, 1, 2), 401), torch.tensor([5, 70000, -3], device="cuda")
+    inv = torch.tensor([0.37], dtype=torch.float64, device="cuda")
+    _check_rotary(x, T.rotary_embed(x, pos, inv), pos, inv, 1.0, True)
+    with pytest.raises(ValueError, match="rotary_embed"):
+        T.rotary_embed(x[:1].expand(1 << 25, 3, 1, 2), pos, inv)
+
+
+def test_the_most_sequences_of_the_cache():
+    """One slot each: attention's result is its value, exactly."""
+    b, d = (1 << 24) - 8, 64
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("20 GB of queries and rows")
+    _say("attention of", b)
+    cache = T.Kv4Cache(*P.random_cache(b, 1, 1, d, 402))
+    pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+    rows = T.kv4_rows(cache, pos)[1].view(b, d)
+    assert torch.equal(rows[-1000:].double(), P.values(cache.v, cache.v_scale)[-1000:].view(1000, d))
+    q = _randn((1, 1, 1, d), 403).expand(b, 1, 1, d)
+    assert torch.equal(T.kv4_attention(q, pos, cache), rows)
+    more = T.Kv4Cache.empty(1 << 24, 1, 1, d)
+    with pytest.raises(ValueError, match="kv4_attention"):
+        T.kv4_attention(q[:1].expand(1 << 24, 1, 1, d), pos, more)

@@ -1,12 +1,17 @@
 """ternainfer_amd/long_context.py where no GPU is needed: frequencies, sizes, and what is refused before anything is enqueued."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import ternainfer_amd as T
 from ternainfer_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _inv(dim, theta):
@@ -137,6 +142,36 @@ def test_c_entry_points_refuse_before_they_enqueue():
     good = dict(logits=p(64), row=10, fp32=0, targets=p(64), logprob=p(64), entropy=p(64), ids=p(64), lps=p(64), top=3, work=None, M=1, V=10, stream=None)
     refused("ternaspmm_token_logprobs", names, good, [*({n: None} for n in ("logits", "logprob", "entropy", "ids", "lps")), dict(top=-1), dict(top=11), dict(top=65, V=100), dict(M=0), dict(V=0),
                                                       dict(logits=p(65)), dict(logits=p(66), fp32=1), dict(work=p(66)), dict(row=-1), dict(V=(1 << 19) + 1)])
+
+
+LAUNCHES = r"""
+import ctypes
+from ternainfer_amd import _lib
+lib = _lib.load()
+class Kv4(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "k_scale", "v", "v_scale")]
+p, cache, strides = ctypes.c_void_p(64), ctypes.byref(Kv4(64, 64, 64, 64)), (ctypes.c_longlong * 3)(128, 128, 128)
+rotary = lambda b, t, h, d: lib.ternaspmm_rotary(p, strides, ctypes.c_void_p(128), strides, 0, p, 0, p, 1, 1.0, b, t, h, d, 1, None)
+assert rotary(1 << 24, 2, 1, 64) == -1 and rotary(1 << 23, 4, 600, 16) == -1 and rotary(1, 1 << 24, 600, 16) == -1 and rotary(1 << 25, 3, 1, 2) == -1
+store = lambda b, t, h, kv: lib.ternaspmm_kv4_store(p, (h + 2 * kv) * 128, p, 0, p, 64, 1.0, p, cache, b, t, h, kv, 128, 1, 1, None)
+assert store(1 << 24, 1, 16, 16) == -1
+assert lib.ternaspmm_kv4_rows(cache, p, 0, p, p, 1 << 24, 1, 16, 128, 1, None) == -1
+attention = lambda b, t, h, kv: lib.ternaspmm_kv4_attention(p, cache, p, 0, p, None, b, t, h, kv, 64, 1, 1.0, None)
+assert attention(1 << 24, 1, 1, 1) == -1 and attention(1 << 20, 1, 256, 16) == -1 and attention(1 << 16, 16, 256, 256) == -1 and attention(1 << 21, 1, 128, 1) == -1
+step = lambda b, h, kv: lib.ternaspmm_kv4_step(p, (h + 2 * kv) * 64, p, 0, p, 32, 1.0, cache, p, None, b, h, kv, 64, 1, 1.0, 1, None)
+assert step(1 << 24, 1, 1) == -1 and step(1 << 20, 256, 16) == -1 and step(1 << 21, 128, 1) == -1
+assert lib.ternaspmm_kv4_splits(1 << 24, 1, 1, 1, 64, 1) == -1 and lib.ternaspmm_kv4_workspace_bytes(1 << 24, 1, 1, 1, 64, 1) == -1
+assert lib.ternaspmm_kv4_splits((1 << 24) - 8, 1, 1, 1, 64, 1) == 1
+assert lib.ternaspmm_token_logprobs(p, 1, 0, None, None, p, None, None, 0, None, 1 << 24, 1, None) == -1
+assert lib.ternaspmm_token_logprobs_workspace_bytes(1 << 24, 1, 0, 0) == -1 and lib.ternaspmm_token_logprobs_workspace_bytes((1 << 24) - 1, 1, 0, 0) == 0
+print("refused")
+"""
+
+
+def test_sizes_that_a_launch_has_no_room_for_are_refused():
+    """2^32 threads and more.  In a process of its own: one that is not refused ends it at the launch."""
+    r = subprocess.run([sys.executable, "-c", LAUNCHES], capture_output=True, text=True, timeout=120, cwd=ROOT)
+    assert r.returncode == 0 and "refused" in r.stdout, r.stdout + r.stderr
 
 
 def test_python_functions_refuse_tensors_that_are_not_on_the_gpu():
