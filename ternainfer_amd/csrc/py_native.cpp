@@ -135,6 +135,13 @@ float real(PyObject* o)
     return static_cast<float>(v);
 }
 
+bool truth(PyObject* o)
+{
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Refused();                // (a tensor of several elements has none)
+    return v != 0;
+}
+
 template <typename T = void>
 T* data(const at::Tensor* t) { return t == nullptr ? nullptr : static_cast<T*>(t->data_ptr()); }
 
@@ -969,7 +976,7 @@ TERNA_FUNCTION(rotary_embed, 6)
     const at::Tensor* given = optional(a[5]);
     const double amplitude = PyFloat_AsDouble(a[3]);
     if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
-    const int adjacent = PyObject_IsTrue(a[4]);
+    const bool adjacent = truth(a[4]);
     if (x.dim() != 4 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat)) refuse("%s: x is a bfloat16 or float32 [B, T, H, D] tensor", who);
     check_device(who, "x", x, x);
     const int64_t b = x.size(0), t = x.size(1), h = x.size(2), d = x.size(3);
@@ -1046,9 +1053,9 @@ TERNA_FUNCTION(kv4_store, 10)
     const at::Tensor &x = tensor(a[0]), &codes = tensor(a[4]);
     const double amplitude = PyFloat_AsDouble(a[3]);
     if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
-    const Kv4 cache(who, a + 4);
     const int64_t heads = integer32(a[8]);
-    const int adjacent = PyObject_IsTrue(a[9]);
+    const bool adjacent = truth(a[9]);
+    const Kv4 cache(who, a + 4);
     check_device(who, "the cache", codes, codes);
     Guard guard;
     on_device_of(guard, codes);
@@ -1124,9 +1131,9 @@ TERNA_FUNCTION(kv4_step, 11)
     const at::Tensor &x = tensor(a[0]), &codes = tensor(a[4]);
     const double amplitude = PyFloat_AsDouble(a[3]);
     if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
-    const Kv4 cache(who, a + 4);
     const int64_t heads = integer32(a[8]);
-    const int adjacent = PyObject_IsTrue(a[9]);
+    const bool adjacent = truth(a[9]);
+    const Kv4 cache(who, a + 4);
     const float scale = real(a[10]);
     check_device(who, "the cache", codes, codes);
     Guard guard;

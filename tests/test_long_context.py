@@ -208,3 +208,12 @@ def test_the_model_refuses_what_its_cache_does_not_take():
     for tokens, lens in ((torch.zeros((2, 1), dtype=torch.int64), None), (torch.zeros((2, 4), dtype=torch.int64), torch.ones(3))):
         with pytest.raises(ValueError):
             model.score(tokens, lens)
+
+
+def test_what_has_no_truth_value_is_refused_with_its_own_error():
+    f, pos, cache = torch.ones(64, dtype=torch.float64), torch.zeros(1, dtype=torch.int64), T.Kv4Cache.empty(1, 1, 10, 128, device="cpu")
+    rows, both = torch.zeros(1, 384, dtype=torch.bfloat16), torch.tensor([True, False])
+    for call in (lambda: T.rotary_embed(torch.zeros(1, 1, 1, 128), pos, f, adjacent=both), lambda: T.kv4_store(rows, pos, f, cache, 1, adjacent=both),
+                 lambda: T.kv4_step(rows, pos, f, cache, 1, adjacent=both)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()
