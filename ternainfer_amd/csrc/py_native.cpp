@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstdarg>
 #include <optional>
 #include <vector>
@@ -1040,6 +1041,9 @@ at::Tensor projection_rows(const char* who, const at::Tensor& x, const at::Tenso
     if (x.size(0) * heads > 1 << 28 || x.size(0) > 1 << 24) refuse("%s: too many rows", who);
     return x.stride(1) == 1 && x.stride(0) >= x.size(1) && x.stride(0) % 8 == 0 && aligned16(x) ? x : x.clone(at::MemoryFormat::Contiguous);
 }
+// the scale of the scores: None for dim ** -0.5
+std::optional<float> scale_or_none(PyObject* o) { return o == Py_None ? std::nullopt : std::optional<float>(real(o)); }
+float scale_of(const std::optional<float>& given, int64_t dim) { return given ? *given : static_cast<float>(std::pow(static_cast<double>(dim), -0.5)); }
 c10::DataPtr kv4_workspace(int64_t b, int64_t t, int64_t h, const Kv4& cache)
 {
     const long long bytes = lib.ternaspmm_kv4_workspace_bytes(b, t, h, cache.kv, cache.dim, cache.slots);
@@ -1096,13 +1100,14 @@ TERNA_FUNCTION(kv4_rows, 5)
     return pack(unlocked, std::move(k), std::move(v));
 }
 
-// (q [B, H, T, D], pos, k, k_scale, v, v_scale, scale) -> [B * T, H * D]
+// (q [B, H, T, D], pos, k, k_scale, v, v_scale, scale | None) -> [B * T, H * D]
 TERNA_FUNCTION(kv4_attention, 7)
 {
     const char* who = "kv4_attention";
     const at::Tensor &q = tensor(a[0]), &codes = tensor(a[2]);
+    const std::optional<float> given_scale = scale_or_none(a[6]);
     const Kv4 cache(who, a + 2);
-    const float scale = real(a[6]);
+    const float scale = scale_of(given_scale, cache.dim);
     check_device(who, "the cache", codes, codes);
     if (q.dim() != 4 || q.scalar_type() != at::kBFloat16 || q.size(0) != cache.batch || q.size(3) != cache.dim || q.size(1) < 1 || q.size(1) > 4096 || q.size(1) % cache.kv != 0)
         refuse("%s: q is bfloat16 [B, H, T, D] with the cache's B and D and H a multiple of its KV", who);
@@ -1124,7 +1129,7 @@ TERNA_FUNCTION(kv4_attention, 7)
     return THPVariable_Wrap(std::move(out));
 }
 
-// (xqkv, pos, inv_freq, amplitude, k, k_scale, v, v_scale, heads, adjacent, scale) -> [B, H * D]
+// (xqkv, pos, inv_freq, amplitude, k, k_scale, v, v_scale, heads, adjacent, scale | None) -> [B, H * D]
 TERNA_FUNCTION(kv4_step, 11)
 {
     const char* who = "kv4_step";
@@ -1133,8 +1138,9 @@ TERNA_FUNCTION(kv4_step, 11)
     if (amplitude == -1.0 && PyErr_Occurred()) throw Refused();
     const int64_t heads = integer32(a[8]);
     const bool adjacent = truth(a[9]);
+    const std::optional<float> given_scale = scale_or_none(a[10]);
     const Kv4 cache(who, a + 4);
-    const float scale = real(a[10]);
+    const float scale = scale_of(given_scale, cache.dim);
     check_device(who, "the cache", codes, codes);
     Guard guard;
     on_device_of(guard, codes);

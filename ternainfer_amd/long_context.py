@@ -105,14 +105,14 @@ def kv4_rows(cache: Kv4Cache, pos: torch.Tensor):
 def kv4_attention(q: torch.Tensor, pos: torch.Tensor, cache: Kv4Cache, scale: Optional[float] = None) -> torch.Tensor:
     """Attention of q bf16 [B, H, T, D] over the slots 0 .. pos of the cache: bf16 [B * T, H * D].  scale: D ** -0.5 by default.  A negative position
     sees nothing and gives zeros, one past the cache NaN."""
-    return _lib.native().kv4_attention(q, pos, *cache, q.shape[-1] ** -0.5 if scale is None else scale)
+    return _lib.native().kv4_attention(q, pos, *cache, scale)
 
 
 def kv4_step(xqkv: torch.Tensor, pos: torch.Tensor, inv_freq: torch.Tensor, cache: Kv4Cache, n_heads: int, *, amplitude: float = 1.0,
              adjacent: bool = True, scale: Optional[float] = None) -> torch.Tensor:
     """One new token per sequence: `kv4_store` and `kv4_attention` in one launch (two where the slots are split; their own launches for some shapes of
     more than 32 query heads a kv head), with their bits.  xqkv bf16 [B, (H + 2 KV) D], pos int64 [1] or [B, 1]; returns bf16 [B, H * D]."""
-    return _lib.native().kv4_step(xqkv, pos, inv_freq, amplitude, *cache, n_heads, adjacent, (2 * cache.k.shape[-1]) ** -0.5 if scale is None else scale)
+    return _lib.native().kv4_step(xqkv, pos, inv_freq, amplitude, *cache, n_heads, adjacent, scale)
 
 
 class TokenLogprobs(NamedTuple):

@@ -217,3 +217,17 @@ def test_what_has_no_truth_value_is_refused_with_its_own_error():
                  lambda: T.kv4_step(rows, pos, f, cache, 1, adjacent=both)):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
+
+
+def test_the_default_scale_does_not_stand_in_front_of_the_checks():
+    """What is no tensor: TypeError; no query of four dimensions, or one of none: ValueError -- also where the scale is left to the default."""
+    f, pos, cache = torch.ones(64, dtype=torch.float64), torch.zeros(1, dtype=torch.int64), T.Kv4Cache.empty(1, 1, 10, 128, device="cpu")
+    rows = torch.zeros(1, 384, dtype=torch.bfloat16)
+    empty = T.Kv4Cache(*(torch.zeros((1, 1, 10, 0), dtype=torch.uint8) for _ in range(4)))
+    for call in (lambda: T.kv4_attention([1.0], pos, cache), lambda: T.kv4_step([1.0], pos, f, cache, 1), lambda: T.kv4_step(rows, pos, f, (1, 2, 3, 4), 1)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: T.kv4_attention(torch.tensor(1.0), pos, cache), lambda: T.kv4_attention(torch.zeros(1, 1, 1, 0), pos, cache), lambda: T.kv4_step(rows, pos, f, empty, 1),
+                 lambda: T.kv4_step(rows, pos, f, tuple(cache), 1)):
+        with pytest.raises(ValueError, match="kv4_"):
+            call()
