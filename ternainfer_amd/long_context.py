@@ -26,7 +26,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 500000.0, scaling: Option
       {"type": "yarn", "factor", "original_max_position", "beta_fast" = 32, "beta_slow" = 1, "amplitude" = 0.1 ln(factor) + 1}
                                          divided, kept, and between them by a ramp over the pair's index; a larger amplitude (Peng et al.,
                                          "YaRN: Efficient Context Window Extension of Large Language Models")"""
-    if rotary_dim < 2 or rotary_dim % 2 or theta <= 0:
+    if rotary_dim < 2 or rotary_dim % 2 or not 0 < theta < math.inf:
         raise ValueError(f"rotary_frequencies: unsupported rotary_dim={rotary_dim} theta={theta}")
     inv = [theta ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)]
     amplitude = 1.0
@@ -37,7 +37,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 500000.0, scaling: Option
         if kind not in known or not set(need) <= set(scaling) or set(scaling) - {"type", *need, *known[kind]}:
             raise ValueError(f"rotary_frequencies: unsupported scaling {scaling}")
         factor = float(scaling["factor"])
-        if not factor >= 1.0:
+        if not 1.0 <= factor < math.inf:
             raise ValueError(f"rotary_frequencies: a factor of {factor}")
         if kind == "linear":
             inv = [f / factor for f in inv]

@@ -231,3 +231,12 @@ def test_the_default_scale_does_not_stand_in_front_of_the_checks():
                  lambda: T.kv4_step(rows, pos, f, tuple(cache), 1)):
         with pytest.raises(ValueError, match="kv4_"):
             call()
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_frequencies_are_finite(value):
+    with pytest.raises(ValueError, match="rotary_frequencies"):
+        T.rotary_frequencies(64, value, device="cpu")
+    for more in ({"type": "linear"}, {"type": "ntk"}, {"type": "wavelength", "original_max_position": 64}, {"type": "yarn", "original_max_position": 64}):
+        with pytest.raises(ValueError, match="rotary_frequencies"):
+            T.rotary_frequencies(64, 10000.0, {**more, "factor": value}, device="cpu")
