@@ -540,8 +540,8 @@ class Transformer:
 
     def rope_tables(self, max_seq: int, dev):
         """cos / sin of every (cache slot, rotary pair): fp32 [max_seq, 2, head_dim / 2] (cos row, sin row), built
-        once per length; one gather then fetches both rows of a position."""
-        key = (max_seq, str(dev))
+        once per length and set of frequencies; one gather then fetches both rows of a position."""
+        key = (max_seq, str(dev), self.rope_key())
         tables = getattr(self, "_rope_tables", None)
         if tables is None or tables[0] != key:
             a = self.args
@@ -557,10 +557,15 @@ class Transformer:
 
     def rope_frequencies(self, dev):
         """(inv_freq, amplitude) of the rotary positions, as the 4-bit cache's kernels take them; kept: a captured step holds the pointer."""
-        held = getattr(self, "_rope_frequencies", None)
-        if held is None or held[0].device != dev:
-            self._rope_frequencies = held = rotary_frequencies(self.args.head_dim, self.args.rope_theta, self.args.rope_scaling, dev)
-        return held
+        key, held = (str(dev), self.rope_key()), getattr(self, "_rope_frequencies", None)
+        if held is None or held[0] != key:
+            self._rope_frequencies = held = (key, rotary_frequencies(self.args.head_dim, self.args.rope_theta, self.args.rope_scaling, dev))
+        return held[1]
+
+    def rope_key(self):
+        """What the model's rotary positions follow from: tables and frequencies that are kept are those of the arguments as they are now."""
+        a = self.args
+        return (a.head_dim, a.rope_theta, None if a.rope_scaling is None else repr(a.rope_scaling))
 
     def no_rope_table(self, dev):
         """What stands in for the tables where nobody reads them: one position (kept, as the frequencies are)."""

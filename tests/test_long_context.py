@@ -240,3 +240,21 @@ def test_frequencies_are_finite(value):
     for more in ({"type": "linear"}, {"type": "ntk"}, {"type": "wavelength", "original_max_position": 64}, {"type": "yarn", "original_max_position": 64}):
         with pytest.raises(ValueError, match="rotary_frequencies"):
             T.rotary_frequencies(64, 10000.0, {**more, "factor": value}, device="cpu")
+
+
+def test_the_models_positions_follow_its_arguments():
+    """Frequencies and tables that are kept from one call to the next: of the base and the scaling that the model has then."""
+    from ternainfer_amd.model import ModelArgs, Transformer
+    model, dev = Transformer.__new__(Transformer), torch.device("cpu")
+    model.args = ModelArgs(dim=256, n_layers=1, n_heads=4, n_kv_heads=2)
+    scaling = {"type": "linear", "factor": 2.0}
+    seen = []
+    for change in (lambda: None, lambda: setattr(model.args, "rope_scaling", scaling), lambda: scaling.update(factor=8.0), lambda: setattr(model.args, "rope_theta", 10000.0)):
+        change()
+        inv, _ = model.rope_frequencies(dev)
+        assert torch.equal(inv, T.rotary_frequencies(64, model.args.rope_theta, model.args.rope_scaling, device="cpu")[0])
+        assert model.rope_frequencies(dev)[0] is inv                             # kept
+        table = model.rope_tables(7, dev)
+        assert (table[6, 0].double() - (6 * inv).cos()).abs().max() < 1e-5 and model.rope_tables(7, dev) is table
+        seen.append(inv)
+    assert len({tuple(inv.tolist()) for inv in seen}) == 4
