@@ -68,7 +68,7 @@ def rotary_embed(x: torch.Tensor, pos: torch.Tensor, inv_freq: torch.Tensor, *, 
     """Rotary positions on x [B, T, H, D] (bfloat16 or float32, any strides: a view of a fused projection's rows takes queries and keys in one
     call).  pos int64 [T] or [B, T]; inv_freq float64 [pairs] (`rotary_frequencies`).  Pair j of a head -- dimensions 2j and 2j + 1 when
     `adjacent`, else j and j + pairs -- turns by pos * inv_freq[j], an angle formed in 64 bits; the dimensions from 2 * pairs on stay.
-    `out`: x itself, or rows that share no memory with it.  Fewer than 2^24 tokens (more where a workgroup takes several: few heads, or T = 1)."""
+    `out`: x itself, or rows that lie apart from it, from their first element to their last.  Fewer than 2^24 tokens (more where a workgroup takes several: few heads, or T = 1)."""
     return _lib.native().rotary_embed(x, pos, inv_freq, amplitude, adjacent, out)
 
 

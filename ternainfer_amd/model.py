@@ -632,9 +632,9 @@ class Transformer:
     def make_cache(self, bsz: int, max_seq: int, bits: int = 16):
         """The key/value cache of every block, for bsz sequences of max_seq tokens.  bits=4: `Kv4Cache`s, 4.25 bits a value and any length (heads of 64 or
         128 dimensions); it needs the fused kernels, and a step is its launches, never one (whole_step).
-        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 652 and
-        896, of 8192 1069 and 981, of 131072 1417 in 4; 8 of 1528 1132 and 1212, of 8192 1727 and 1443; 16 of 8192 2659 and 1726; 32 of 8192 4381 and
-        2412.  A prompt of 2048 tokens 6.6 and 6.7 ms, of 8192 29.5 and 27.0, of 32768 219 in 4."""
+        For length and for many sequences: us a step of the 30-block shape with the cache filled to 95 %, 16 bits and 4: one sequence of 384 slots 654 and
+        901, of 8192 1069 and 979, of 131072 1400 in 4; 8 of 1528 1133 and 1219, of 8192 1728 and 1452; 16 of 8192 2661 and 1762; 32 of 8192 4402 and
+        2413.  A prompt of 2048 tokens 6.5 and 6.7 ms, of 8192 30.1 and 26.7, of 32768 212 in 4."""
         a = self.args
         if bits == 4:
             return [Kv4Cache.empty(bsz, a.n_kv_heads, max_seq, a.head_dim, self.tok_embeddings.device) for _ in range(a.n_layers)]
