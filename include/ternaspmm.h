@@ -739,6 +739,51 @@ long long ternaspmm_token_logprobs_workspace_bytes(int M, int V, int fp32, int t
 int ternaspmm_token_logprobs(const void* logits, long long row, int fp32, const long long* targets, float* logprob, float* entropy, long long* top_ids,
                              float* top_logprobs, int top, void* workspace, int M, int V, terna_stream stream);
 
+/* ---- Drafted tokens and 8-bit projections (no counterpart in the reference) -------------------------------------------------------
+ * Conventions as in the section above: 0, or -1 with nothing enqueued; scratch memory of the caller's, not shared by calls that overlap.
+ *
+ * A tree of T nodes (1 .. 512) a sequence: parents[i] int64 in 0 .. i - 1, or -1 for a root; with any other parent, and behind such a node, it is none
+ * (padding).  ternaspmm_draft_tree: mask int64 [B][T][(T + 63) / 64], bit j of a row for node j, set for the node and its ancestors (padding: no bit),
+ * and depth int64 [B][T], 0 for a root, -1 for padding. */
+int ternaspmm_draft_tree(const long long* parents, long long* mask, long long* depth, int B, int T, terna_stream stream);
+/* Attention of the nodes: q, k and v bf16 with strides (elements) of [B][H][T][D] and [B][KV][S][D]'s first three dimensions, the last contiguous; every
+ * address and stride a multiple of 16 bytes, a slot's stride below 2^24; D 64 or 128, S <= 2^25, B * T * H <= 2^28.  Node j's key and value lie in slot start[b] + j.  Row (b, i) of out bf16 [B * T][H * D]:
+ * the softmax of scale * q . k over the slots 0 .. start[b] - 1 and those of the nodes in its mask -- int64 [T][(T + 63) / 64], with per_sequence
+ * [B][T][...] -- times the values.  A row without a bit, and a sequence with start[b] < 0: zeros.  A row that sees a slot from S on, or start[b] > S: NaN.
+ * A slot that a row does not see does not reach it, whatever it holds.  scale is finite.
+ * workspace: ternaspmm_tree_attention_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for long caches of few rows. */
+long long ternaspmm_tree_attention_workspace_bytes(int B, int T, int H, int KV, int D, int S);
+int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, const terna_bf16* k, const long long* k_strides, const terna_bf16* v, const long long* v_strides,
+                             const long long* start, const long long* mask, int per_sequence, terna_bf16* out, void* workspace, int B, int T, int H, int KV, int D, int S,
+                             float scale, terna_stream stream);
+/* The branch that greedy decoding takes: logits (bf16, or fp32; rows `row` elements apart) of the nodes b * T + i, tokens int64 [B][T].  From node 0 on,
+ * while a child of the node -- the first of them -- carries the token of the node's largest logit (equal ones: the lowest; NaN never wins), it is next.
+ * path int64 [B][T]: those nodes, then -1; count int64 [B]; next int64 [B]: the token behind the last.  Where node 0 is no root, count 0 and next -1.
+ * V <= 2^19.  workspace: ternaspmm_tree_accept_workspace_bytes, 8-byte aligned. */
+long long ternaspmm_tree_accept_workspace_bytes(int B, int T, int V, int fp32);
+int ternaspmm_tree_accept(const void* logits, long long row, int fp32, const long long* tokens, const long long* parents, long long* path, long long* count, long long* next,
+                          void* workspace, int B, int T, int V, terna_stream stream);
+/* Rows of n caches, of any types: slot start[b] + path[b][i] -> start[b] + i for i < count[b] (at most T), of every head.  A path ascends, as ternaspmm_tree_accept's do; a row
+ * outside the cache, one in front of its place, and the rows of a sequence whose start lies outside the cache stay.  Strides and `bytes` of a row in bytes, slot >= bytes. */
+typedef struct ternaspmm_cache_rows {
+    void* rows;
+    long long sequence, head, slot;
+    int heads, slots, bytes;
+} ternaspmm_cache_rows;
+int ternaspmm_cache_move(const ternaspmm_cache_rows* caches, int n, const long long* start, const long long* path, const long long* count, int B, int T, terna_stream stream);
+
+/* Rows in 8 bits: `packed` holds R rows of K as blocks of 16 rows by 64 columns, 1 KB each, blocks of a row band adjacent, (R + 15) / 16 bands of 2 * ((K + 127) / 128)
+ * blocks; byte ((k % 64) / 16 * 16 + r % 16) * 16 + k % 16 of its block is element (r, k).  Columns from K on are zeros, what rows from R on hold does not matter.  scale fp32 [R]: row r stands for
+ * scale[r] * integer.  ternaspmm_int8_bytes: of `packed` (-1: sizes refused; K <= 131056, R <= 2^28).
+ * ternaspmm_int8_quantise: rows of bf16 (or fp32) x, `row` elements apart: scale = max|x| / 127, integers rint(x * (127 / max|x|)); a row whose
+ * magnitudes all lie below 2^-120 is zeros with scale 0, one with NaN or infinity zeros with scale NaN.
+ * ternaspmm_int8_pack: int8 rows as they are.
+ * ternaspmm_int8_linear: out [M][N] (bf16, or fp32) = float(sum_k x w) * x_scale[m] * w_scale[n], sums exact in 32 bits; x and w packed rows of K. */
+long long ternaspmm_int8_bytes(int R, int K);
+int ternaspmm_int8_quantise(const void* x, long long row, int fp32, void* packed, float* scale, int R, int K, terna_stream stream);
+int ternaspmm_int8_pack(const void* x, long long row, void* packed, int R, int K, terna_stream stream);
+int ternaspmm_int8_linear(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out, int fp32, int M, int N, int K, terna_stream stream);
+
 /* Library version string, e.g. "ternaspmm-gfx950 0.1". */
 const char* ternaspmm_version(void);
 

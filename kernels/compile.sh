@@ -41,6 +41,9 @@ compile abi_rotary.hip abi_rotary.o
 # (the output accumulators are rescaled between matrix instructions here too)
 compile abi_kv4.hip abi_kv4.o -mllvm -amdgpu-mfma-vgpr-form
 compile abi_logprobs.hip abi_logprobs.o
+# (and here)
+compile abi_tree.hip abi_tree.o -mllvm -amdgpu-mfma-vgpr-form
+compile abi_int8.hip abi_int8.o
 compile abi_probe.hip abi_probe.o
 compile format_host.cpp format_host.o
 # The host path of the Python package: a CPython module on torch's C++ headers, bound to the library at run time.  The library

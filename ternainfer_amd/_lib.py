@@ -112,6 +112,16 @@ PROTOTYPES = {
     "ternaspmm_kv4_step": ([_vp, ctypes.c_longlong, _vp, _ci, _vp, _ci, ctypes.c_double, _vp, _vp, _vp] + [_ci] * 5 + [ctypes.c_float, _ci, _vp], _ci),
     "ternaspmm_token_logprobs_workspace_bytes": ([_ci] * 4, ctypes.c_longlong),
     "ternaspmm_token_logprobs": ([_vp, ctypes.c_longlong, _ci] + [_vp] * 5 + [_ci, _vp, _ci, _ci, _vp], _ci),
+    "ternaspmm_draft_tree": ([_vp] * 3 + [_ci, _ci, _vp], ctypes.c_int),
+    "ternaspmm_tree_attention_workspace_bytes": ([_ci] * 6, ctypes.c_longlong),
+    "ternaspmm_tree_attention": ([_vp] * 8 + [_ci, _vp, _vp] + [_ci] * 6 + [ctypes.c_float, _vp], ctypes.c_int),
+    "ternaspmm_tree_accept_workspace_bytes": ([_ci] * 4, ctypes.c_longlong),
+    "ternaspmm_tree_accept": ([_vp, ctypes.c_longlong, _ci] + [_vp] * 6 + [_ci] * 3 + [_vp], ctypes.c_int),
+    "ternaspmm_cache_move": ([_vp, _ci] + [_vp] * 3 + [_ci, _ci, _vp], ctypes.c_int),
+    "ternaspmm_int8_bytes": ([_ci, _ci], ctypes.c_longlong),
+    "ternaspmm_int8_quantise": ([_vp, ctypes.c_longlong, _ci, _vp, _vp, _ci, _ci, _vp], ctypes.c_int),
+    "ternaspmm_int8_pack": ([_vp, ctypes.c_longlong, _vp, _ci, _ci, _vp], ctypes.c_int),
+    "ternaspmm_int8_linear": ([_vp] * 5 + [_ci] * 4 + [_vp], ctypes.c_int),
     "ternaspmm_version": ([], ctypes.c_char_p),
 }
 

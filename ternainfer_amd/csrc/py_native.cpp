@@ -72,7 +72,17 @@ namespace {
     X(ternaspmm_kv4_attention)                                                                                         \
     X(ternaspmm_kv4_step)                                                                                              \
     X(ternaspmm_token_logprobs_workspace_bytes)                                                                        \
-    X(ternaspmm_token_logprobs)
+    X(ternaspmm_token_logprobs)                                                                                        \
+    X(ternaspmm_draft_tree)                                                                                            \
+    X(ternaspmm_tree_attention_workspace_bytes)                                                                        \
+    X(ternaspmm_tree_attention)                                                                                        \
+    X(ternaspmm_tree_accept_workspace_bytes)                                                                           \
+    X(ternaspmm_tree_accept)                                                                                           \
+    X(ternaspmm_cache_move)                                                                                            \
+    X(ternaspmm_int8_bytes)                                                                                            \
+    X(ternaspmm_int8_quantise)                                                                                         \
+    X(ternaspmm_int8_pack)                                                                                             \
+    X(ternaspmm_int8_linear)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     TERNA_ENTRY_POINTS(X)
@@ -1202,6 +1212,262 @@ TERNA_FUNCTION(token_logprobs, 3)
     return pack(unlocked, std::move(logprob), std::move(entropy), std::move(ids), std::move(values));
 }
 
+// ---- drafted tokens, 8-bit projections: tensors of any device here too
+const long long* longs(const at::Tensor& t) { return reinterpret_cast<const long long*>(t.const_data_ptr<int64_t>()); }
+long long* mutable_longs(at::Tensor& t) { return reinterpret_cast<long long*>(t.mutable_data_ptr<int64_t>()); }
+
+constexpr int64_t kMaxNodes = 512;
+// int64 [B, T] of a tree's nodes, contiguous
+at::Tensor nodes_of(const char* who, const char* name, PyObject* o)
+{
+    const at::Tensor& t = tensor(o);
+    if (t.scalar_type() != at::kLong || t.dim() != 2 || t.size(1) > kMaxNodes || t.size(0) > 65535) refuse("%s: %s is int64 [B, T], of at most 65535 sequences of 512 nodes", who, name);
+    check_device(who, name, t, t);
+    return t;
+}
+// int64 [B]
+void check_each(const char* who, const char* name, const at::Tensor& t, int64_t batch, const at::Tensor& with)
+{
+    if (t.scalar_type() != at::kLong || t.dim() != 1 || t.size(0) != batch) refuse("%s: %s is int64 [B] with B = %lld", who, name, static_cast<long long>(batch));
+    check_device(who, name, t, with);
+}
+
+// (parents) -> (mask [B, T, W], depth [B, T])
+TERNA_FUNCTION(draft_tree, 1)
+{
+    const char* who = "draft_tree";
+    const at::Tensor parents = nodes_of(who, "parents", a[0]);
+    const int64_t b = parents.size(0), t = parents.size(1);
+    Guard guard;
+    on_device_of(guard, parents);
+    Unlocked unlocked;
+    const at::Tensor rows = parents.contiguous();
+    at::Tensor mask = make({b, t, (t + 63) / 64}, at::kLong, parents), depth = make({b, t}, at::kLong, parents);
+    const int rc = depth.numel() == 0 ? 0 : lib.ternaspmm_draft_tree(longs(rows), mutable_longs(mask), mutable_longs(depth), b, t, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return pack(unlocked, std::move(mask), std::move(depth));
+}
+
+// (q [B, H, T, D], k, v [B, KV, S, D], start [B], mask [T, W] | [B, T, W], scale | None) -> [B * T, H * D]
+TERNA_FUNCTION(tree_attention, 6)
+{
+    const char* who = "tree_attention";
+    const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &start = tensor(a[3]), &mask = tensor(a[4]);
+    const std::optional<float> given_scale = scale_or_none(a[5]);
+    if (k.dim() != 4 || v.dim() != 4 || k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16 || k.sizes() != v.sizes())
+        refuse("%s: the cache's keys and values are bfloat16 [B, KV, S, D]", who);
+    check_device(who, "the cache", k, k);
+    check_device(who, "the cache", v, k);
+    const int64_t b = k.size(0), kv = k.size(1), s = k.size(2), d = k.size(3);
+    if ((d != 64 && d != 128) || kv < 1 || s < 1 || s > 1 << 25) refuse("%s: a cache has heads of 64 or 128 dimensions and 1 to 2^25 slots", who);
+    for (const at::Tensor* t : {&k, &v})
+        if (t->stride(3) != 1 || (t->stride(0) & 7) || (t->stride(1) & 7) || (t->stride(2) & 7) || t->stride(2) >= 1 << 24 || !aligned16(*t))
+            refuse("%s: the cache's rows are contiguous, each from a multiple of 16 bytes on, slots fewer than 2^24 elements apart", who);
+    if (q.dim() != 4 || q.scalar_type() != at::kBFloat16 || q.size(0) != b || q.size(3) != d || q.size(1) < 1 || q.size(1) > 4096 || q.size(1) % kv != 0)
+        refuse("%s: q is bfloat16 [B, H, T, D] with the cache's B and D and H a multiple of its KV", who);
+    check_device(who, "q", q, k);
+    const int64_t h = q.size(1), t = q.size(2), words = (t + 63) / 64;
+    if (t > kMaxNodes || b * t * h > 1 << 28) refuse("%s: at most 512 nodes a tree, 2^28 rows of all heads", who);
+    check_each(who, "start", start, b, k);
+    const bool each = mask.dim() == 3;
+    if (mask.scalar_type() != at::kLong || (!each && mask.dim() != 2) || (each && mask.size(0) != b) || mask.size(-2) != t || mask.size(-1) != words)
+        refuse("%s: mask is int64 [T, W] or [B, T, W] with W = (T + 63) / 64", who);
+    check_device(who, "mask", mask, k);
+    const float scale = scale_of(given_scale, d);
+    if (!std::isfinite(scale)) refuse("%s: a scale that is not finite", who);
+    Guard guard;
+    on_device_of(guard, k);
+    Unlocked unlocked;
+    at::Tensor out = make({b * t, h * d}, at::kBFloat16, k);
+    if (out.numel() == 0) return wrap(std::move(out), unlocked);
+    const at::Tensor rows = q.stride(3) == 1 && !(q.stride(0) & 7) && !(q.stride(1) & 7) && !(q.stride(2) & 7) && aligned16(q) ? q : q.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor starts = start.contiguous(), masks = mask.contiguous();
+    const long long q_strides[3] = {rows.stride(0), rows.stride(1), rows.stride(2)}, k_strides[3] = {k.stride(0), k.stride(1), k.stride(2)},
+                    v_strides[3] = {v.stride(0), v.stride(1), v.stride(2)};
+    const long long bytes = lib.ternaspmm_tree_attention_workspace_bytes(b, t, h, kv, d, s);
+    const c10::DataPtr work = bytes > 0 ? device_allocator()->allocate(bytes) : c10::DataPtr();
+    const int rc = lib.ternaspmm_tree_attention(data<terna_bf16>(&rows), q_strides, data<terna_bf16>(&k), k_strides, data<terna_bf16>(&v), v_strides, longs(starts), longs(masks), each,
+                                                data<terna_bf16>(&out), work.get(), b, t, h, kv, d, s, scale, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// (logits [B, T, V], tokens, parents) -> (path [B, T], count [B], next [B])
+TERNA_FUNCTION(tree_accept, 3)
+{
+    const char* who = "tree_accept";
+    const at::Tensor& logits = tensor(a[0]);
+    const at::Tensor tokens = nodes_of(who, "tokens", a[1]), parents = nodes_of(who, "parents", a[2]);
+    if (logits.dim() != 3 || (logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)) refuse("%s: logits are bfloat16 or float32 [B, T, V]", who);
+    check_device(who, "logits", logits, logits);
+    const int64_t b = logits.size(0), t = logits.size(1), v = logits.size(2);
+    if (t < 1 || v < 1 || v > 1 << 19) refuse("%s: 1 to 512 nodes, 1 to 2^19 logits", who);
+    for (const at::Tensor* x : {&tokens, &parents})
+        if (x->size(0) != b || x->size(1) != t) refuse("%s: tokens and parents are [B, T] as the logits' rows", who);
+    check_device(who, "tokens", tokens, logits);
+    check_device(who, "parents", parents, logits);
+    Guard guard;
+    on_device_of(guard, logits);
+    Unlocked unlocked;
+    at::Tensor path = make({b, t}, at::kLong, logits), count = make({b}, at::kLong, logits), next = make({b}, at::kLong, logits);
+    int rc = 0;
+    if (b > 0) {
+        const bool fp32 = logits.scalar_type() == at::kFloat;
+        const at::Tensor rows = (v == 1 || logits.stride(2) == 1) && (b == 1 || t == 1 || logits.stride(0) == t * logits.stride(1)) ? logits : logits.contiguous();
+        const at::Tensor drafted = tokens.contiguous(), of = parents.contiguous();
+        const c10::DataPtr work = device_allocator()->allocate(std::max(0ll, static_cast<long long>(lib.ternaspmm_tree_accept_workspace_bytes(b, t, v, fp32))));
+        rc = lib.ternaspmm_tree_accept(rows.const_data_ptr(), t == 1 ? rows.stride(0) : rows.stride(1), fp32, longs(drafted), longs(of), mutable_longs(path), mutable_longs(count),
+                                       mutable_longs(next), work.get(), b, t, v, stream());
+    }
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return pack(unlocked, std::move(path), std::move(count), std::move(next));
+}
+
+// ([cache [B, heads, S, ...] ...], start [B], path [B, T], count [B])
+TERNA_FUNCTION(cache_move, 4)
+{
+    const char* who = "cache_move";
+    const at::Tensor path = nodes_of(who, "path", a[2]);
+    const at::Tensor &start = tensor(a[1]), &count = tensor(a[3]);
+    const int64_t b = path.size(0), t = path.size(1);
+    check_each(who, "start", start, b, path);
+    check_each(who, "count", count, b, path);
+    if (!PyTuple_Check(a[0]) && !PyList_Check(a[0])) refuse("%s: caches is a list of tensors", who);
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(a[0]);
+    std::vector<ternaspmm_cache_rows> caches(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor& c = tensor(PySequence_Fast_GET_ITEM(a[0], i));
+        if (c.dim() != 4 || c.size(0) != b || c.size(1) > 65535 || c.size(2) > INT32_MAX || c.size(3) > 1 << 20) refuse("%s: a cache is [B, heads, S, D] with the path's B", who);
+        check_device(who, "a cache", c, path);
+        if (c.numel() != 0 && ((c.size(3) > 1 && c.stride(3) != 1) || overlaps_itself(c) || c.stride(2) < c.size(3))) refuse("%s: a cache's rows are contiguous and apart from each other", who);
+        const long long size = c.element_size();
+        const bool empty = c.numel() == 0;
+        caches[i] = ternaspmm_cache_rows{empty ? nullptr : c.mutable_data_ptr(), c.stride(0) * size, c.stride(1) * size, c.stride(2) * size, static_cast<int>(c.size(1)),
+                                         static_cast<int>(c.size(2)), static_cast<int>(c.size(3) * size)};
+    }
+    caches.erase(std::remove_if(caches.begin(), caches.end(), [](const ternaspmm_cache_rows& c) { return c.rows == nullptr; }), caches.end());
+    std::vector<const void*> sorted;
+    for (const ternaspmm_cache_rows& c : caches) sorted.push_back(c.rows);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) refuse("%s: a cache is given twice", who);
+    Guard guard;
+    on_device_of(guard, path);
+    Unlocked unlocked;
+    const at::Tensor starts = start.contiguous(), lines = path.contiguous(), counts = count.contiguous();
+    const int rc = caches.empty() || path.numel() == 0 ? 0 : lib.ternaspmm_cache_move(caches.data(), static_cast<int>(caches.size()), longs(starts), longs(lines), longs(counts), b, t, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    Py_RETURN_NONE;
+}
+
+constexpr int64_t kInt8MaxRows = 1 << 28, kInt8MaxK = 131056;
+// rows [R, K] of a type that the kernels read
+void check_int8_rows(const char* who, const at::Tensor& x)
+{
+    check_device(who, "the rows", x, x);
+    if (x.dim() != 2 || x.size(1) < 1 || x.size(1) > kInt8MaxK || x.size(0) > kInt8MaxRows) refuse("%s: rows [R, K] of 1 to 131056 columns, at most 2^28 of them", who);
+}
+at::Tensor rows_in_order(const at::Tensor& x) { return (x.size(1) == 1 || x.stride(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous(); }
+
+// (x [R, K] bf16 | fp32) -> (packed, scale [R])
+TERNA_FUNCTION(int8_quantise, 1)
+{
+    const char* who = "quantise_rows";
+    const at::Tensor& x = tensor(a[0]);
+    if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) refuse("%s: rows are bfloat16 or float32", who);
+    check_int8_rows(who, x);
+    const int64_t r = x.size(0), k = x.size(1);
+    Guard guard;
+    on_device_of(guard, x);
+    Unlocked unlocked;
+    const at::Tensor rows = rows_in_order(x);
+    at::Tensor packed = make({r == 0 ? 0 : lib.ternaspmm_int8_bytes(r, k)}, at::kByte, x), scale = make({r}, at::kFloat, x);
+    const int rc = r == 0 ? 0
+                          : lib.ternaspmm_int8_quantise(rows.const_data_ptr(), rows.stride(0), x.scalar_type() == at::kFloat, packed.mutable_data_ptr(), data<float>(&scale), r, k, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return pack(unlocked, std::move(packed), std::move(scale));
+}
+
+// (q int8 [R, K]) -> packed
+TERNA_FUNCTION(int8_pack, 1)
+{
+    const char* who = "int8_rows";
+    const at::Tensor& x = tensor(a[0]);
+    if (x.scalar_type() != at::kChar) refuse("%s: rows are int8", who);
+    check_int8_rows(who, x);
+    const int64_t r = x.size(0), k = x.size(1);
+    Guard guard;
+    on_device_of(guard, x);
+    Unlocked unlocked;
+    const at::Tensor rows = rows_in_order(x);
+    at::Tensor packed = make({r == 0 ? 0 : lib.ternaspmm_int8_bytes(r, k)}, at::kByte, x);
+    const int rc = r == 0 ? 0 : lib.ternaspmm_int8_pack(rows.const_data_ptr(), rows.stride(0), packed.mutable_data_ptr(), r, k, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(packed));
+}
+
+// packed rows and their scales, of R rows and K columns
+struct Int8Side {
+    at::Tensor packed, scale;
+
+    Int8Side(const char* who, PyObject* p, PyObject* s, int64_t r, int64_t k, const at::Tensor& with) : packed(tensor(p)), scale(tensor(s))
+    {
+        check_device(who, "packed rows", packed, with);
+        check_device(who, "scales", scale, with);
+        if (r < 0 || r > kInt8MaxRows || k < 1 || k > kInt8MaxK || packed.scalar_type() != at::kByte || !packed.is_contiguous() || !aligned16(packed) ||
+            packed.numel() != (r == 0 ? 0 : lib.ternaspmm_int8_bytes(r, k)) || scale.scalar_type() != at::kFloat || scale.dim() != 1 || scale.size(0) != r)
+            refuse("%s: packed rows of another size, or scales that are not float32, one a row", who);
+        scale = scale.contiguous();
+    }
+};
+
+// (x | packed, x_scale | None, M, w packed, w_scale, N, K, float32) -> [M, N]
+TERNA_FUNCTION(int8_linear, 8)
+{
+    const char* who = "int8_linear";
+    const at::Tensor& x = tensor(a[0]);
+    const bool given = a[1] != Py_None, fp32 = truth(a[7]);
+    const int64_t n = integer(a[5]), k = integer(a[6]);
+    check_device(who, "x", x, x);
+    const Int8Side w(who, a[3], a[4], n, k, x);
+    int64_t m = integer(a[2]);
+    if (!given) {
+        if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) refuse("%s: x is bfloat16 or float32 [M, K], or rows in 8 bits", who);
+        check_int8_rows(who, x);
+        if (x.size(1) != k) refuse("%s: x has %lld columns, the weights %lld", who, static_cast<long long>(x.size(1)), static_cast<long long>(k));
+        m = x.size(0);
+    }
+    std::optional<Int8Side> rows8;
+    Guard guard;
+    on_device_of(guard, x);
+    if (given) rows8.emplace(who, a[0], a[1], m, k, x);
+    Unlocked unlocked;
+    at::Tensor out = make({m, n}, fp32 ? at::kFloat : at::kBFloat16, x);
+    if (out.numel() == 0) return wrap(std::move(out), unlocked);
+    c10::DataPtr held;
+    const void* packed = given ? rows8->packed.const_data_ptr() : nullptr;
+    const float* scale = given ? rows8->scale.const_data_ptr<float>() : nullptr;
+    int rc = 0;
+    if (!given) {
+        const at::Tensor rows = rows_in_order(x);
+        const long long bytes = lib.ternaspmm_int8_bytes(m, k);
+        held = device_allocator()->allocate(bytes + 4 * m);
+        packed = held.get();
+        float* const scales = reinterpret_cast<float*>(static_cast<uint8_t*>(held.get()) + bytes);
+        scale = scales;
+        rc = lib.ternaspmm_int8_quantise(rows.const_data_ptr(), rows.stride(0), x.scalar_type() == at::kFloat, held.get(), scales, m, k, stream());
+    }
+    if (rc == 0) rc = lib.ternaspmm_int8_linear(packed, scale, w.packed.const_data_ptr(), w.scale.const_data_ptr<float>(), out.mutable_data_ptr(), fp32, m, n, k, stream());
+    unlocked.end();
+    if (rc != 0) refuse("%s: the library refused the launch", who);
+    return THPVariable_Wrap(std::move(out));
+}
+
 // (path of libternaspmm.so)
 TERNA_FUNCTION(init, 1)
 {
@@ -1227,7 +1493,9 @@ PyMethodDef methods[] = {METHOD(init), METHOD(bit_linear), METHOD(bit_linear_bf1
                          METHOD(linear_bf16_packed), METHOD(rmsnorm_quant), METHOD(relu2_mul_rmsnorm_quant), METHOD(quant_from_stats),
                          METHOD(fused_linear), METHOD(fused_linear_own_stats), METHOD(prompt_attention), METHOD(decode_attention), METHOD(block),
                          METHOD(attention_merge_rmsnorm_quant), METHOD(step_attention_merge), METHOD(step_inputs), METHOD(prompt_inputs), METHOD(decode_step),
-                         METHOD(rotary_embed), METHOD(kv4_store), METHOD(kv4_rows), METHOD(kv4_attention), METHOD(kv4_step), METHOD(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(rotary_embed), METHOD(kv4_store), METHOD(kv4_rows), METHOD(kv4_attention), METHOD(kv4_step), METHOD(token_logprobs),
+                         METHOD(draft_tree), METHOD(tree_attention), METHOD(tree_accept), METHOD(cache_move), METHOD(int8_quantise), METHOD(int8_pack), METHOD(int8_linear),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
