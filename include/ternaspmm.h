@@ -778,11 +778,14 @@ int ternaspmm_cache_move(const ternaspmm_cache_rows* caches, int n, const long l
  * ternaspmm_int8_quantise: rows of bf16 (or fp32) x, `row` elements apart: scale = max|x| / 127, integers rint(x * (127 / max|x|)); a row whose
  * magnitudes all lie below 2^-120 is zeros with scale 0, one with NaN or infinity zeros with scale NaN.
  * ternaspmm_int8_pack: int8 rows as they are.
- * ternaspmm_int8_linear: out [M][N] (bf16, or fp32) = float(sum_k x w) * x_scale[m] * w_scale[n], sums exact in 32 bits; x and w packed rows of K. */
+ * ternaspmm_int8_linear: out [M][N] (bf16, or fp32) = float(sum_k x w) * x_scale[m] * w_scale[n], sums exact in 32 bits; x and w packed rows of K.
+ * workspace: ternaspmm_int8_linear_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for few rows and channels of many columns. */
 long long ternaspmm_int8_bytes(int R, int K);
 int ternaspmm_int8_quantise(const void* x, long long row, int fp32, void* packed, float* scale, int R, int K, terna_stream stream);
 int ternaspmm_int8_pack(const void* x, long long row, void* packed, int R, int K, terna_stream stream);
-int ternaspmm_int8_linear(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out, int fp32, int M, int N, int K, terna_stream stream);
+long long ternaspmm_int8_linear_workspace_bytes(int M, int N, int K);
+int ternaspmm_int8_linear(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out, int fp32, void* workspace, int M, int N, int K,
+                          terna_stream stream);
 
 /* Library version string, e.g. "ternaspmm-gfx950 0.1". */
 const char* ternaspmm_version(void);

@@ -121,7 +121,8 @@ PROTOTYPES = {
     "ternaspmm_int8_bytes": ([_ci, _ci], ctypes.c_longlong),
     "ternaspmm_int8_quantise": ([_vp, ctypes.c_longlong, _ci, _vp, _vp, _ci, _ci, _vp], ctypes.c_int),
     "ternaspmm_int8_pack": ([_vp, ctypes.c_longlong, _vp, _ci, _ci, _vp], ctypes.c_int),
-    "ternaspmm_int8_linear": ([_vp] * 5 + [_ci] * 4 + [_vp], ctypes.c_int),
+    "ternaspmm_int8_linear_workspace_bytes": ([_ci] * 3, ctypes.c_longlong),
+    "ternaspmm_int8_linear": ([_vp] * 5 + [_ci, _vp] + [_ci] * 3 + [_vp], ctypes.c_int),
     "ternaspmm_version": ([], ctypes.c_char_p),
 }
 

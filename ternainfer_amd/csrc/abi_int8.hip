@@ -20,29 +20,42 @@ void launch_quantise(const E* x, long long row, void* packed, float* scale, int 
 {
     const int wide = aligned16(x) && (row * static_cast<long long>(sizeof(E)) & 15) == 0;
     uint8_t* const to = static_cast<uint8_t*>(packed);
-    if (R < 2048) launch(terna_int8_quantise_kernel<E, 1>, dim3(R), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
-    else launch(terna_int8_quantise_kernel<E, 16>, dim3((R + 15) / 16), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
+    const int held = (4 * int8_k_blocks(K) + 63) / 64;
+    auto kernel = held <= 1 ? terna_int8_quantise_kernel<E, 1> : held <= 3 ? terna_int8_quantise_kernel<E, 3> : terna_int8_quantise_kernel<E, 7>;
+    launch(kernel, dim3((R + 3) / 4), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
 }
 
-template <typename Out, int WN, int WM, int NA, int MB, int SK, int ST>
-bool launch_int8(Int8Linear a, hipStream_t st)
+template <typename Out, int KIND, int WN, int WM, int NA, int MB, int SK, int ST>
+void launch_int8(const Int8Linear& a, long long tiles, hipStream_t st)
 {
     using Tile = Int8Tile<WN, WM, NA, MB, SK, ST>;
-    a.tiles_m = (a.M + Tile::BM - 1) / Tile::BM, a.tiles_n = (a.N + Tile::BN - 1) / Tile::BN;
-    const long long grid = static_cast<long long>(a.tiles_m) * a.tiles_n;
-    if (!launch_fits(grid, 256)) return false;
+    static_assert(Tile::BN == kInt8Tiles[KIND].features && Tile::BM == kInt8Tiles[KIND].rows);
+    constexpr int lds = Tile::template bytes<Out>(), join_lds = 32 * WM * Tile::template pitch<Out>();
     auto kernel = terna_int8_linear_kernel<Out, WN, WM, NA, MB, SK, ST>;
-    if (Tile::kBytes > kPlainLds) allow_dynamic_lds(kernel, Tile::kBytes, "hipFuncSetAttribute(int8 linear)", __LINE__);
-    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), Tile::kBytes, st, a);
-    return true;
+    if (lds > kPlainLds) allow_dynamic_lds(kernel, lds, "hipFuncSetAttribute(int8 linear)", __LINE__);
+    launch(kernel, dim3(static_cast<unsigned>((tiles * a.splits + 7) / 8 * 8)), dim3(256), lds, st, a);
+    if constexpr (KIND == kInt8SplitTile) {
+        static_assert(join_lds <= kPlainLds);
+        if (a.splits > 1)
+            launch(terna_int8_join_kernel<Out, WN, WM, NA, MB, SK, ST>, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(256), join_lds, st, a);
+    }
 }
 template <typename Out>
-bool launch_int8_linear(const Int8Linear& a, hipStream_t st)
+void launch_int8_linear(const Int8Linear& a, const Int8Plan& plan, hipStream_t st)
 {
-    if (a.M <= 32) return launch_int8<Out, 4, 1, 1, 1, 2, 4>(a, st);
-    if (a.M <= 64) return launch_int8<Out, 4, 1, 1, 2, 1, 6>(a, st);
-    if (a.M <= 512) return launch_int8<Out, 2, 2, 2, 2, 1, 5>(a, st);
-    return launch_int8<Out, 2, 2, 4, 4, 1, 4>(a, st);
+    switch (plan.tile) {                       // (the order of kInt8Tiles)
+    case 0: return launch_int8<Out, 0, 4, 1, 1, 1, 2, 4>(a, plan.tiles, st);
+    case 1: return launch_int8<Out, 1, 2, 2, 1, 1, 2, 5>(a, plan.tiles, st);
+    case 2: return launch_int8<Out, 2, 4, 1, 1, 2, 1, 6>(a, plan.tiles, st);
+    case 3: return launch_int8<Out, 3, 4, 1, 2, 2, 1, 4>(a, plan.tiles, st);
+    case 4: return launch_int8<Out, 4, 2, 2, 2, 2, 1, 5>(a, plan.tiles, st);
+    case 5: return launch_int8<Out, 5, 2, 2, 2, 3, 1, 4>(a, plan.tiles, st);
+    default: return launch_int8<Out, 6, 2, 2, 2, 4, 1, 3>(a, plan.tiles, st);
+    }
+}
+bool int8_linear_ok(int M, int N, int K)
+{
+    return int8_rows_ok(M, K) && int8_rows_ok(N, K) && launch_fits(int8_plan(M, N, K, true).tiles * kInt8MaxSplits + 8, 256);
 }
 
 }  // namespace
@@ -53,7 +66,7 @@ long long ternaspmm_int8_bytes(int R, int K) { return int8_rows_ok(R, K) ? int8_
 
 int ternaspmm_int8_quantise(const void* x, long long row, int fp32, void* packed, float* scale, int R, int K, terna_stream stream)
 {
-    if (!int8_rows_ok(R, K) || !x || !packed || !scale || !aligned16(packed) || (reinterpret_cast<uintptr_t>(x) & (fp32 ? 3 : 1)) || row < 0 || !launch_fits(R, kInt8Threads / 16))
+    if (!int8_rows_ok(R, K) || !x || !packed || !scale || !aligned16(packed) || (reinterpret_cast<uintptr_t>(x) & (fp32 ? 3 : 1)) || row < 0 || !launch_fits((R + 3) / 4, kInt8Threads))
         return -1;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (fp32) launch_quantise(static_cast<const float*>(x), row, packed, scale, R, K, st);
@@ -65,20 +78,31 @@ int ternaspmm_int8_quantise(const void* x, long long row, int fp32, void* packed
 
 int ternaspmm_int8_pack(const void* x, long long row, void* packed, int R, int K, terna_stream stream)
 {
-    if (!int8_rows_ok(R, K) || !x || !packed || !aligned16(packed) || row < 0 || !launch_fits((R + 15) / 16, kInt8Threads)) return -1;
-    launch(terna_int8_pack_kernel, dim3((R + 15) / 16), dim3(kInt8Threads), 0, static_cast<hipStream_t>(stream), static_cast<const uint8_t*>(x), row,
+    const long long waves = int8_bands(R) * ((int8_k_blocks(K) + kInt8PackBlocks - 1) / kInt8PackBlocks), groups = (waves + kInt8Threads / 64 - 1) / (kInt8Threads / 64);
+    if (!int8_rows_ok(R, K) || !x || !packed || !aligned16(packed) || row < 0 || !launch_fits(groups, kInt8Threads)) return -1;
+    launch(terna_int8_pack_kernel, dim3(static_cast<unsigned>(groups)), dim3(kInt8Threads), 0, static_cast<hipStream_t>(stream), static_cast<const uint8_t*>(x), row,
            static_cast<uint8_t*>(packed), R, K, aligned16(x) && (row & 15) == 0);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_int8_pack", e, __LINE__);
     return 0;
 }
 
-int ternaspmm_int8_linear(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out, int fp32, int M, int N, int K, terna_stream stream)
+long long ternaspmm_int8_linear_workspace_bytes(int M, int N, int K)
 {
-    if (!int8_rows_ok(M, K) || !int8_rows_ok(N, K) || !x || !x_scale || !w || !w_scale || !out || !aligned16(x) || !aligned16(w) || !aligned16(out)) return -1;
-    Int8Linear a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(w), x_scale, w_scale, out, M, N, K, 0, 0};
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!(fp32 ? launch_int8_linear<float>(a, st) : launch_int8_linear<uint16_t>(a, st))) return -1;
+    if (!int8_linear_ok(M, N, K)) return -1;
+    const Int8Plan plan = int8_plan(M, N, K, true);
+    return plan.splits == 1 ? 0 : 4ll * plan.tiles * plan.splits * kInt8Tiles[plan.tile].features * kInt8Tiles[plan.tile].rows;
+}
+
+int ternaspmm_int8_linear(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out, int fp32, void* workspace, int M, int N, int K, terna_stream stream)
+{
+    if (!int8_linear_ok(M, N, K) || !x || !x_scale || !w || !w_scale || !out || !aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(workspace)) return -1;
+    const Int8Plan plan = int8_plan(M, N, K, workspace != nullptr);
+    const Int8TileTime& tile = kInt8Tiles[plan.tile];
+    Int8Linear a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(w), x_scale, w_scale, out, static_cast<int32_t*>(workspace), M, N, K,
+                 (M + tile.rows - 1) / tile.rows, (N + tile.features - 1) / tile.features, plan.splits};
+    if (fp32) launch_int8_linear<float>(a, plan, static_cast<hipStream_t>(stream));
+    else launch_int8_linear<uint16_t>(a, plan, static_cast<hipStream_t>(stream));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_int8_linear", e, __LINE__);
     return 0;

@@ -82,6 +82,7 @@ namespace {
     X(ternaspmm_int8_bytes)                                                                                            \
     X(ternaspmm_int8_quantise)                                                                                         \
     X(ternaspmm_int8_pack)                                                                                             \
+    X(ternaspmm_int8_linear_workspace_bytes)                                                                           \
     X(ternaspmm_int8_linear)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -1462,7 +1463,9 @@ TERNA_FUNCTION(int8_linear, 8)
         scale = scales;
         rc = lib.ternaspmm_int8_quantise(rows.const_data_ptr(), rows.stride(0), x.scalar_type() == at::kFloat, held.get(), scales, m, k, stream());
     }
-    if (rc == 0) rc = lib.ternaspmm_int8_linear(packed, scale, w.packed.const_data_ptr(), w.scale.const_data_ptr<float>(), out.mutable_data_ptr(), fp32, m, n, k, stream());
+    const long long sums = lib.ternaspmm_int8_linear_workspace_bytes(m, n, k);
+    const c10::DataPtr work = sums > 0 ? device_allocator()->allocate(sums) : c10::DataPtr();
+    if (rc == 0) rc = lib.ternaspmm_int8_linear(packed, scale, w.packed.const_data_ptr(), w.scale.const_data_ptr<float>(), out.mutable_data_ptr(), fp32, work.get(), m, n, k, stream());
     unlocked.end();
     if (rc != 0) refuse("%s: the library refused the launch", who);
     return THPVariable_Wrap(std::move(out));
