@@ -22,7 +22,7 @@ bool tree_shape_ok(int B, int T, int H, int KV, int D, int S)
 {
     if (!tree_nodes_ok(B, T) || H < 1 || KV < 1 || H % KV != 0 || (D != 64 && D != 128) || S < 1 || S > 1 << 25 || H > 4096 || static_cast<long long>(B) * T * H > 1 << 28) return false;
     const TreePlan plan = tree_plan(B, T, H, KV, D, S);
-    return launch_fits(((static_cast<long long>(B) * KV * plan.splits + 7) / 8) * 8 * plan.tiles, 256);
+    return launch_fits(((static_cast<long long>(B) * KV * plan.splits + 7) / 8) * 8 * plan.tiles, 512);
 }
 // Strides in elements of rows that are read 16 bytes at a time.
 bool strides_ok(const long long* s, int n)
@@ -32,32 +32,32 @@ bool strides_ok(const long long* s, int n)
     return true;
 }
 
-template <int D, int RW, int ST>
+template <int D, int RW, int ST, bool TWO, int PER_SIMD>
 void launch_tree(const TreeAttention& a, long long grid, hipStream_t st)
 {
-    constexpr int lds = TreeShape<D, RW, ST>::kBytes;
-    auto kernel = terna_tree_attention_kernel<D, RW, ST>;
-    if (lds > kPlainLds - 4096) allow_dynamic_lds(kernel, lds, "hipFuncSetAttribute(tree attention)", __LINE__);
-    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), lds, st, a);
+    using Shape = TreeShape<D, RW, ST>;
+    auto kernel = terna_tree_attention_kernel<D, RW, ST, TWO, PER_SIMD>;
+    if (Shape::kBytes > kPlainLds - 4096) allow_dynamic_lds(kernel, Shape::kBytes, "hipFuncSetAttribute(tree attention)", __LINE__);
+    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), Shape::kBytes, st, a);
 }
 template <int D>
-void launch_tree_attention(const TreeAttention& a, int row_waves, long long grid, hipStream_t st)
+void launch_tree_attention(const TreeAttention& a, int rows, long long grid, hipStream_t st)
 {
-    if (row_waves == 1) launch_tree<D, 1, D == 128 ? 2 : 4>(a, grid, st);
-    else if (row_waves == 2) launch_tree<D, 2, D == 128 ? 2 : 4>(a, grid, st);
-    else launch_tree<D, 4, D == 128 ? 4 : 8>(a, grid, st);
-    if (a.splits > 1) {
-        const int rows = a.B * a.T * a.H;
-        launch(terna_tree_merge_kernel<D>, dim3((rows + 3) / 4), dim3(256), 0, st, a.partial, a.out, rows, a.splits);
+    if (rows == 32) launch_tree<D, 1, D == 128 ? 2 : 4, true, 1>(a, grid, st);
+    else if (rows == 64) launch_tree<D, 2, D == 128 ? 2 : 4, true, 2>(a, grid, st);
+    else launch_tree<D, 4, 4, false, 2>(a, grid, st);
+    if (a.parts != 0) {
+        const int all = a.T * a.H;
+        launch(terna_tree_merge_kernel<D>, dim3((a.B * all + 3) / 4), dim3(256), 0, st, a.partial, a.out, a.B, all, a.parts);
     }
 }
 
-// Parts of a row of logits: enough workgroups for every CU to have two, of two rounds of loads at least.
+// Parts of a row of logits: up to eight workgroups a CU, of a round of loads at least (512 rows of 128256: two a CU 30 us, eight 26).
 int accept_parts(int rows, int V, int fp32)
 {
     const int pieces = V / (fp32 ? 4 : 8), round = kTreeThreads * kAcceptBatch;
     int parts = 1;
-    while (parts < 64 && static_cast<long long>(rows) * parts < 512 && pieces > parts * round) parts *= 2;
+    while (parts < 64 && 2ll * rows * parts <= 2048 && pieces > parts * round) parts *= 2;
     return parts;
 }
 bool accept_shape_ok(int B, int T, int V, int fp32) { return tree_nodes_ok(B, T) && V >= 1 && V <= 1 << 19 && launch_fits(static_cast<long long>(B) * T * accept_parts(B * T, V, fp32), kTreeThreads); }
@@ -82,7 +82,7 @@ long long ternaspmm_tree_attention_workspace_bytes(int B, int T, int H, int KV, 
 {
     if (!tree_shape_ok(B, T, H, KV, D, S)) return -1;
     const int splits = tree_plan(B, T, H, KV, D, S).splits;
-    return splits == 1 ? 0 : 4ll * B * T * H * splits * (D + 2);
+    return splits == 1 ? 0 : 4ll * B * T * H * splits * (D + 2) + static_cast<long long>(sizeof(TreeShare)) * B;
 }
 
 int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, const terna_bf16* k, const long long* k_strides, const terna_bf16* v, const long long* v_strides,
@@ -100,11 +100,11 @@ int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, co
     a.k_seq = k_strides[0], a.k_head = k_strides[1], a.k_slot = static_cast<int>(2 * k_strides[2]);
     a.v_seq = v_strides[0], a.v_head = v_strides[1], a.v_slot = static_cast<int>(2 * v_strides[2]);
     a.B = B, a.T = T, a.H = H, a.KV = KV, a.S = S, a.W = (T + 63) / 64, a.per_seq = per_sequence != 0;
-    a.splits = workspace ? plan.splits : 1, a.tiles = plan.tiles;
+    a.parts = workspace && plan.splits > 1 ? B * plan.splits : 0, a.tiles = plan.tiles;
     a.scale = scale * static_cast<float>(M_LOG2E);
-    const long long grid = ((static_cast<long long>(B) * KV * a.splits + 7) / 8) * 8 * plan.tiles;
-    if (D == 128) launch_tree_attention<128>(a, plan.row_waves, grid, static_cast<hipStream_t>(stream));
-    else launch_tree_attention<64>(a, plan.row_waves, grid, static_cast<hipStream_t>(stream));
+    const long long grid = ((static_cast<long long>(a.parts == 0 ? B : a.parts) * KV + 7) / 8) * 8 * plan.tiles;
+    if (D == 128) launch_tree_attention<128>(a, plan.rows, grid, static_cast<hipStream_t>(stream));
+    else launch_tree_attention<64>(a, plan.rows, grid, static_cast<hipStream_t>(stream));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_tree_attention", e, __LINE__);
     return 0;

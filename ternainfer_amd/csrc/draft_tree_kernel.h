@@ -150,9 +150,12 @@ __global__ __launch_bounds__(kTreeThreads) void terna_accept_path_kernel(const A
     for (int i = tid; i < T; i += kTreeThreads) {
         float best = -INFINITY;
         int idx = 0x7fffffff;
-        for (int c = 0; c < parts; ++c) {
-            const AcceptBest b = best_of[(first + i) * parts + c];
-            accept_merge(best, idx, b.value, b.index);
+        for (int c = 0; c < parts; c += kAcceptBatch) {
+            AcceptBest b[kAcceptBatch];
+#pragma unroll
+            for (int u = 0; u < kAcceptBatch; ++u) b[u] = best_of[(first + i) * parts + min(c + u, parts - 1)];
+#pragma unroll
+            for (int u = 0; u < kAcceptBatch; ++u) accept_merge(best, idx, b[u].value, b[u].index);
         }
         says[i] = idx == 0x7fffffff ? 0 : idx;
         child[i] = kTreeMaxNodes;
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(kTreeThreads) void terna_accept_path_kernel(const A
 // written before it has been read; a thread has a column of its own (a piece of a head's rows) and reads eight rows at a time.  A row outside the cache
 // stays where it is.
 
-constexpr int kMoveCaches = 48;                // of a launch: their descriptions are kernel arguments
+constexpr int kMoveCaches = 64;                // of a launch: their descriptions are kernel arguments
 constexpr int kMoveAhead = 8;
 
 struct MoveCache {

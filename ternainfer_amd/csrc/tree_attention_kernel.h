@@ -30,20 +30,33 @@ struct TreeAttention {
     const uint16_t *q, *k, *v;
     const long long *start, *mask;
     uint16_t* out;                             // [B * T][H * D], or
-    float* partial;                            // more than one split: fp32 [rows][splits][D] numerators, then [rows][splits][2] maximum, sum
+    float* partial;                            // more than one part a sequence: fp32 [parts][T * H][D] numerators, [parts][T * H][2] maximum and sum, then TreeShare [B]
     long long q_seq, q_head, q_node;           // strides, elements
     long long k_seq, k_head, v_seq, v_head;
     int k_slot, v_slot;                        // ... of a slot, bytes
-    int B, T, H, KV, S, W, splits, tiles, per_seq;
+    int B, T, H, KV, S, W, parts, tiles, per_seq;       // parts: of all sequences together, 0 where none is split
     float scale;                               // times log2(e)
 };
 
+// Two bf16 added to a sum
+__device__ __forceinline__ float tree_sum2(uint32_t both, float sum)
+{
+    typedef __bf16 two __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, both), __builtin_bit_cast(two, 0x3f803f80u), sum, false);
+}
+
+// A sequence's parts: the first of them, and how many.
+struct TreeShare {
+    int first, count;
+};
+
+// A workgroup's shape: four waves, RW of them share the slots, 32 query rows each; ST tiles of keys and values in each group's ring.
 template <int D, int RW, int ST>
 struct TreeShape {
-    static constexpr int KW = 4 / RW;
+    static constexpr int KW = 4 / RW;                                      // groups
     static constexpr int kTile = kTreeTile * D * 2;                        // bytes of a tile's keys, or values
     static constexpr int kRing = KW * ST * 2 * kTile;
-    static constexpr int kRow = D + 4;                                     // floats of a row of numerators in LDS
+    static constexpr int kRow = D / 2 + 4;                                 // floats of a row of numerators in LDS, half of its dimensions at a time
     static constexpr int kJoin = 4 * 32 * kRow * 4;
     static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
@@ -66,37 +79,103 @@ __device__ __forceinline__ float tree_halves(float v)
     return IS_MAX ? max_keep_nan(a, b) : a + b;
 }
 
-template <int D, int RW, int ST>
-__global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_kernel(TreeAttention a)
+// Which part of which sequence a workgroup takes.  The parts that the launch has room for are dealt out by the sequences' lengths, all at most `longest` tiles long, the
+// shortest such length within an eighth: with as many for each, the longest sequence's would last longest (8 sequences of 1670 to 4001 slots: 33 us, so 30).
+// Every wave works it out, a sequence a lane.
+struct TreePart {
+    int b, start, split;                       // b < 0: none; start: -1 for a sequence without a tree, S + 1 for one behind the cache
+    TreeShare share;
+};
+__device__ __forceinline__ uint32_t tree_wave_sum(uint32_t x)
 {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ TreePart tree_part(const TreeAttention& a, int part)
+{
+    const int lane = threadIdx.x & 63;
+    auto start_of = [&](int b) { return static_cast<int>(min(max(a.start[b], -1ll), a.S + 1ll)); };
+    auto tiles_of = [&](int start) { return start < 0 ? 0u : static_cast<uint32_t>(min(start + a.T, a.S) + kTreeTile - 1) / kTreeTile; };
+    TreePart p;
+    if (a.parts == 0) {
+        p.b = part, p.start = start_of(part), p.split = 0, p.share = TreeShare{part, 1};
+        return p;
+    }
+    if (a.B == 1) {
+        p.b = part < kTreeMaxSplits ? 0 : -1, p.start = start_of(0), p.split = part, p.share = TreeShare{0, min(a.parts, kTreeMaxSplits)};
+        return p;
+    }
+    int start = lane < a.B ? start_of(lane) : -1;
+    auto start_at = [&](int b0) { return b0 == 0 && a.B <= 64 ? start : b0 + lane < a.B ? start_of(b0 + lane) : -1; };
+    auto count_of = [&](int b, int start, uint32_t longest) {              // (a sequence has one at least)
+        return b < a.B ? min(max((tiles_of(start) + longest - 1) / longest, 1u), static_cast<uint32_t>(kTreeMaxSplits)) : 0u;
+    };
+    uint32_t all = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) all += tree_wave_sum(tiles_of(start_at(b0)));
+    const uint32_t parts = static_cast<uint32_t>(a.parts);
+    // (at all / (parts - B), rounded up, they certainly fit)
+    for (uint32_t longest = max((all + parts - 1) / parts, 1u);; longest += max(longest / 8, 1u)) {
+        uint32_t total = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) total += tree_wave_sum(count_of(b0 + lane, start_at(b0), longest));
+        if (total > parts) continue;
+        int before = 0;
+        p.b = -1;
+        for (int b0 = 0; b0 < a.B && p.b < 0; b0 += 64) {
+            const int at = start_at(b0), count = count_of(b0 + lane, at, longest);
+            int upto = count;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int x = __shfl_up(upto, off);
+                if (lane >= off) upto += x;
+            }
+            const int first = before + upto - count;
+            const unsigned long long found = __ballot(part >= first && part < first + count);
+            if (found != 0) {
+                const int who = __builtin_ctzll(found);
+                p.b = b0 + who, p.start = __builtin_amdgcn_readlane(at, who);
+                p.share = TreeShare{__builtin_amdgcn_readlane(first, who), __builtin_amdgcn_readlane(count, who)};
+                p.split = part - p.share.first;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+        return p;
+    }
+}
+
+template <int D, int RW, int ST, bool TWO, int PER_SIMD>
+__global__ __launch_bounds__(256, PER_SIMD) void terna_tree_attention_kernel(TreeAttention a)
+{
+    static_assert(ST == 2 || ST == 4);
     using Shape = TreeShape<D, RW, ST>;
     constexpr int KW = Shape::KW, KS = D / 16, DT = D / 32, TILE = Shape::kTile;
-    constexpr int PIECES = D / 8, PER_LOAD = 64 / PIECES, LOADS = kTreeTile / RW / PER_LOAD;      // rows of a 1 KB load; loads of a wave and tile
+    constexpr int PIECES = D / 8, PER_LOAD = 64 / PIECES, PER_TILE = TILE / 1024, LOADS = 2 * PER_TILE / RW;       // rows of a 1 KB load; loads of a tile's keys; of a wave and step
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float2 stat[4][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wave / RW, rw = wave % RW, qi = lane & 31, half = lane >> 5;
-    // Workgroups go to the XCDs round robin: the row tiles of one (sequence, kv head, split) -- which read the same slots -- eight apart, on one XCD.
-    const int G = a.H / a.KV, units = a.B * a.KV * a.splits;
+    // Workgroups go to the XCDs round robin: the row tiles of one part of a kv head -- which read the same slots -- eight apart, on one XCD.
+    const int G = a.H / a.KV, units = (a.parts == 0 ? a.B : a.parts) * a.KV;
     const int block = blockIdx.x / (8 * a.tiles), within = blockIdx.x - block * (8 * a.tiles);
     const int unit = 8 * block + (within & 7), tile = within >> 3;
     if (unit >= units) return;
-    const int split = unit % a.splits, bk = unit / a.splits, kvh = bk % a.KV, b = bk / a.KV;
+    const int kvh = unit % a.KV;
+    const TreePart part = tree_part(a, unit / a.KV);
+    if (part.b < 0) return;
+    const int b = part.b, splits = part.share.count;
 
     // ---- rows
-    const int rows = a.T * G, r = (tile * RW + rw) * 32 + qi;
-    const bool real = r < rows;
-    const int node = real ? r / G : 0, h = kvh * G + (real ? r - node * G : 0);
-    const long long st64 = a.start[b];
+    const int rows = a.T * G, start = min(max(part.start, 0), a.S), inside = min(a.T, a.S - start);        // inside: nodes that have a slot
+    const int r = (tile * RW + rw) * 32 + qi, node = r < rows ? r / G : 0, h = kvh * G + (r < rows ? r - node * G : 0);
     const unsigned long long* const mask = reinterpret_cast<const unsigned long long*>(a.mask) + (static_cast<size_t>(a.per_seq ? b : 0) * a.T + node) * a.W;
-    const uint16_t* const qrow = a.q + b * a.q_seq + h * a.q_head + node * a.q_node;
-    u32x4 q[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(qrow + 16 * ks + 8 * half);
-    const int start = static_cast<int>(min(max(st64, 0ll), static_cast<long long>(a.S)));
-    const int inside = min(a.T, a.S - start);                              // nodes that have a slot
     const unsigned long long first_word = mask[0];
-    bool active = false, outside = false;                                  // the row has a node; sees a slot behind the cache
+    u32x4 q[KS];
+    {
+        const uint16_t* const row = a.q + b * a.q_seq + h * a.q_head + node * a.q_node;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(row + 16 * ks + 8 * half);
+    }
+    bool active = false, outside = part.start > a.S;                       // the row has a node; sees a slot behind the cache
     for (int w = 0; w < a.W; ++w) {
         const unsigned long long bits = w == 0 ? first_word : mask[w];
         const int has = min(max(inside - 64 * w, 0), 64), in_tree = min(a.T - 64 * w, 64);
@@ -104,53 +183,58 @@ __global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_ker
         active |= (bits & valid) != 0;
         outside |= (bits & valid & ~fit) != 0;
     }
-    active = active && real && st64 >= 0;
-    outside = active && (outside || st64 > a.S);
-    const int n = __syncthreads_or(active) ? start + inside : 0;           // slots that the workgroup reads
-    const int all_tiles = (n + kTreeTile - 1) / kTreeTile, share = (all_tiles + a.splits - 1) / a.splits;
-    const int begin = split * share, end = min(begin + share, all_tiles);
+    active = active && r < rows && part.start >= 0;
+    outside = outside && active;
+    const int n = __syncthreads_or(active) ? start + inside : 0;       // slots that the workgroup reads
+    const int all_tiles = (n + kTreeTile - 1) / kTreeTile, share = (all_tiles + splits - 1) / splits;
+    const int begin = part.split * share, end = min(begin + share, all_tiles);
     const int steps = end > begin ? (end - begin + KW - 1) / KW : 0;       // of every group: a tile behind the end has no slot that counts
 
     // a negative scale's sign, and a scale of zero (0 * -inf would unmask a slot), go into the queries
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-        if (a.scale == 0.0f) {
-            float x[8];
-            unpack_bf16x8(q[ks], x);
+            if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+            if (a.scale == 0.0f) {
+                float x[8];
+                unpack_bf16x8(q[ks], x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
-            q[ks] = pack_bf16x8(x);
+                for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
+                q[ks] = pack_bf16x8(x);
+            }
+            pin_registers(q[ks]);                                      // landed before the first hand-issued request
         }
-        pin_registers(q[ks]);                                              // landed before the first hand-issued request
-    }
 
     // ---- the cache's tiles
     const uint8_t* const kb = reinterpret_cast<const uint8_t*>(a.k + b * a.k_seq + kvh * a.k_head);
     const uint8_t* const vb = reinterpret_cast<const uint8_t*>(a.v + b * a.v_seq + kvh * a.v_head);
     uint8_t* const ring = smem + group * (ST * 2 * TILE);
-    const uint32_t ring0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + rw * (LOADS * 1024);
-    const int load_row = rw * (kTreeTile / RW) + lane / PIECES, piece = lane & (PIECES - 1);
-    uint32_t k_at[LOADS], v_at[LOADS];
+    const uint32_t ring0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + rw * 1024;
+    // Of a step's loads a wave has those rw, rw + RW, ...: first the keys', then the values'.
+    int load_row[LOADS];
+    uint32_t load_piece[LOADS], load_at[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        k_at[i] = tree_key_piece<D>(load_row + i * PER_LOAD, piece) << 4;
-        v_at[i] = tree_value_piece<D>(load_row + i * PER_LOAD, piece) << 4;
+        const int l = rw + RW * i;
+        load_row[i] = (l % PER_TILE) * PER_LOAD + lane / PIECES;
+        load_piece[i] = (l < PER_TILE ? tree_key_piece<D>(load_row[i], lane & (PIECES - 1)) : tree_value_piece<D>(load_row[i], lane & (PIECES - 1))) << 4;
+        load_at[i] = static_cast<uint32_t>(load_row[i] * (l < PER_TILE ? a.k_slot : a.v_slot)) + load_piece[i];
     }
     auto slot_of = [&](int step) __attribute__((always_inline)) { return (begin + KW * step + group) * kTreeTile; };
-    auto load = [&](int step, int at) __attribute__((always_inline)) {     // slots behind the last are read from its row
+    // a step's keys and values into their place of the ring; slots behind the last are read from its row
+    auto load = [&](int step, int at) __attribute__((always_inline)) {
         const int k0 = min(slot_of(step), n - 1), left = n - 1 - k0;
         const uint8_t *const kt = kb + static_cast<long long>(k0) * a.k_slot, *const vt = vb + static_cast<long long>(k0) * a.v_slot;
+        const uint32_t to = ring0 + at * (2 * TILE);
+        if (left >= kTreeTile - 1) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const uint32_t row = min(load_row + i * PER_LOAD, left);
-            lds_dma_b128(kt, row * a.k_slot + k_at[i], ring0 + at * (2 * TILE) + i * 1024);
-        }
+            for (int i = 0; i < LOADS; ++i) lds_dma_b128(rw + RW * i < PER_TILE ? kt : vt, load_at[i], to + i * (RW * 1024));
+        } else {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const uint32_t row = min(load_row + i * PER_LOAD, left);
-            lds_dma_b128(vt, row * a.v_slot + v_at[i], ring0 + at * (2 * TILE) + TILE + i * 1024);
+            for (int i = 0; i < LOADS; ++i) {
+                const bool keys = rw + RW * i < PER_TILE;
+                lds_dma_b128(keys ? kt : vt, static_cast<uint32_t>(min(load_row[i], left) * (keys ? a.k_slot : a.v_slot)) + load_piece[i], to + i * (RW * 1024));
+            }
         }
     };
     int va[DT];
@@ -166,7 +250,7 @@ __global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_ker
         const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(vals + va[dt] + (i * 16 + 8) * 2 * D)));
         return u32x4{a0.x, a0.y, a1.x, a1.y};
     };
-    // bits of this row's mask for the 32 slots from k0 on: those in front of the tree are seen
+    // bits of a row's mask for the 32 slots from k0 on: those in front of the tree are seen
     auto seen_bits = [&](int k0) __attribute__((always_inline)) {
         const int first = k0 - start;                                      // node of the tile's first slot
         uint32_t bits = 0;
@@ -189,45 +273,69 @@ __global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_ker
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[dt][v] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
     bool taken_out = false;                                                // a value that is not finite, among the tree's
 
-    if (steps > 0) {
+    // Infinities and NaN -- exponents of ones -- out of pieces of values, remembered.  There are hardly ever any: one look at all of them.
+    auto finite = [&](u32x4* x, int pieces) __attribute__((always_inline)) {
+        typedef unsigned short two __attribute__((ext_vector_type(2)));
+        two most{0, 0};
 #pragma unroll
-        for (int i = 0; i < ST - 1; ++i) load(i, i);
-    }
-    int at = 0;
-    for (int step = 0; step < steps; ++step) {
+        for (int i = 0; i < pieces; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(two, x[i][e] & 0x7fff7fffu));
+        const bool broken = most.x >= 0x7f80u || most.y >= 0x7f80u;
+        if (!__any(broken)) return;
+        taken_out |= broken;
+#pragma unroll
+        for (int i = 0; i < pieces; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[i][e] &= ((x[i][e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x[i][e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+    };
+    auto unseen = [&](f32x16& s, int k0) __attribute__((always_inline)) {
+        const uint32_t bits = k0 >= end * kTreeTile ? 0u : seen_bits(k0);
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+            if (!(bits >> (8 * (v >> 2) + 4 * half + (v & 3)) & 1u)) s[v] = -INFINITY;
+    };
+    auto largest = [&](const f32x16& s) __attribute__((always_inline)) {
+        float tops[2] = {tree_max3(s[0], s[1], s[2]), tree_max3(s[3], s[4], s[5])};
+#pragma unroll
+        for (int v = 6; v < 14; v += 4) {
+            tops[0] = tree_max3(tops[0], s[v], s[v + 1]);
+            tops[1] = tree_max3(tops[1], s[v + 2], s[v + 3]);
+        }
+        return tree_max3(tree_max3(tops[0], tops[1], s[14]), s[15], s[15]);
+    };
+    float l_run = 0.0f, m_run = -INFINITY;
+    // steps whose tiles lie in front of the tree, all of them
+    const int plain = max(min(start / kTreeTile, end) - begin, 0) / KW;
+    int at = 0;                                                            // place in the ring
+    auto take = [&](int step, auto last_tiles, auto place) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_tiles)::value;                 // may have slots of the tree, or behind the end
+        constexpr int PLACE = decltype(place)::value;                      // known: offsets that instructions carry; -1: `at`
+        const int here = PLACE < 0 ? at : PLACE, behind = PLACE < 0 ? (at == 0 ? ST - 1 : at - 1) : (PLACE + ST - 1) % ST;
         if constexpr (RW == 1) {
             // (this wave's reads of the tile that is overwritten have returned: the products took them)
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load(step + ST - 1, at == 0 ? ST - 1 : at - 1);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * 2 * LOADS) : "memory");
+            load(step + ST - 1, behind);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * LOADS) : "memory");
         } else {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * 2 * LOADS) : "memory");
-            load(step + ST - 1, at == 0 ? ST - 1 : at - 1);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * LOADS) : "memory");
+            load(step + ST - 1, behind);
         }
-        const uint8_t *const keys = ring + at * (2 * TILE), *const vals = keys + TILE;
-        at = at + 1 == ST ? 0 : at + 1;
-        const int k0 = slot_of(step);
+        const uint8_t *const keys = ring + here * (2 * TILE), *const vals = keys + TILE;
+        if constexpr (PLACE < 0) at = at + 1 == ST ? 0 : at + 1;
         f32x16 s;
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_operand(keys, ks), __builtin_bit_cast(bf16x8, q[ks]), s, 0, 0, 0);
-        const bool last_tiles = k0 + kTreeTile > start || k0 >= end * kTreeTile;
-        if (last_tiles) {
-            const uint32_t bits = k0 >= end * kTreeTile ? 0u : seen_bits(k0);
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (!(bits >> (8 * (v >> 2) + 4 * half + (v & 3)) & 1u)) s[v] = -INFINITY;
-        }
-        float top = tree_max3(tree_max3(s[0], s[1], s[2]), s[3], s[4]);
-#pragma unroll
-        for (int v = 5; v < 15; v += 2) top = tree_max3(top, s[v], s[v + 1]);
-        top = tree_halves<true>(max_keep_nan(top, s[15])) * scale;
-        if (__any(top > m_run + kTreeGrowth)) {
-            const float m_new = top > m_run + kTreeGrowth ? top : m_run;   // a row by its own growth alone: its bits do not hang on the rows beside it
+        if constexpr (LAST) unseen(s, slot_of(step));
+        const float top = tree_halves<true>(largest(s)) * scale;
+        const bool more = top > m_run + kTreeGrowth;                // a row by its own growth alone: its bits do not hang on the rows beside it
+        if (__any(more)) {
+            const float m_new = more ? top : m_run;
             const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
             m_run = m_new;
             l_run *= alpha;
@@ -235,41 +343,60 @@ __global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_ker
             for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
         const float shift = m_run == -INFINITY ? 0.0f : -m_run;
-        u32x4 p_hi[2], p_lo[2];
+        float sum[2] = {0.0f, 0.0f};
+        u32x4 high[2], low[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float p[8], high[8];
+            float p[8], rounded[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[8 * i + e], scale, shift));
+            high[i] = pack_bf16x8(p);
+            unpack_bf16x8(high[i], rounded);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[8 * i + e], scale, shift));
-                l_run += p[e];
+                sum[e & 1] += TWO ? p[e] : 0.0f;
+                rounded[e] = p[e] - rounded[e];
             }
-            p_hi[i] = pack_bf16x8(p);
-            unpack_bf16x8(p_hi[i], high);
+            if constexpr (TWO) low[i] = pack_bf16x8(rounded);
+            else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) high[e] = p[e] - high[e];
-            p_lo[i] = pack_bf16x8(high);
+                for (int e = 0; e < 4; ++e) sum[e & 1] = tree_sum2(high[i][e], sum[e & 1]);
+            }
         }
+        l_run += sum[0] + sum[1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            u32x4 x[DT];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) x[dt] = value_operand(vals, i, dt);
+            if constexpr (LAST) finite(x, DT);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                u32x4 x = value_operand(vals, i, dt);
-                if (last_tiles) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {                          // exponents of ones: infinity or NaN
-                        const bool low = (x[e] & 0x7f80u) == 0x7f80u, upper = (x[e] & 0x7f800000u) == 0x7f800000u;
-                        taken_out |= low || upper;
-                        x[e] &= (low ? 0u : 0xffffu) | (upper ? 0u : 0xffff0000u);
-                    }
-                }
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, p_hi[i]), o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, p_lo[i]), o[dt], 0, 0, 0);
+                const bf16x8 y = __builtin_bit_cast(bf16x8, x[dt]);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, __builtin_bit_cast(bf16x8, high[i]), o[dt], 0, 0, 0);
+                if constexpr (TWO) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, __builtin_bit_cast(bf16x8, low[i]), o[dt], 0, 0, 0);
             }
+        }
+    };
+    if (steps > 0) {
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) load(i, i);
     }
+    using Anywhere = std::integral_constant<int, -1>;
+    int step = 0;
+    for (; step + ST <= plain; step += ST) {
+        take(step, std::false_type{}, std::integral_constant<int, 0>{});
+        take(step + 1, std::false_type{}, std::integral_constant<int, 1>{});
+        if constexpr (ST > 2) {
+            take(step + 2, std::false_type{}, std::integral_constant<int, 2>{});
+            take(step + 3, std::false_type{}, std::integral_constant<int, 3>{});
+        }
+    }
+    for (; step < plain; ++step) take(step, std::false_type{}, Anywhere{});
+    for (; step < steps; ++step) take(step, std::true_type{}, Anywhere{});
     l_run = tree_halves<false>(l_run);
     if (__any(taken_out)) {                                                // rare: they are added where they are seen
-        const int from = max(start / kTreeTile, begin);
+        const int from = max(min(start / kTreeTile, end) - KW, begin);     // (whatever tile it can have been; added twice, they are what they were)
         for (int k_tile = from; k_tile < end; ++k_tile) {
             if ((k_tile - begin) % KW != group) continue;
             const uint32_t bits = seen_bits(k_tile * kTreeTile);
@@ -287,76 +414,87 @@ __global__ __launch_bounds__(256, RW == 1 ? 1 : 2) void terna_tree_attention_ker
         }
     }
 
+    if (a.parts != 0 && part.split == 0 && kvh == 0 && tile == 0 && tid == 0)
+        reinterpret_cast<TreeShare*>(a.partial + static_cast<size_t>(a.parts) * a.T * a.H * (D + 2))[b] = part.share;
+
     // ---- the groups' numerators, over their largest maximum
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");                // (requests behind the end too)
     float* const join = reinterpret_cast<float*>(smem);
-    if (half == 0) stat[wave][qi] = float2{m_run, l_run};
     constexpr int ROW = Shape::kRow;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(join + (wave * 32 + qi) * ROW + 32 * dt + 8 * i + 4 * half) = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
-    // (flags of a row, from the lane that has them to the threads that write it)
+    __shared__ uint32_t flags[RW][2];                                      // of a row, from the lane that has them to the threads that write it
+    if (half == 0) stat[wave][qi] = float2{m_run, l_run};
     const unsigned long long rows_outside = __ballot(outside), rows_active = __ballot(active);
-    __shared__ uint32_t flags[RW][2];
     if (group == 0 && lane == 0) flags[rw][0] = static_cast<uint32_t>(rows_active), flags[rw][1] = static_cast<uint32_t>(rows_outside);
-    __syncthreads();
-    constexpr int STEP = 256 / PIECES;                                     // rows of the workgroup at a time, eight dimensions a thread
-    const int dim = (tid & (PIECES - 1)) * 8;
+    constexpr int EIGHTS = D / 16, STEP = 256 / EIGHTS;                    // of half a row; rows of the workgroup at a time, eight dimensions a thread
 #pragma unroll
-    for (int row0 = 0; row0 < 32 * RW; row0 += STEP) {
-        const int row = row0 + tid / PIECES, row_at = tile * 32 * RW + row, rwave = row >> 5, in_wave = row & 31;
-        if (row_at >= rows) continue;
-        const bool is_active = flags[rwave][0] >> in_wave & 1u, is_outside = flags[rwave][1] >> in_wave & 1u;
-        float m = -INFINITY, l = 0.0f, weight[KW], x[8];
+    for (int part_of = 0; part_of < 2; ++part_of) {
+        if (part_of != 0) __syncthreads();
 #pragma unroll
-        for (int g = 0; g < KW; ++g) m = fmaxf(m, stat[g * RW + rwave][in_wave].x);
-        const float m_use = m == -INFINITY ? 0.0f : m;
+        for (int dt = 0; dt < DT / 2; ++dt)
 #pragma unroll
-        for (int g = 0; g < KW; ++g) {
-            const float2 one = stat[g * RW + rwave][in_wave];
-            weight[g] = KW == 1 ? 1.0f : __builtin_amdgcn_exp2f(one.x - m_use);
-            l += one.y * weight[g];
-        }
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& x = o[part_of * (DT / 2) + dt];
+                *reinterpret_cast<f32x4*>(join + (wave * 32 + qi) * ROW + 32 * dt + 8 * i + 4 * half) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+            }
+        __syncthreads();
+        const int in_half = (tid & (EIGHTS - 1)) * 8, dim = part_of * (D / 2) + in_half;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        for (int row0 = 0; row0 < 32 * RW; row0 += STEP) {
+            const int row = row0 + tid / EIGHTS, row_at = tile * (32 * RW) + row, rwave = row >> 5, in_wave = row & 31;
+            if ((STEP > 32 * RW && row >= 32 * RW) || row_at >= rows) continue;
+            const bool is_active = flags[rwave][0] >> in_wave & 1u, is_outside = flags[rwave][1] >> in_wave & 1u;
+            float m = -INFINITY, l = 0.0f, weight[KW], x[8];
 #pragma unroll
-        for (int g = 0; g < KW; ++g) {
-            const float* const from = join + ((g * RW + rwave) * 32 + in_wave) * ROW + dim;
-            const f32x4 lower = *reinterpret_cast<const f32x4*>(from), upper = *reinterpret_cast<const f32x4*>(from + 4);
+            for (int g = 0; g < KW; ++g) m = fmaxf(m, stat[g * RW + rwave][in_wave].x);
+            const float m_use = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] += lower[e] * weight[g], x[4 + e] += upper[e] * weight[g];
-        }
-        const int of_node = row_at / G;
-        const size_t out_row = (static_cast<size_t>(b) * a.T + of_node) * a.H + kvh * G + row_at - of_node * G;
-        // nothing seen: zeros
-        const float factor = is_outside ? NAN : !is_active || l == 0.0f ? 0.0f : a.splits > 1 ? 1.0f : 1.0f / l;
+            for (int g = 0; g < KW; ++g) {
+                const float2 one = stat[g * RW + rwave][in_wave];
+                weight[g] = KW == 1 ? 1.0f : __builtin_amdgcn_exp2f(one.x - m_use);
+                l += one.y * weight[g];
+            }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = factor == 0.0f ? 0.0f : x[e] * factor;
-        if (a.splits > 1) {
-            float* const to = a.partial + (out_row * a.splits + split) * D + dim;
-            *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
-            *reinterpret_cast<f32x4*>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
-            if (dim == 0)
-                *reinterpret_cast<float2*>(a.partial + static_cast<size_t>(a.B) * a.T * a.H * a.splits * D + (out_row * a.splits + split) * 2) =
-                    is_outside ? float2{0.0f, 1.0f} : is_active ? float2{m, l} : float2{-INFINITY, 0.0f};
-        } else {
-            *reinterpret_cast<u32x4*>(a.out + out_row * D + dim) = pack_bf16x8(x);
+            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < KW; ++g) {
+                const float* const from = join + ((g * RW + rwave) * 32 + in_wave) * ROW + in_half;
+                const f32x4 lower = *reinterpret_cast<const f32x4*>(from), upper = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] += lower[e] * weight[g], x[4 + e] += upper[e] * weight[g];
+            }
+            const int of_node = row_at / G;
+            const size_t out_row = (static_cast<size_t>(b) * a.T + of_node) * a.H + kvh * G + row_at - of_node * G;
+            // nothing seen: zeros
+            const float factor = is_outside ? NAN : !is_active || l == 0.0f ? 0.0f : splits > 1 ? 1.0f : 1.0f / l;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = factor == 0.0f ? 0.0f : x[e] * factor;
+            if (splits > 1) {
+                const size_t all = static_cast<size_t>(a.T) * a.H, at = (part.share.first + part.split) * all + (out_row - b * all);
+                float* const to = a.partial + at * D + dim;
+                *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
+                *reinterpret_cast<f32x4*>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+                if (dim == 0)
+                    reinterpret_cast<float2*>(a.partial + a.parts * all * D)[at] = is_outside ? float2{0.0f, 1.0f} : is_active ? float2{m, l} : float2{-INFINITY, 0.0f};
+            } else {
+                *reinterpret_cast<u32x4*>(a.out + out_row * D + dim) = pack_bf16x8(x);
+            }
         }
     }
 }
 
-// The splits' numerators over their largest maximum: a wave a row, D / 64 dimensions a lane.
+// The parts' numerators of the sequences that have several, over their largest maximum: a wave a row, D / 64 dimensions a lane.
 template <int D>
-__global__ __launch_bounds__(256) void terna_tree_merge_kernel(const float* __restrict__ partial, uint16_t* __restrict__ out, int rows, int splits)
+__global__ __launch_bounds__(256) void terna_tree_merge_kernel(const float* __restrict__ partial, uint16_t* __restrict__ out, int B, int rows, int parts)
 {
     constexpr int E = D / 64, AHEAD = 8;
-    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= rows) return;
-    const float* const x = partial + static_cast<size_t>(row) * splits * D + E * lane;
-    const float2 one = lane < splits ? reinterpret_cast<const float2*>(partial + static_cast<size_t>(rows) * splits * D)[static_cast<size_t>(row) * splits + lane]
-                                     : float2{-INFINITY, 0.0f};
+    const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (at >= B * rows) return;
+    const int b = at / rows, row = at - b * rows;                          // rows: of a sequence
+    const size_t all = static_cast<size_t>(parts) * rows;
+    const TreeShare share = reinterpret_cast<const TreeShare*>(partial + all * (D + 2))[b];
+    if (share.count == 1) return;                                          // written by its workgroups
+    const float* const x = partial + (static_cast<size_t>(share.first) * rows + row) * D + E * lane;
+    const float2 one = lane < share.count ? reinterpret_cast<const float2*>(partial + all * D)[static_cast<size_t>(share.first + lane) * rows + row] : float2{-INFINITY, 0.0f};
     float m = one.x;
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
@@ -367,25 +505,29 @@ __global__ __launch_bounds__(256) void terna_tree_merge_kernel(const float* __re
     float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-    for (int s0 = 0; s0 < splits; s0 += AHEAD) {
+    for (int s0 = 0; s0 < share.count; s0 += AHEAD) {
         float y[AHEAD][E];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[i][e] = x[static_cast<size_t>(min(s0 + i, splits - 1)) * D + e];
+        for (int i = 0; i < AHEAD; ++i) {
+            const float* const from = x + static_cast<size_t>(min(s0 + i, share.count - 1)) * rows * D;
+            if constexpr (E == 2) {
+                const float2 two = *reinterpret_cast<const float2*>(from);
+                y[i][0] = two.x, y[i][1] = two.y;
+            } else {
+                y[i][0] = *from;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const float w = s0 + i < splits ? __shfl(weight, s0 + i) : 0.0f;
+            const float w = __shfl(weight, min(s0 + i, share.count - 1));
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += w == 0.0f && s0 + i >= splits ? 0.0f : y[i][e] * w;
+            for (int e = 0; e < E; ++e) sum[e] += s0 + i < share.count ? y[i][e] * w : 0.0f;
         }
     }
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    if constexpr (E == 2) {
-        *reinterpret_cast<uint32_t*>(out + static_cast<size_t>(row) * D + 2 * lane) = l == 0.0f ? 0u : pack_bf16x2(sum[0] * inverse, sum[1] * inverse);
-    } else {
-        out[static_cast<size_t>(row) * D + lane] = l == 0.0f ? static_cast<uint16_t>(0) : float_to_bf16_bits(sum[0] * inverse);
-    }
+    uint16_t* const to = out + static_cast<size_t>(at) * D + E * lane;
+    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(to) = l == 0.0f ? 0u : pack_bf16x2(sum[0] * inverse, sum[1] * inverse);
+    else *to = l == 0.0f ? static_cast<uint16_t>(0) : float_to_bf16_bits(sum[0] * inverse);
 }
 
 }  // namespace terna
