@@ -37,7 +37,8 @@ inline Int8Plan int8_plan(int M, int N, int K, bool room)
         const Int8TileTime& t = kInt8Tiles[i];
         const long long tiles = static_cast<long long>((M + t.rows - 1) / t.rows) * ((N + t.features - 1) / t.features);
         for (int splits = 1; splits <= (room && i == kInt8SplitTile ? kInt8MaxSplits : 1); ++splits) {
-            const int steps = (blocks / 2 + splits - 1) / splits * 2;                   // (whole stages of 128 columns)
+            const int share = (blocks / 2 + splits - 1) / splits, steps = 2 * share;    // (whole stages of 128 columns)
+            if (splits > 1 && share * (splits - 1) >= blocks / 2) continue;             // a part without a stage
             const float wgs = static_cast<float>(tiles) * splits;
             if (splits > 1 && (wgs > 512.0f || steps < 4)) break;
             float time;

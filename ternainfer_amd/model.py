@@ -13,7 +13,8 @@ its last rows through the LM head with a PyTorch-ROCm matmul); one decode step i
 generate.py:204-224 does.
 
 Next to the bf16 cache, of up to 8192 slots for the kernels, stands one in 4 bits of any length (`Transformer.make_cache(..., bits=4)`), and
-`Transformer.score` gives the log probabilities of the tokens of a text.
+`Transformer.score` gives the log probabilities of the tokens of a text.  `Transformer.tree_step` runs a tree of drafted tokens through the model at once,
+`speculative_decode` decodes greedily by it; `Transformer.quantise_head` puts the projection to the vocabulary into 8 bits.
 """
 from __future__ import annotations
 
@@ -28,6 +29,8 @@ from . import _lib
 from .linear import (EPILOGUE_GATE, EPILOGUE_RESIDUAL, argmax_rows, attention_merge_rmsnorm_linear_packed, fused_linear, get_global_workspace, greedy_step,
                      greedy_step_state, interleave_gate_up, lm_head, prompt_inputs, quant_from_stats, quant_input, row_stats, relu2_mul_rmsnorm_linear_packed, relu2_mul_rmsnorm_quant, step_inputs,
                      repack_weight, rmsnorm_linear_packed, rmsnorm_quant)
+from .drafting import DraftTree, cache_move, draft_tree, tree_accept, tree_attention
+from .int8_linear import Int8Rows, int8_linear, quantise_rows
 from .long_context import Kv4Cache, TokenLogprobs, kv4_attention, kv4_step, kv4_store, rotary_frequencies, token_logprobs
 
 
@@ -114,6 +117,12 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, adjacent: 
 
 
 KERNEL_ATTENTION = object()    # in place of a mask: several new tokens, attention by ternaspmm_prefill_attention
+
+
+@dataclass
+class TreeNodes:                   # in place of a mask: the new tokens are the nodes of trees, attention by tree_attention
+    start: torch.Tensor            # int64 [B]: slots in front of them
+    mask: torch.Tensor             # int64 [B, T, words]: whom each sees among them
 
 
 class Block:
@@ -401,6 +410,8 @@ class Block:
         elif self.fused:
             # RoPE + cache write, and on the prompt pass the library's multi-token attention over the cache
             q = o = native.prompt_attention(*attend, mask is KERNEL_ATTENTION)
+            if isinstance(mask, TreeNodes):
+                o = tree_attention(q, cache_k, cache_v, mask.start, mask.mask)
         else:
             qkv = qkv.view(bsz, t, a.n_heads + 2 * a.n_kv_heads, a.head_dim).transpose(1, 2)
             q, k, v = qkv[:, :a.n_heads], qkv[:, a.n_heads:a.n_heads + a.n_kv_heads], qkv[:, a.n_heads + a.n_kv_heads:]
@@ -417,7 +428,7 @@ class Block:
             else:
                 cache_k.index_copy_(2, pos_idx, k)
                 cache_v.index_copy_(2, pos_idx, v)
-        if not one_token and mask is not KERNEL_ATTENTION and kv4 is None:
+        if not one_token and mask is not KERNEL_ATTENTION and not isinstance(mask, TreeNodes) and kv4 is None:
             kk = cache_k.repeat_interleave(rep, dim=1)
             vv = cache_v.repeat_interleave(rep, dim=1)
             o = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
@@ -733,10 +744,23 @@ class Transformer:
                 trace(index, x_in, pending_in, x, pending)
         return x, pending
 
+    head8: Optional[Int8Rows] = None       # see quantise_head
+
+    def quantise_head(self, on: bool = True) -> None:
+        """The projection to the vocabulary in 8 bits, a scale for every token of it (`int8_linear`), or, with `on` False, in bf16 again: half the bytes of what a step
+        reads most of (one row of the 128256 x 2560 shape 115 -> 60 us; 60 rows by a bf16 library product 173 -> 70).  Logits then differ by the rounding of weights and
+        rows to 8 bits; the embedding itself stays as it is.  To be called again where the embedding is changed."""
+        self.head8 = quantise_rows(self.tok_embeddings) if on else None
+
     def head(self, x, pending, bsz):
         """Logits of the rows x (+ pending): last residual add, final norm, LM head."""
+        return self.project(self.final_norm(x, pending), bsz)
+
+    def project(self, x, bsz):
+        """Logits of normed rows."""
         a = self.args
-        x = self.final_norm(x, pending)
+        if self.head8 is not None:
+            return int8_linear(x, self.head8)
         if x.is_cuda and bsz <= 16 and a.dim % 32 == 0 and bsz * (2 * a.dim + 16) <= 160 * 1024:
             return lm_head(x, self.tok_embeddings)                            # tied LM head (model.py:367): one HBM-bound pass
         return F.linear(x, self.tok_embeddings)
@@ -747,6 +771,26 @@ class Transformer:
         if self.layers[0].fused and x.is_cuda:                                # one launch
             return rmsnorm_quant(x, self.norm, a.norm_eps, residual=pending, quant=False)[0]     # (pending None: the stream has it)
         return rms_norm(x + pending, self.norm, a.norm_eps)
+
+    def tree_step(self, tokens: torch.Tensor, cache, start: torch.Tensor, tree: DraftTree) -> torch.Tensor:
+        """The nodes of trees in one pass: tokens int64 [B, T], `start` int64 [B] cache slots in front of each tree, `tree` of `draft_tree`.  Node i's key and
+        value go to slot start + i, at the position start + depth; every node sees the slots in front and its ancestors.  Returns logits [B, T, vocab].  (Padding writes
+        nothing, and its logits do not matter; so all of a sequence with a negative start.)  For the bf16 cache and the fused kernels."""
+        a = self.args
+        bsz, t = tokens.shape
+        if isinstance(cache[0], Kv4Cache) or not self.layers[0].fused or not tokens.is_cuda or a.head_dim not in (64, 128) or a.dim % 8:
+            raise ValueError("tree_step: only with a bf16 cache and the fused kernels, on a GPU, heads of 64 or 128 dimensions")
+        if tuple(start.shape) != (bsz,) or tuple(tree.depth.shape) != (bsz, t):
+            raise ValueError("tree_step: one start a sequence, a tree of its tokens")
+        max_seq = cache[0][0].shape[2]
+        real = (tree.depth >= 0) & (start >= 0)[:, None]
+        slots = torch.where(real, start[:, None] + torch.arange(t, device=tokens.device), -1)
+        table = self.rope_tables(max_seq, tokens.device)
+        x, cos, sin = prompt_inputs(tokens, (start[:, None] + tree.depth).clamp(0, max_seq - 1), self.tok_embeddings, table)
+        nodes, pending = TreeNodes(start, tree.mask), None
+        for layer, (ck, cv) in zip(self.layers, cache):
+            x, pending = layer.forward(x, pending, ck, cv, slots, cos, sin, nodes)
+        return self.head(x, pending, bsz * t).view(bsz, t, -1)
 
     score_rows = 1024              # rows of logits that `score` holds at a time (1024 x 128256 in bf16: 263 MB)
 
@@ -767,7 +811,7 @@ class Transformer:
         if lens is not None:
             targets = targets.masked_fill(torch.arange(1, t, device=dev) >= lens.to(dev)[:, None], -1)
         targets, h = targets.view(-1), self.final_norm(x, pending)
-        parts = [token_logprobs(F.linear(h[i:i + self.score_rows], self.tok_embeddings), targets[i:i + self.score_rows], top)
+        parts = [token_logprobs(self.project(h[i:i + self.score_rows], self.score_rows), targets[i:i + self.score_rows], top)
                  for i in range(0, h.shape[0], self.score_rows)]
         join = lambda field: None if field[0] is None else torch.cat(field).view(bsz, t - 1, *field[0].shape[1:])
         return TokenLogprobs(*map(join, zip(*parts)))
@@ -851,3 +895,64 @@ def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use
     seconds = _greedy_steps(step, gen_tokens, use_graph)
     result = out, ev[0].elapsed_time(ev[1]) * 1e-3, seconds
     return result if history is None else (*result, TokenLogprobs(*[None if f is None else f[:, :gen_tokens] for f in history]))
+
+
+def ngram_drafts(text: torch.Tensor, length: torch.Tensor, branches: int = 2, depth: int = 4):
+    """Drafts by looking the text up in itself: where its last two tokens stood before -- the latest `branches` places -- what followed there, `depth` tokens
+    each.  text int64 [B, L], `length` int64 [B] tokens of it that count.  Returns (tokens, parents) int64 [B, 1 + branches * depth]: the last token and, behind it, a
+    branch for every place; parents of -2 (padding) where there is none, or where the text ends.  On the device alone: it can be captured."""
+    bsz, cap = text.shape
+    dev = text.device
+    last = length[:, None] - 1
+    root, before = text.gather(1, last.clamp(min=0)), text.gather(1, (last - 1).clamp(min=0))
+    at = torch.arange(cap, device=dev)
+    match = (text == root) & (torch.cat([text[:, :1] - text[:, :1] - 1, text[:, :-1]], 1) == before) & (at < last) & (last >= 2)
+    places = torch.topk(torch.where(match, at, -1), min(branches, cap), 1).values                            # latest first
+    places = torch.cat([places, places.new_full((bsz, branches - places.shape[1]), -1)], 1)
+    ahead = places[:, :, None] + 1 + torch.arange(depth, device=dev)                                         # [B, branches, depth]
+    real = (places >= 0)[:, :, None] & (ahead <= last[:, :, None])
+    tokens = torch.where(real, text.gather(1, ahead.clamp(0, cap - 1).view(bsz, -1)).view_as(ahead), 0)
+    node = 1 + torch.arange(branches * depth, device=dev).view(branches, depth)
+    parents = torch.where(torch.arange(depth, device=dev) == 0, 0, node - 1)
+    parents = torch.where(real, parents, -2)
+    head = torch.where(length[:, None] > 0, -1, -2)
+    return torch.cat([root, tokens.view(bsz, -1)], 1), torch.cat([head, parents.view(bsz, -1)], 1)
+
+
+@torch.inference_mode()
+def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, draft=ngram_drafts, prompt_lens=None):
+    """Prefill `prompt` [B, P], then greedy decoding by drafted tokens: a step runs a tree of them through the model (`Transformer.tree_step`), keeps the branch that the
+    model would have written itself and the token behind it (`tree_accept`), and puts its keys and values where the text ends (`cache_move`) -- one token a
+    step at least.  `draft(text, length)` proposes: int64 (tokens, parents) [B, T] from the text so far, int64 [B, L], and its length [B]; node 0 is the text's last
+    token.  Returns (tokens [B, gen_tokens], steps).  The tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the
+    two ways.  `prompt_lens` as there."""
+    bsz, plen = prompt.shape
+    dev = prompt.device
+    if gen_tokens < 1:
+        return prompt.new_empty((bsz, 0)), 0
+    lens = torch.full((bsz,), plen, dtype=torch.int64, device=dev) if prompt_lens is None else prompt_lens.to(device=dev, dtype=torch.int64)
+    text = torch.cat([prompt, prompt.new_zeros((bsz, gen_tokens))], 1)
+    text[torch.arange(plen + gen_tokens, device=dev) >= lens[:, None]] = 0
+    widest = draft(text, lens)[0].shape[1]                                    # nodes of a step
+    cache = model.make_cache(bsz, plen + gen_tokens + widest)
+    logits = model.forward(prompt, cache, torch.arange(plen, device=dev), last_idx=lens - 1)
+    text.scatter_(1, lens[:, None], argmax_rows(logits.contiguous()))
+    length, whole, steps = lens + 1, lens + gen_tokens, 0
+    while bool((length < whole).any()):
+        on = length < whole                                                   # sequences that are not done
+        tokens, parents = draft(text, length)
+        parents = torch.where(on[:, None], parents, -2)
+        start = length - 1                                                    # (the last token is not in the cache yet)
+        step_logits = model.tree_step(tokens, cache, start, draft_tree(parents))
+        path, count, behind = tree_accept(step_logits, tokens, parents)
+        cache_move([c for pair in cache for c in pair], start, path, count)
+        # the accepted nodes but the root, and the token behind them
+        t = tokens.shape[1]
+        following = torch.cat([path[:, 1:], path.new_full((bsz, 1), -1)], 1)
+        new = torch.where(following >= 0, tokens.gather(1, following.clamp(min=0)), behind[:, None])
+        at = length[:, None] + torch.arange(t, device=dev)
+        fits = (torch.arange(t, device=dev) < count[:, None]) & (at < whole[:, None])
+        text = torch.cat([text, text.new_zeros((bsz, 1))], 1).scatter_(1, torch.where(fits, at, text.shape[1]), new)[:, :-1].contiguous()
+        length = torch.minimum(length + count, whole)
+        steps += 1
+    return text.gather(1, lens[:, None] + torch.arange(gen_tokens, device=dev)), steps
