@@ -764,7 +764,8 @@ long long ternaspmm_tree_accept_workspace_bytes(int B, int T, int V, int fp32);
 int ternaspmm_tree_accept(const void* logits, long long row, int fp32, const long long* tokens, const long long* parents, long long* path, long long* count, long long* next,
                           void* workspace, int B, int T, int V, terna_stream stream);
 /* Rows of n caches, of any types: slot start[b] + path[b][i] -> start[b] + i for i < count[b] (at most T), of every head.  A path ascends, as ternaspmm_tree_accept's do; a row
- * outside the cache, one in front of its place, and the rows of a sequence whose start lies outside the cache stay.  Strides and `bytes` of a row in bytes, slot >= bytes. */
+ * outside the cache, one in front of its place, and the rows of a sequence whose start lies outside the cache stay.  Strides and `bytes` of a row in bytes,
+ * slot >= bytes, heads * bytes at most 2^30. */
 typedef struct ternaspmm_cache_rows {
     void* rows;
     long long sequence, head, slot;

@@ -22,7 +22,7 @@ void launch_quantise(const E* x, long long row, void* packed, float* scale, int 
     uint8_t* const to = static_cast<uint8_t*>(packed);
     const int held = (4 * int8_k_blocks(K) + 63) / 64;
     auto kernel = held <= 1 ? terna_int8_quantise_kernel<E, 1> : held <= 3 ? terna_int8_quantise_kernel<E, 3> : terna_int8_quantise_kernel<E, 7>;
-    launch(kernel, dim3((R + 3) / 4), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
+    launch(kernel, dim3((R + 31) / 32 * 8), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
 }
 
 template <typename Out, int KIND, int WN, int WM, int NA, int MB, int SK, int ST>

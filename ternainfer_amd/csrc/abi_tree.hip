@@ -32,35 +32,37 @@ bool strides_ok(const long long* s, int n)
     return true;
 }
 
-template <int D, int RW, int ST, bool TWO, int PER_SIMD>
+template <int D, int RW, int KW, int ST, bool TWO, int PER_SIMD>
 void launch_tree(const TreeAttention& a, long long grid, hipStream_t st)
 {
-    using Shape = TreeShape<D, RW, ST>;
-    auto kernel = terna_tree_attention_kernel<D, RW, ST, TWO, PER_SIMD>;
+    using Shape = TreeShape<D, RW, KW, ST>;
+    auto kernel = terna_tree_attention_kernel<D, RW, KW, ST, TWO, PER_SIMD>;
     if (Shape::kBytes > kPlainLds - 4096) allow_dynamic_lds(kernel, Shape::kBytes, "hipFuncSetAttribute(tree attention)", __LINE__);
-    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), Shape::kBytes, st, a);
+    launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(Shape::kThreads), Shape::kBytes, st, a);
 }
 template <int D>
-void launch_tree_attention(const TreeAttention& a, int rows, long long grid, hipStream_t st)
+void launch_tree_attention(const TreeAttention& a, const TreePlan& plan, long long grid, hipStream_t st)
 {
-    if (rows == 32) launch_tree<D, 1, D == 128 ? 2 : 4, true, 1>(a, grid, st);
-    else if (rows == 64) launch_tree<D, 2, D == 128 ? 2 : 4, true, 2>(a, grid, st);
-    else launch_tree<D, 4, 4, false, 2>(a, grid, st);
+    if (plan.rows == 32) launch_tree<D, 1, 4, D == 128 ? 2 : 4, true, 1>(a, grid, st);
+    else if (plan.rows == 64) launch_tree<D, 2, 2, D == 128 ? 2 : 4, true, 2>(a, grid, st);
+    else if (plan.groups == 1) launch_tree<D, 4, 1, 4, false, 2>(a, grid, st);
+    else launch_tree<D, 4, 2, 4, false, 2>(a, grid, st);
     if (a.parts != 0) {
         const int all = a.T * a.H;
         launch(terna_tree_merge_kernel<D>, dim3((a.B * all + 3) / 4), dim3(256), 0, st, a.partial, a.out, a.B, all, a.parts);
     }
 }
 
-// Parts of a row of logits: up to eight workgroups a CU, of a round of loads at least (512 rows of 128256: two a CU 30 us, eight 26).
-int accept_parts(int rows, int V, int fp32)
+// Parts of a row of logits: up to eight workgroups a CU, of a round of loads at least (acceptance of
+// 16 rows of 128256 with one part each 16.1 us, so 7.0; of 512 28.9, so 28.6).
+int accept_parts(long long rows, int V, int fp32)
 {
     const int pieces = V / (fp32 ? 4 : 8), round = kTreeThreads * kAcceptBatch;
     int parts = 1;
-    while (parts < 64 && 2ll * rows * parts <= 2048 && pieces > parts * round) parts *= 2;
+    while (parts < 64 && 2 * rows * parts <= 2048 && pieces > parts * round) parts *= 2;
     return parts;
 }
-bool accept_shape_ok(int B, int T, int V, int fp32) { return tree_nodes_ok(B, T) && V >= 1 && V <= 1 << 19 && launch_fits(static_cast<long long>(B) * T * accept_parts(B * T, V, fp32), kTreeThreads); }
+bool accept_shape_ok(int B, int T, int V, int fp32) { return tree_nodes_ok(B, T) && V >= 1 && V <= 1 << 19 && launch_fits(static_cast<long long>(B) * T * accept_parts(static_cast<long long>(B) * T, V, fp32), kTreeThreads); }
 
 }  // namespace
 
@@ -90,7 +92,7 @@ int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, co
                              float scale, terna_stream stream)
 {
     if (!tree_shape_ok(B, T, H, KV, D, S) || !q || !k || !v || !start || !mask || !out || !q_strides || !k_strides || !v_strides || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
-        !aligned16(out) || !aligned16(workspace) || !strides_ok(q_strides, 3) || !strides_ok(k_strides, 3) || !strides_ok(v_strides, 3) || !std::isfinite(scale) ||
+        !aligned16(out) || !aligned16(workspace) || !strides_ok(q_strides, 3) || !strides_ok(k_strides, 3) || !strides_ok(v_strides, 3) || !std::isfinite(scale * static_cast<float>(M_LOG2E)) ||
         k_strides[2] >= 1 << 24 || v_strides[2] >= 1 << 24)
         return -1;
     const TreePlan plan = tree_plan(B, T, H, KV, D, S);
@@ -103,8 +105,8 @@ int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, co
     a.parts = workspace && plan.splits > 1 ? B * plan.splits : 0, a.tiles = plan.tiles;
     a.scale = scale * static_cast<float>(M_LOG2E);
     const long long grid = ((static_cast<long long>(a.parts == 0 ? B : a.parts) * KV + 7) / 8) * 8 * plan.tiles;
-    if (D == 128) launch_tree_attention<128>(a, plan.rows, grid, static_cast<hipStream_t>(stream));
-    else launch_tree_attention<64>(a, plan.rows, grid, static_cast<hipStream_t>(stream));
+    if (D == 128) launch_tree_attention<128>(a, plan, grid, static_cast<hipStream_t>(stream));
+    else launch_tree_attention<64>(a, plan, grid, static_cast<hipStream_t>(stream));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) die("ternaspmm_tree_attention", e, __LINE__);
     return 0;
@@ -112,7 +114,7 @@ int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, co
 
 long long ternaspmm_tree_accept_workspace_bytes(int B, int T, int V, int fp32)
 {
-    return accept_shape_ok(B, T, V, fp32) ? static_cast<long long>(sizeof(AcceptBest)) * B * T * accept_parts(B * T, V, fp32) : -1;
+    return accept_shape_ok(B, T, V, fp32) ? static_cast<long long>(sizeof(AcceptBest)) * B * T * accept_parts(static_cast<long long>(B) * T, V, fp32) : -1;
 }
 
 int ternaspmm_tree_accept(const void* logits, long long row, int fp32, const long long* tokens, const long long* parents, long long* path, long long* count, long long* next,
@@ -121,7 +123,7 @@ int ternaspmm_tree_accept(const void* logits, long long row, int fp32, const lon
     if (!accept_shape_ok(B, T, V, fp32) || !logits || !tokens || !parents || !path || !count || !next || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 7) || row < 0 ||
         (reinterpret_cast<uintptr_t>(logits) & (fp32 ? 3 : 1)))
         return -1;
-    const int parts = accept_parts(B * T, V, fp32);
+    const int parts = accept_parts(static_cast<long long>(B) * T, V, fp32);
     AcceptBest* const best = static_cast<AcceptBest*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (fp32) launch(terna_accept_best_kernel<float>, dim3(B * T * parts), dim3(kTreeThreads), 0, st, static_cast<const float*>(logits), row, best, V, parts);
@@ -137,7 +139,8 @@ int ternaspmm_cache_move(const ternaspmm_cache_rows* caches, int n, const long l
     if (n < 0 || !tree_nodes_ok(B, T) || B > 65535 || !start || !path || !count || (n > 0 && !caches)) return -1;
     for (int i = 0; i < n; ++i) {
         const ternaspmm_cache_rows& c = caches[i];
-        if (!c.rows || c.heads < 1 || c.slots < 1 || c.bytes < 1 || c.slot < c.bytes || c.head < 0 || c.sequence < 0) return -1;
+        if (!c.rows || c.heads < 1 || c.slots < 1 || c.bytes < 1 || c.slot < c.bytes || c.head < 0 || c.sequence < 0 || static_cast<long long>(c.heads) * c.bytes > 1ll << 30)
+            return -1;
     }
     MoveCaches m{};
     for (int i0 = 0; i0 < n; i0 += kMoveCaches) {

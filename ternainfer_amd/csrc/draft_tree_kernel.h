@@ -13,7 +13,7 @@ constexpr int kTreeMaxNodes = 512, kTreeMaxWords = kTreeMaxNodes / 64;
 constexpr int kTreeThreads = 256, kTreeEach = kTreeMaxNodes / kTreeThreads;      // nodes of a thread
 
 // One workgroup a sequence.  Ancestors by doubling: a node takes over what the node that it points at has seen, and points where that one points;
-// nine rounds for the longest chain of 512, where walking it node by node is 512 reads of LDS one after the other (512 nodes in a chain: 7 us, so 25).
+// nine rounds for the longest chain of 512, where walking it node by node is 512 reads of LDS one after the other.  16 nodes 2.5 us, 64 sequences of 512 10.6.
 template <int W>
 __global__ __launch_bounds__(kTreeThreads) void terna_draft_tree_kernel(const long long* __restrict__ parents, long long* __restrict__ mask,
                                                                         long long* __restrict__ depth, int T)

@@ -4,6 +4,12 @@
 //
 // Both sides lie in blocks of 16 rows by 64 columns, 1 KB in the order in which the matrix cores' operands are read: a lane's 16 columns of a row are 16
 // bytes, 16 rows beside each other.  A block goes global -> LDS as it is, one load a wave, and a 32x32x32 operand is one conflict-free 16-byte read a lane.
+//
+// What bounds the product: of few rows the weights' bytes (a vocabulary of 128256 by 2560 and one row 58 us, 5.7 TB/s; a library's product in bf16 119), of many
+// the matrix instructions, at 2400 of the 5000 Tera-operations a second that they could have: integers that are not all alike draw so much power that the clock falls
+// (8192 x 8192 x 8192 455 us; 4096 x 13824 x 2560 147 us, 1980), and a library's own product in 8-bit integers of the same shape reaches 2300.  Between
+// them it is what a CU can fetch: a stage of a 64 x 64 tile is 16 KB for 0.18 us (333 x 2501 x 6912, 240 workgroups: 14.8 us; a second group of four waves for
+// half of a stage's columns changes nothing there, nor do two parts with a launch that joins them, 19.6).
 #pragma once
 
 #include "int8_plan.h"
@@ -63,15 +69,17 @@ struct Int8Piece {
     }
 };
 
-// A wave a row, HELD pieces of 16 columns a lane in registers; longer rows are read again for their integers.  (2048 rows of 2560: 4 us, 13 where sixteen threads took
-// a row, read twice.)
+// A wave a row, HELD pieces of 16 columns a lane in registers; longer rows are read again for their integers.  2048 rows of 2560 take 5.6 us, 13 where
+// sixteen threads took a row, read twice; 8192 of 6912 43 us, 4 TB/s.
 template <typename E, int HELD>
 __global__ __launch_bounds__(kInt8Threads) void terna_int8_quantise_kernel(const E* __restrict__ x, long long row_stride, uint8_t* __restrict__ packed,
                                                                            float* __restrict__ scale, int R, int K, int wide)
 {
 // the product is rounded before it is rounded to an integer
 #pragma clang fp contract(off)
-    const int lane = threadIdx.x & 63, r = blockIdx.x * (kInt8Threads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Workgroups go to the XCDs round robin: each XCD takes a run of the rows, whose pieces -- eight rows' to a line of memory -- meet in its L2 (8192 x 6912: 46 us without)
+    const int lane = threadIdx.x & 63, group = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int r = group * (kInt8Threads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (r >= R) return;
     const int k_blocks = int8_k_blocks(K), pieces = 4 * k_blocks;
     const E* const row = x + static_cast<size_t>(r) * row_stride;
@@ -122,7 +130,7 @@ __global__ __launch_bounds__(kInt8Threads) void terna_int8_quantise_kernel(const
     }
 }
 
-// int8 rows as they are: a wave four blocks of a band, whole kilobytes out  (8192 x 6912: 38 us with a wave a row, whose pieces go out one by one)
+// int8 rows as they are: a wave four blocks of a band, whole kilobytes out: 8192 x 6912 20 us, 38 with a wave a row, whose pieces go out one by one
 constexpr int kInt8PackBlocks = 4;
 __global__ __launch_bounds__(kInt8Threads) void terna_int8_pack_kernel(const uint8_t* __restrict__ x, long long row_stride, uint8_t* __restrict__ packed, int R, int K, int wide)
 {

@@ -1276,7 +1276,7 @@ TERNA_FUNCTION(tree_attention, 6)
         refuse("%s: mask is int64 [T, W] or [B, T, W] with W = (T + 63) / 64", who);
     check_device(who, "mask", mask, k);
     const float scale = scale_of(given_scale, d);
-    if (!std::isfinite(scale)) refuse("%s: a scale that is not finite", who);
+    if (!std::isfinite(scale * static_cast<float>(M_LOG2E))) refuse("%s: a scale that is not finite, in powers of two", who);
     Guard guard;
     on_device_of(guard, k);
     Unlocked unlocked;

@@ -6,15 +6,21 @@
 // The rows of a kv head -- its G = H / KV query heads times the nodes, row r = node * G + head -- are the columns of 32x32x16 products, 32 a wave: the scores
 // (slots x rows) come out of the matrix cores in the layout in which their exponentials go back in as the second product's operand, and a row's maximum
 // and sum are one exchange between two lanes.
-//   * A workgroup is four waves: RW of them share the slots, 32 rows each, and 4 / RW groups of those take turns of 32 slots, so that a few rows still
-//     read a cache with four waves.  The groups' numerators are joined in LDS at the end, the splits' by a second launch.
+//   * RW waves of a workgroup share the slots, 32 rows each, and KW groups of those take turns of 32 slots, so that a few rows still read a cache with four waves
+//     and many leave few numerators to join.  The groups' are joined in LDS at the end, the splits' by a second launch (which groups, how many splits: tree_plan.h).
 //   * Keys and values go global -> LDS directly, ST - 1 steps ahead; 16-byte pieces are XOR-swizzled on the way, so that neither the keys' 16-byte operand reads
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
-//   * Probabilities are two bf16, high and low part: 16 bits of them count.  The running maximum is raised, and the output rescaled, only where it grows by
-//     more than 2^3 -- a row's own.
+//   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 16 bits of them count, and the second product's extra instructions are hidden
+//     there by the cache.  With more rows the kernel is bound by its instructions and they are one bf16, their sum taken of the rounded ones, so that rounding
+//     leaves the weights a sum of one: 60 nodes of 4 heads over 32768 slots 42 us, with two 48; largest error of values of unit variance 2.1e-3, with two 1.7e-3.
+//     The running maximum is raised, and the output rescaled, only where it grows by more than
+//     2^3 -- a row's own.
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
-// What bounds it: see the launch's side (abi_tree.hip) and the times there.
+// What bounds it: of few rows a sequence and many sequences the cache's bytes (64 sequences of one token over 8000 slots 229 us, 5.7 TB/s; 32 of 13 nodes over
+// 3500 119 us, 4.9), of many rows the steps -- 32 slots of 128 rows: 512 clocks of matrix instructions a wave, 420 of exponentials and the like, 24 LDS reads;
+// they overlap in part, 0.64 us a step with one wave to a SIMD, 1.0 with two, which is 45 % of the rate that the matrix instructions alone would have -- and with little to
+// read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 7 for the second launch.
 #pragma once
 
 #include "draft_tree_kernel.h"
@@ -50,14 +56,14 @@ struct TreeShare {
     int first, count;
 };
 
-// A workgroup's shape: four waves, RW of them share the slots, 32 query rows each; ST tiles of keys and values in each group's ring.
-template <int D, int RW, int ST>
+// A workgroup's shape: KW groups of RW waves that share the slots, 32 query rows each; ST tiles of keys and values in each group's ring.
+template <int D, int RW, int KW, int ST>
 struct TreeShape {
-    static constexpr int KW = 4 / RW;                                      // groups
+    static constexpr int kWaves = RW * KW, kThreads = 64 * kWaves;
     static constexpr int kTile = kTreeTile * D * 2;                        // bytes of a tile's keys, or values
     static constexpr int kRing = KW * ST * 2 * kTile;
     static constexpr int kRow = D / 2 + 4;                                 // floats of a row of numerators in LDS, half of its dimensions at a time
-    static constexpr int kJoin = 4 * 32 * kRow * 4;
+    static constexpr int kJoin = kWaves * 32 * kRow * 4;
     static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
 
@@ -143,15 +149,15 @@ __device__ __forceinline__ TreePart tree_part(const TreeAttention& a, int part)
     }
 }
 
-template <int D, int RW, int ST, bool TWO, int PER_SIMD>
-__global__ __launch_bounds__(256, PER_SIMD) void terna_tree_attention_kernel(TreeAttention a)
+template <int D, int RW, int KW, int ST, bool TWO, int PER_SIMD>
+__global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_kernel(TreeAttention a)
 {
     static_assert(ST == 2 || ST == 4);
-    using Shape = TreeShape<D, RW, ST>;
-    constexpr int KW = Shape::KW, KS = D / 16, DT = D / 32, TILE = Shape::kTile;
+    using Shape = TreeShape<D, RW, KW, ST>;
+    constexpr int KS = D / 16, DT = D / 32, TILE = Shape::kTile;
     constexpr int PIECES = D / 8, PER_LOAD = 64 / PIECES, PER_TILE = TILE / 1024, LOADS = 2 * PER_TILE / RW;       // rows of a 1 KB load; loads of a tile's keys; of a wave and step
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float2 stat[4][32];
+    __shared__ float2 stat[Shape::kWaves][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wave / RW, rw = wave % RW, qi = lane & 31, half = lane >> 5;
     // Workgroups go to the XCDs round robin: the row tiles of one part of a kv head -- which read the same slots -- eight apart, on one XCD.
@@ -194,16 +200,16 @@ __global__ __launch_bounds__(256, PER_SIMD) void terna_tree_attention_kernel(Tre
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-            if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-            if (a.scale == 0.0f) {
-                float x[8];
-                unpack_bf16x8(q[ks], x);
+        if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        if (a.scale == 0.0f) {
+            float x[8];
+            unpack_bf16x8(q[ks], x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
-                q[ks] = pack_bf16x8(x);
-            }
-            pin_registers(q[ks]);                                      // landed before the first hand-issued request
+            for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
+            q[ks] = pack_bf16x8(x);
         }
+        pin_registers(q[ks]);                                              // landed before the first hand-issued request
+    }
 
     // ---- the cache's tiles
     const uint8_t* const kb = reinterpret_cast<const uint8_t*>(a.k + b * a.k_seq + kvh * a.k_head);
@@ -425,7 +431,7 @@ __global__ __launch_bounds__(256, PER_SIMD) void terna_tree_attention_kernel(Tre
     if (half == 0) stat[wave][qi] = float2{m_run, l_run};
     const unsigned long long rows_outside = __ballot(outside), rows_active = __ballot(active);
     if (group == 0 && lane == 0) flags[rw][0] = static_cast<uint32_t>(rows_active), flags[rw][1] = static_cast<uint32_t>(rows_outside);
-    constexpr int EIGHTS = D / 16, STEP = 256 / EIGHTS;                    // of half a row; rows of the workgroup at a time, eight dimensions a thread
+    constexpr int EIGHTS = D / 16, STEP = Shape::kThreads / EIGHTS;                    // of half a row; rows of the workgroup at a time, eight dimensions a thread
 #pragma unroll
     for (int part_of = 0; part_of < 2; ++part_of) {
         if (part_of != 0) __syncthreads();

@@ -11,35 +11,46 @@ constexpr int kTreeMaxSplits = 64;             // parts of a row: one a lane of 
 
 struct TreePlan {
     int rows;                                  // query rows of a workgroup: 32, 64 or 128
+    int groups;                                // of its waves, that take turns of the tiles: 4, 2, and for 128 rows 1 or 2
     int tiles;                                 // workgroups along the rows of a kv head
     int splits;                                // parts that the slots are read in, of a sequence of the cache's length
 };
-// The parts by the time they take, us, fitted to 250 measured shapes and numbers of parts (an error of 12 %; the parts chosen by it took 1 % longer than the
-// best ones, 11 % at the worst): a step of a workgroup's four waves -- 4, 2 or 1 tiles -- 0.97, 1.03 or 0.75, 1.08 with a second workgroup of
-// 128 rows beside it; 8 around a workgroup's steps, 4 for the launch that joins the parts, their numerators written and read at 5.9 TB/s, and the cache
-// itself at 5.8, less where workgroups are fewer than the CUs or do not fill their last round.
+// The groups and the parts by the time they take, us: steps of a workgroup and what surrounds them, in rounds of the workgroups that there is room for, or the
+// cache's bytes -- at 5.8 TB/s, less where workgroups are fewer than the CUs or do not fill their last round --, and the launch that joins the parts, whose
+// numerators are written and read at 5.4 to 5.9.  Fitted to 250 measured shapes and numbers of parts of up to 64 rows (an error of 12 %) and 750 of more (13 %; the
+// plan chosen by it took 1.7 % longer than the best one in the mean of 31 shapes, 23 % at the worst).  128 rows in two groups are a workgroup of eight waves, one to a CU, with half
+// the numerators that two workgroups of four have: 240 rows over 32768 slots 40.6 us, with one group 45.0; where nothing is split and workgroups are many,
+// those of one group start and end while others compute: 32 sequences of 256 rows over 2048 slots 81 us, with two groups 91.
 inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
 {
     const long long rows = static_cast<long long>(T) * (H / KV), heads = static_cast<long long>(B) * KV, tiles = (S + kTreeTile - 1) / kTreeTile;
     TreePlan p;
     p.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-    const int together = 128 / p.rows;         // tiles of a workgroup's step
     const float cache = static_cast<float>(heads) * static_cast<float>(S) * static_cast<float>(4 * D) * 0.172e-6f;
-    auto time = [&](long long n) {
-        const float wgs = static_cast<float>(heads * p.tiles) * static_cast<float>(n), steps = static_cast<float>((tiles + together * n - 1) / (together * n));
-        const float places = wgs <= 256.0f || (p.rows == 32 && D == 128) ? 256.0f : 512.0f;        // (32 rows of 128 dimensions: one to a CU)
-        const float step = (p.rows == 32 ? 0.97f : p.rows == 64 ? 1.03f : places == 256.0f ? 0.75f : 1.08f) * (D == 64 ? 0.67f : 1.0f);
-        const float full = std::max(1.0f, wgs / places), whole = std::ceil(full), rounds = full > 3.0f ? full : 0.5f * (full + whole);
+    auto time = [&](int groups, long long n) {
+        const float wgs = static_cast<float>(heads * p.tiles) * static_cast<float>(n), steps = static_cast<float>((tiles + groups * n - 1) / (groups * n));
+        // (32 rows of 128 dimensions and eight waves: one to a CU)
+        const float places = wgs <= 256.0f || (p.rows == 32 && D == 128) || (p.rows == 128 && groups == 2) ? 256.0f : 512.0f;
+        float step, around = 8.0f;
+        if (p.rows == 32) step = 0.97f;
+        else if (p.rows == 64) step = 1.03f;
+        else if (groups == 2) step = 0.97f, around = 6.7f;
+        else if (places == 256.0f) step = 0.64f, around = 7.3f;
+        else step = 1.02f, around = 3.5f;
+        if (D == 64) step *= p.rows == 128 ? 0.52f : 0.67f;
+        const float full = std::max(1.0f, wgs / places), whole = std::ceil(full), rounds = full > 3.0f ? full : p.rows == 128 ? whole : 0.5f * (full + whole);
         const float memory = cache * std::pow(std::max(1.0f, 0.9f * places * whole / wgs), 0.6f);
-        return std::max(rounds * (8.0f + steps * step), memory + 8.0f) +
-               (n == 1 ? 0.0f : 4.0f + static_cast<float>(rows * heads) * static_cast<float>(8 * D * n) * 0.171e-6f);
+        return std::max(rounds * (around + steps * step), memory + 8.0f) +
+               (n == 1 ? 0.0f : (p.rows == 128 ? 7.1f : 4.0f) + static_cast<float>(rows * heads) * static_cast<float>(8 * D * n) * (p.rows == 128 ? 0.185e-6f : 0.171e-6f));
     };
-    p.splits = 1;
-    float best = time(1);
+    const int least = 128 / p.rows, widest = std::max(least, 2);
+    p.groups = least, p.splits = 1;
+    float best = time(least, 1);
     const long long most = std::min<long long>({kTreeMaxSplits, (tiles + 1) / 2, std::max(1ll, 4096 / (heads * p.tiles))});
-    for (long long n = 2; n <= most; ++n)
-        if (const float t = time(n); t < best) best = t, p.splits = static_cast<int>(n);
+    for (int groups = least; groups <= widest; ++groups)
+        for (long long n = 1; n <= most; ++n)
+            if (const float t = time(groups, n); t < best) best = t, p.groups = groups, p.splits = static_cast<int>(n);
     return p;
 }
 

@@ -8,7 +8,7 @@ using namespace terna;
 
 int main()
 {
-    int shapes = 0, split = 0, wrong = 0;
+    int shapes = 0, split = 0, wrong = 0, groups[5] = {};
     for (int B : {1, 2, 3, 8, 31, 64, 300, 65535})
         for (int T : {1, 2, 7, 16, 33, 64, 65, 512})
             for (int KV : {1, 2, 5, 8})
@@ -20,6 +20,8 @@ int main()
                             const long long rows = static_cast<long long>(T) * G, covered = static_cast<long long>(p.tiles) * p.rows;
                             ++shapes;
                             split += p.splits > 1;
+                            ++groups[p.groups < 1 || p.groups > 4 ? 0 : p.groups];
+                            if (p.groups * p.rows != 128 && !(p.rows == 128 && p.groups == 2)) std::printf("tree: %d rows in %d groups\n", p.rows, p.groups), ++wrong;
                             if ((p.rows != 32 && p.rows != 64 && p.rows != 128) || covered < rows || covered - rows >= p.rows || p.splits < 1 || p.splits > kTreeMaxSplits ||
                                 (p.splits > 1 && (p.splits - 1) * static_cast<long long>(kTreeTile) >= S)) {
                                 std::printf("tree: B %d T %d KV %d G %d D %d S %d: rows %d tiles %d splits %d\n", B, T, KV, G, D, S, p.rows, p.tiles, p.splits);
@@ -54,6 +56,7 @@ int main()
     for (int i = 0; i < kInt8TileKinds; ++i)
         if (!reached[i]) std::printf("int8: no shape takes tile %d\n", i), ++wrong;
     std::printf("%d shapes, %d trees in parts, %d products in parts, %d wrong\n", shapes, split, joined, wrong);
+    if (!groups[1] || !groups[2] || !groups[4]) std::printf("tree: no shape has 1, 2 or 4 groups\n"), ++wrong;
     if (wrong || !split || !joined) return 1;
     std::printf("draft plans ok\n");
     return 0;

@@ -71,7 +71,7 @@ def _case(b, t, h, kv, d, slots, seed, padding=0.0):
 @pytest.mark.parametrize("b,t,h,kv,slots,starts", [
     (1, 1, 1, 1, 1, (0,)), (2, 1, 20, 5, 40, (31, 0)), (3, 8, 20, 5, 100, (32, 33, 92)), (2, 13, 8, 4, 300, (256, 287)), (1, 16, 20, 5, 200, (161,)), (2, 17, 4, 1, 96, (64, 63)),
     (2, 33, 12, 6, 700, (600, 5)), (1, 60, 20, 5, 1200, (1100,)), (2, 64, 8, 1, 128, (64, 0)), (1, 65, 4, 4, 400, (303,)), (1, 130, 10, 2, 500, (300,)), (1, 512, 4, 2, 700, (101,)),
-    (1, 3, 64, 1, 90, (77,)), (1, 100, 17, 1, 333, (222,))])
+    (1, 3, 64, 1, 90, (77,)), (1, 100, 17, 1, 333, (222,)), (64, 20, 20, 5, 200, tuple(range(0, 192, 3))), (2, 70, 800, 200, 400, (300, 64))])
 def test_attention(d, b, t, h, kv, slots, starts):
     _say("tree attention", d, b, t, h, kv, slots, starts)
     q, k, v, mask = _case(b, t, h, kv, d, slots, 10, padding=0.1)
@@ -103,7 +103,7 @@ def test_attention_in_parts(d, b, t, h, kv, slots, starts):
     assert same_or_near(out.view(b, t, h, d), want, tol) <= 0
 
 
-@pytest.mark.parametrize("t,h,kv,slots", [(6, 20, 5, 200), (20, 8, 2, 200), (40, 20, 5, 300), (6, 20, 5, 8000)])
+@pytest.mark.parametrize("t,h,kv,slots", [(6, 20, 5, 200), (20, 8, 2, 200), (40, 20, 5, 300), (6, 20, 5, 8000), (40, 1200, 300, 300)])
 def test_what_a_node_does_not_see_does_not_reach_it(t, h, kv, slots):
     """Bit for bit: other nodes' queries; keys and values, finite ones, infinities and NaN, in the slots of nodes that are no ancestors, and behind the tree."""
     _say("unseen", t, h, kv, slots)
@@ -125,7 +125,7 @@ def test_what_a_node_does_not_see_does_not_reach_it(t, h, kv, slots):
             assert torch.equal(got[node], want[node]), (fill, node)
 
 
-@pytest.mark.parametrize("t,h,kv,start,slots", [(5, 4, 2, 70, 100), (5, 4, 2, 0, 100), (70, 8, 1, 100, 200), (9, 20, 5, 7000, 7100)])
+@pytest.mark.parametrize("t,h,kv,start,slots", [(5, 4, 2, 70, 100), (5, 4, 2, 0, 100), (70, 8, 1, 100, 200), (9, 20, 5, 7000, 7100), (40, 1200, 300, 190, 260)])
 def test_values_that_are_not_finite_where_they_are_seen(t, h, kv, start, slots):
     """Infinities and NaN among the seen slots -- of the text and of the tree -- come out where the definition has them."""
     _say("not finite", t, h, kv, start, slots)
@@ -222,6 +222,9 @@ def test_attention_refusals():
                  (q.cpu(), k, v, start, mask), (q, k, v, start.cpu(), mask), (q, k, v, start, mask.cpu())):
         with pytest.raises(ValueError, match="tree_attention"):
             T.tree_attention(*args)
+    for scale in (float("inf"), float("nan"), 3e38):                                     # (the last times log2(e) is none)
+        with pytest.raises(ValueError, match="tree_attention"):
+            T.tree_attention(q, k, v, start, mask, scale)
     with pytest.raises(ValueError, match="tree_attention"):
         T.tree_attention(_randn((1, 1, 513, 64), 102), k[:1, :1], v[:1, :1], start[:1], torch.ones((513, 9), dtype=torch.int64, device="cuda"))
 
