@@ -924,24 +924,34 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
     """Prefill `prompt` [B, P], then greedy decoding by drafted tokens: a step runs a tree of them through the model (`Transformer.tree_step`), keeps the branch that the
     model would have written itself and the token behind it (`tree_accept`), and puts its keys and values where the text ends (`cache_move`) -- one token a
     step at least.  `draft(text, length)` proposes: int64 (tokens, parents) [B, T] from the text so far, int64 [B, L], and its length [B]; node 0 is the text's last
-    token.  Returns (tokens [B, gen_tokens], steps).  The tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the
+    token, whatever they say there.  It is called once before the first step, for T, which later calls do not exceed.  Returns (tokens [B, gen_tokens], steps).  The tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the
     two ways.  `prompt_lens` as there."""
     bsz, plen = prompt.shape
     dev = prompt.device
     if gen_tokens < 1:
         return prompt.new_empty((bsz, 0)), 0
+    if prompt.dtype != torch.int64 or plen < 1 or (prompt_lens is not None and (tuple(prompt_lens.shape) != (bsz,) or not bool(((prompt_lens >= 1) & (prompt_lens <= plen)).all()))):
+        raise ValueError(f"speculative_decode: prompts are int64 [B, P], their lengths [B], each 1 .. P = {plen}")
     lens = torch.full((bsz,), plen, dtype=torch.int64, device=dev) if prompt_lens is None else prompt_lens.to(device=dev, dtype=torch.int64)
     text = torch.cat([prompt, prompt.new_zeros((bsz, gen_tokens))], 1)
     text[torch.arange(plen + gen_tokens, device=dev) >= lens[:, None]] = 0
-    widest = draft(text, lens)[0].shape[1]                                    # nodes of a step
+
+    def drafted(length, on):
+        tokens, parents = draft(text, length)
+        if tokens.dtype != torch.int64 or parents.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape != parents.shape or not 1 <= tokens.shape[1] <= widest or tokens.shape[0] != bsz:
+            raise ValueError(f"speculative_decode: drafts are int64 tokens and parents [B, T] with T = 1 .. {widest}, not {tuple(tokens.shape)} and {tuple(parents.shape)}")
+        last = text.gather(1, length[:, None] - 1)
+        return torch.cat([last, tokens[:, 1:]], 1), torch.where(on[:, None], torch.cat([torch.full_like(last, -1), parents[:, 1:]], 1), -2)
+
+    widest = 512
+    widest = drafted(lens, lens > 0)[0].shape[1]                              # nodes of a step
     cache = model.make_cache(bsz, plen + gen_tokens + widest)
     logits = model.forward(prompt, cache, torch.arange(plen, device=dev), last_idx=lens - 1)
     text.scatter_(1, lens[:, None], argmax_rows(logits.contiguous()))
     length, whole, steps = lens + 1, lens + gen_tokens, 0
     while bool((length < whole).any()):
         on = length < whole                                                   # sequences that are not done
-        tokens, parents = draft(text, length)
-        parents = torch.where(on[:, None], parents, -2)
+        tokens, parents = drafted(length, on)
         start = length - 1                                                    # (the last token is not in the cache yet)
         step_logits = model.tree_step(tokens, cache, start, draft_tree(parents))
         path, count, behind = tree_accept(step_logits, tokens, parents)

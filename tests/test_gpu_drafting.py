@@ -655,3 +655,34 @@ def test_a_head_in_8_bits():
     assert torch.equal(greedy_decode(model, tokens, 6)[0], eager)
     model.quantise_head(False)
     assert torch.equal(run(), before)
+
+
+def test_drafts_of_any_kind_and_refusals():
+    """A step takes one token at least, whatever the drafts say: roots that are none, tokens outside the vocabulary, parents anywhere."""
+    model, count = _model(0), 12
+    prompt = _tokens(2, 9)
+    lens = torch.tensor([9, 4])
+    alone = lambda text, length: (text[:, :5], torch.full((2, 5), -2, device="cuda"))      # (as many rows in the linears: the same bits)
+    plain, _ = speculative_decode(model, prompt, count, draft=alone, prompt_lens=lens)
+
+    def nonsense(text, length):
+        tokens = torch.tensor([[5, -1, 1 << 40, 1000, 999]], device="cuda").expand(2, 5).contiguous()
+        return tokens, torch.tensor([[-2, 0, 0, 7, -1], [3, 0, 1, 2, 1 << 40]], device="cuda")
+
+    got, steps = speculative_decode(model, prompt, count, draft=nonsense, prompt_lens=lens)
+    assert torch.equal(got, plain) and steps <= count
+    calls = []
+
+    def wider(text, length):
+        calls.append(0)
+        return torch.zeros((2, len(calls)), dtype=torch.int64, device="cuda"), torch.zeros((2, len(calls)), dtype=torch.int64, device="cuda")
+
+    for draft in (wider, lambda text, length: (text[:, :3], text[:, :2]), lambda text, length: (text[:, :0], text[:, :0]), lambda text, length: (text[:, :2].int(), text[:, :2].int()),
+                  lambda text, length: (text[:1, :2], text[:1, :2])):
+        with pytest.raises(ValueError, match="speculative_decode"):
+            speculative_decode(model, prompt, count, draft=draft)
+    for bad in (torch.tensor([9, 10]), torch.tensor([0, 3]), torch.tensor([9]), torch.tensor([-1, 1 << 40])):
+        with pytest.raises(ValueError, match="speculative_decode"):
+            speculative_decode(model, prompt, count, draft=alone, prompt_lens=bad)
+    with pytest.raises(ValueError, match="speculative_decode"):
+        speculative_decode(model, prompt.int(), count, draft=alone)
