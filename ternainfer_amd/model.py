@@ -920,12 +920,14 @@ def ngram_drafts(text: torch.Tensor, length: torch.Tensor, branches: int = 2, de
 
 
 @torch.inference_mode()
-def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, draft=ngram_drafts, prompt_lens=None):
+def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, draft=ngram_drafts, prompt_lens=None, use_graph: Optional[bool] = None):
     """Prefill `prompt` [B, P], then greedy decoding by drafted tokens: a step runs a tree of them through the model (`Transformer.tree_step`), keeps the branch that the
     model would have written itself and the token behind it (`tree_accept`), and puts its keys and values where the text ends (`cache_move`) -- one token a
     step at least.  `draft(text, length)` proposes: int64 (tokens, parents) [B, T] from the text so far, int64 [B, L], and its length [B]; node 0 is the text's last
-    token, whatever they say there.  It is called once before the first step, for T, which later calls do not exceed.  Returns (tokens [B, gen_tokens], steps).  The tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the
-    two ways.  `prompt_lens` as there."""
+    token, whatever they say there.  It is called once before the first step, for T, which later calls do not exceed.  Returns (tokens [B, gen_tokens], steps).  The
+    tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the two ways.  `prompt_lens` as there.
+    `use_graph`: the step is captured once and replayed; `draft` is called for the first step and the captured one alone then and works on the device only.  By
+    default where it is `ngram_drafts`."""
     bsz, plen = prompt.shape
     dev = prompt.device
     if gen_tokens < 1:
@@ -933,8 +935,10 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
     if prompt.dtype != torch.int64 or plen < 1 or (prompt_lens is not None and (tuple(prompt_lens.shape) != (bsz,) or not bool(((prompt_lens >= 1) & (prompt_lens <= plen)).all()))):
         raise ValueError(f"speculative_decode: prompts are int64 [B, P], their lengths [B], each 1 .. P = {plen}")
     lens = torch.full((bsz,), plen, dtype=torch.int64, device=dev) if prompt_lens is None else prompt_lens.to(device=dev, dtype=torch.int64)
-    text = torch.cat([prompt, prompt.new_zeros((bsz, gen_tokens))], 1)
+    room = torch.cat([prompt, prompt.new_zeros((bsz, gen_tokens + 1))], 1)    # (a last column for what is not kept)
+    text = room[:, :-1]
     text[torch.arange(plen + gen_tokens, device=dev) >= lens[:, None]] = 0
+    whole, widest = lens + gen_tokens, 512
 
     def drafted(length, on):
         tokens, parents = draft(text, length)
@@ -943,26 +947,37 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
         last = text.gather(1, length[:, None] - 1)
         return torch.cat([last, tokens[:, 1:]], 1), torch.where(on[:, None], torch.cat([torch.full_like(last, -1), parents[:, 1:]], 1), -2)
 
-    widest = 512
     widest = drafted(lens, lens > 0)[0].shape[1]                              # nodes of a step
     cache = model.make_cache(bsz, plen + gen_tokens + widest)
+    caches = [c for pair in cache for c in pair]
     logits = model.forward(prompt, cache, torch.arange(plen, device=dev), last_idx=lens - 1)
     text.scatter_(1, lens[:, None], argmax_rows(logits.contiguous()))
-    length, whole, steps = lens + 1, lens + gen_tokens, 0
-    while bool((length < whole).any()):
-        on = length < whole                                                   # sequences that are not done
+    length, left = lens + 1, torch.zeros((), dtype=torch.bool, device=dev)    # left: sequences that are not done
+
+    def step():
+        on = length < whole
         tokens, parents = drafted(length, on)
         start = length - 1                                                    # (the last token is not in the cache yet)
         step_logits = model.tree_step(tokens, cache, start, draft_tree(parents))
         path, count, behind = tree_accept(step_logits, tokens, parents)
-        cache_move([c for pair in cache for c in pair], start, path, count)
+        cache_move(caches, start, path, count)
         # the accepted nodes but the root, and the token behind them
-        t = tokens.shape[1]
         following = torch.cat([path[:, 1:], path.new_full((bsz, 1), -1)], 1)
         new = torch.where(following >= 0, tokens.gather(1, following.clamp(min=0)), behind[:, None])
-        at = length[:, None] + torch.arange(t, device=dev)
-        fits = (torch.arange(t, device=dev) < count[:, None]) & (at < whole[:, None])
-        text = torch.cat([text, text.new_zeros((bsz, 1))], 1).scatter_(1, torch.where(fits, at, text.shape[1]), new)[:, :-1].contiguous()
-        length = torch.minimum(length + count, whole)
+        at = length[:, None] + torch.arange(tokens.shape[1], device=dev)
+        fits = (torch.arange(tokens.shape[1], device=dev) < count[:, None]) & (at < whole[:, None])
+        room.scatter_(1, torch.where(fits, at, text.shape[1]), new)
+        length.copy_(torch.minimum(length + count, whole))
+        left.copy_((length < whole).any())
+
+    steps, again, captured = 0, step, draft is ngram_drafts if use_graph is None else use_graph
+    left.copy_((length < whole).any())
+    while bool(left):
+        if captured and steps == 1:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+            again = graph.replay
+        again()
         steps += 1
     return text.gather(1, lens[:, None] + torch.arange(gen_tokens, device=dev)), steps

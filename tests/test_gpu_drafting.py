@@ -686,3 +686,32 @@ def test_drafts_of_any_kind_and_refusals():
             speculative_decode(model, prompt, count, draft=alone, prompt_lens=bad)
     with pytest.raises(ValueError, match="speculative_decode"):
         speculative_decode(model, prompt.int(), count, draft=alone)
+
+
+@pytest.mark.parametrize("batch,length", [(1, 40000), (3, 700), (1, 3)])
+def test_drafts_captured(batch, length):
+    """`ngram_drafts` in a graph that is replayed on other texts, with eager work between, says what it says eagerly."""
+    _say("drafts captured", batch, length)
+    text, count = torch.zeros((batch, length), dtype=torch.int64, device="cuda"), torch.full((batch,), length, device="cuda")
+    ngram_drafts(text, count)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ngram_drafts(text, count)
+    for i in range(6):
+        text.copy_(_tokens(batch, length, seed=40 + i) % (5 + 40 * i))
+        count.copy_(torch.randint(1, length + 1, (batch,), generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        want = ngram_drafts(text, count)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize("lens", [None, [30, 7, 19, 22]])
+def test_speculative_decode_captured(lens):
+    """The captured step gives the eager one's tokens, in as many steps."""
+    model, prompt = _model(1), _tokens(4, 10).repeat(1, 3)
+    lens = None if lens is None else torch.tensor(lens)
+    want, steps = speculative_decode(model, prompt, 50, prompt_lens=lens, use_graph=False)
+    for graph in (None, True):
+        got, replays = speculative_decode(model, prompt, 50, prompt_lens=lens, use_graph=graph)
+        assert torch.equal(got, want) and replays == steps
