@@ -62,7 +62,7 @@ struct TreeShape {
     static constexpr int kWaves = RW * KW, kThreads = 64 * kWaves;
     static constexpr int kTile = kTreeTile * D * 2;                        // bytes of a tile's keys, or values
     static constexpr int kRing = KW * ST * 2 * kTile;
-    static constexpr int kRow = D / 2 + 4;                                 // floats of a row of numerators in LDS, half of its dimensions at a time
+    static constexpr int kRow = D + 4;                                     // floats of a row of numerators in LDS
     static constexpr int kJoin = kWaves * 32 * kRow * 4;
     static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
@@ -181,37 +181,11 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(row + 16 * ks + 8 * half);
     }
-    bool active = false, outside = part.start > a.S;                       // the row has a node; sees a slot behind the cache
-    for (int w = 0; w < a.W; ++w) {
-        const unsigned long long bits = w == 0 ? first_word : mask[w];
-        const int has = min(max(inside - 64 * w, 0), 64), in_tree = min(a.T - 64 * w, 64);
-        const unsigned long long fit = has == 64 ? ~0ull : (1ull << has) - 1, valid = in_tree == 64 ? ~0ull : (1ull << in_tree) - 1;
-        active |= (bits & valid) != 0;
-        outside |= (bits & valid & ~fit) != 0;
-    }
-    active = active && r < rows && part.start >= 0;
-    outside = outside && active;
-    const int n = __syncthreads_or(active) ? start + inside : 0;       // slots that the workgroup reads
+    // ---- the cache's tiles
+    const int n = part.start < 0 ? 0 : start + inside;                     // slots that the workgroup reads
     const int all_tiles = (n + kTreeTile - 1) / kTreeTile, share = (all_tiles + splits - 1) / splits;
     const int begin = part.split * share, end = min(begin + share, all_tiles);
-    const int steps = end > begin ? (end - begin + KW - 1) / KW : 0;       // of every group: a tile behind the end has no slot that counts
-
-    // a negative scale's sign, and a scale of zero (0 * -inf would unmask a slot), go into the queries
-    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-        if (a.scale == 0.0f) {
-            float x[8];
-            unpack_bf16x8(q[ks], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
-            q[ks] = pack_bf16x8(x);
-        }
-        pin_registers(q[ks]);                                              // landed before the first hand-issued request
-    }
-
-    // ---- the cache's tiles
+    const int all_steps = end > begin ? (end - begin + KW - 1) / KW : 0;   // of every group: a tile behind the end has no slot that counts
     const uint8_t* const kb = reinterpret_cast<const uint8_t*>(a.k + b * a.k_seq + kvh * a.k_head);
     const uint8_t* const vb = reinterpret_cast<const uint8_t*>(a.v + b * a.v_seq + kvh * a.v_head);
     uint8_t* const ring = smem + group * (ST * 2 * TILE);
@@ -243,6 +217,36 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
             }
         }
     };
+    if (all_steps > 0) load(0, 0);                                         // on its way while the masks are looked at
+
+    bool active = false, outside = part.start > a.S;                       // the row has a node; sees a slot behind the cache
+    for (int w = 0; w < a.W; ++w) {
+        const unsigned long long bits = w == 0 ? first_word : mask[w];
+        const int has = min(max(inside - 64 * w, 0), 64), in_tree = min(a.T - 64 * w, 64);
+        const unsigned long long fit = has == 64 ? ~0ull : (1ull << has) - 1, valid = in_tree == 64 ? ~0ull : (1ull << in_tree) - 1;
+        active |= (bits & valid) != 0;
+        outside |= (bits & valid & ~fit) != 0;
+    }
+    active = active && r < rows && part.start >= 0;
+    outside = outside && active;
+    const bool needed = __syncthreads_or(active);
+    const int steps = needed ? all_steps : 0;
+
+    // a negative scale's sign, and a scale of zero (0 * -inf would unmask a slot), go into the queries
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        if (a.scale < 0.0f) q[ks] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        if (a.scale == 0.0f) {
+            float x[8];
+            unpack_bf16x8(q[ks], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= 0.0f;
+            q[ks] = pack_bf16x8(x);
+        }
+        pin_registers(q[ks]);                                              // landed before the next hand-issued request
+    }
+
     int va[DT];
     const int vrow = 4 * half + ((lane & 15) >> 2);
 #pragma unroll
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     };
     float l_run = 0.0f, m_run = -INFINITY;
     // steps whose tiles lie in front of the tree, all of them
-    const int plain = max(min(start / kTreeTile, end) - begin, 0) / KW;
+    const int plain = needed ? max(min(start / kTreeTile, end) - begin, 0) / KW : 0;
     int at = 0;                                                            // place in the ring
     auto take = [&](int step, auto last_tiles, auto place) __attribute__((always_inline)) {
         constexpr bool LAST = decltype(last_tiles)::value;                 // may have slots of the tree, or behind the end
@@ -386,7 +390,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     };
     if (steps > 0) {
 #pragma unroll
-        for (int i = 0; i < ST - 1; ++i) load(i, i);
+        for (int i = 1; i < ST - 1; ++i) load(i, i);
     }
     using Anywhere = std::integral_constant<int, -1>;
     int step = 0;
@@ -431,59 +435,55 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     if (half == 0) stat[wave][qi] = float2{m_run, l_run};
     const unsigned long long rows_outside = __ballot(outside), rows_active = __ballot(active);
     if (group == 0 && lane == 0) flags[rw][0] = static_cast<uint32_t>(rows_active), flags[rw][1] = static_cast<uint32_t>(rows_outside);
-    constexpr int EIGHTS = D / 16, STEP = Shape::kThreads / EIGHTS;                    // of half a row; rows of the workgroup at a time, eight dimensions a thread
+    constexpr int EIGHTS = D / 8, STEP = Shape::kThreads / EIGHTS;               // of a row; rows of the workgroup at a time, eight dimensions a thread
 #pragma unroll
-    for (int part_of = 0; part_of < 2; ++part_of) {
-        if (part_of != 0) __syncthreads();
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT / 2; ++dt)
+        for (int i = 0; i < 4; ++i) {
+            const f32x16& x = o[dt];
+            *reinterpret_cast<f32x4*>(join + (wave * 32 + qi) * ROW + 32 * dt + 8 * i + 4 * half) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        }
+    __syncthreads();
+    const int dim = (tid & (EIGHTS - 1)) * 8;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x16& x = o[part_of * (DT / 2) + dt];
-                *reinterpret_cast<f32x4*>(join + (wave * 32 + qi) * ROW + 32 * dt + 8 * i + 4 * half) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-            }
-        __syncthreads();
-        const int in_half = (tid & (EIGHTS - 1)) * 8, dim = part_of * (D / 2) + in_half;
+    for (int row0 = 0; row0 < 32 * RW; row0 += STEP) {
+        const int row = row0 + tid / EIGHTS, row_at = tile * (32 * RW) + row, rwave = row >> 5, in_wave = row & 31;
+        if ((STEP > 32 * RW && row >= 32 * RW) || row_at >= rows) continue;
+        const bool is_active = flags[rwave][0] >> in_wave & 1u, is_outside = flags[rwave][1] >> in_wave & 1u;
+        float m = -INFINITY, l = 0.0f, weight[KW], x[8];
 #pragma unroll
-        for (int row0 = 0; row0 < 32 * RW; row0 += STEP) {
-            const int row = row0 + tid / EIGHTS, row_at = tile * (32 * RW) + row, rwave = row >> 5, in_wave = row & 31;
-            if ((STEP > 32 * RW && row >= 32 * RW) || row_at >= rows) continue;
-            const bool is_active = flags[rwave][0] >> in_wave & 1u, is_outside = flags[rwave][1] >> in_wave & 1u;
-            float m = -INFINITY, l = 0.0f, weight[KW], x[8];
+        for (int g = 0; g < KW; ++g) m = fmaxf(m, stat[g * RW + rwave][in_wave].x);
+        const float m_use = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int g = 0; g < KW; ++g) m = fmaxf(m, stat[g * RW + rwave][in_wave].x);
-            const float m_use = m == -INFINITY ? 0.0f : m;
+        for (int g = 0; g < KW; ++g) {
+            const float2 one = stat[g * RW + rwave][in_wave];
+            weight[g] = KW == 1 ? 1.0f : __builtin_amdgcn_exp2f(one.x - m_use);
+            l += one.y * weight[g];
+        }
 #pragma unroll
-            for (int g = 0; g < KW; ++g) {
-                const float2 one = stat[g * RW + rwave][in_wave];
-                weight[g] = KW == 1 ? 1.0f : __builtin_amdgcn_exp2f(one.x - m_use);
-                l += one.y * weight[g];
-            }
+        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        for (int g = 0; g < KW; ++g) {
+            const float* const from = join + ((g * RW + rwave) * 32 + in_wave) * ROW + dim;
+            const f32x4 lower = *reinterpret_cast<const f32x4*>(from), upper = *reinterpret_cast<const f32x4*>(from + 4);
 #pragma unroll
-            for (int g = 0; g < KW; ++g) {
-                const float* const from = join + ((g * RW + rwave) * 32 + in_wave) * ROW + in_half;
-                const f32x4 lower = *reinterpret_cast<const f32x4*>(from), upper = *reinterpret_cast<const f32x4*>(from + 4);
+            for (int e = 0; e < 4; ++e) x[e] += lower[e] * weight[g], x[4 + e] += upper[e] * weight[g];
+        }
+        const int of_node = row_at / G;
+        const size_t out_row = (static_cast<size_t>(b) * a.T + of_node) * a.H + kvh * G + row_at - of_node * G;
+        // nothing seen: zeros
+        const float factor = is_outside ? NAN : !is_active || l == 0.0f ? 0.0f : splits > 1 ? 1.0f : 1.0f / l;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] += lower[e] * weight[g], x[4 + e] += upper[e] * weight[g];
-            }
-            const int of_node = row_at / G;
-            const size_t out_row = (static_cast<size_t>(b) * a.T + of_node) * a.H + kvh * G + row_at - of_node * G;
-            // nothing seen: zeros
-            const float factor = is_outside ? NAN : !is_active || l == 0.0f ? 0.0f : splits > 1 ? 1.0f : 1.0f / l;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = factor == 0.0f ? 0.0f : x[e] * factor;
-            if (splits > 1) {
-                const size_t all = static_cast<size_t>(a.T) * a.H, at = (part.share.first + part.split) * all + (out_row - b * all);
-                float* const to = a.partial + at * D + dim;
-                *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
-                *reinterpret_cast<f32x4*>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
-                if (dim == 0)
-                    reinterpret_cast<float2*>(a.partial + a.parts * all * D)[at] = is_outside ? float2{0.0f, 1.0f} : is_active ? float2{m, l} : float2{-INFINITY, 0.0f};
-            } else {
-                *reinterpret_cast<u32x4*>(a.out + out_row * D + dim) = pack_bf16x8(x);
-            }
+        for (int e = 0; e < 8; ++e) x[e] = factor == 0.0f ? 0.0f : x[e] * factor;
+        if (splits > 1) {
+            const size_t all = static_cast<size_t>(a.T) * a.H, at = (part.share.first + part.split) * all + (out_row - b * all);
+            float* const to = a.partial + at * D + dim;
+            *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+            if (dim == 0)
+                reinterpret_cast<float2*>(a.partial + a.parts * all * D)[at] = is_outside ? float2{0.0f, 1.0f} : is_active ? float2{m, l} : float2{-INFINITY, 0.0f};
+        } else {
+            *reinterpret_cast<u32x4*>(a.out + out_row * D + dim) = pack_bf16x8(x);
         }
     }
 }
