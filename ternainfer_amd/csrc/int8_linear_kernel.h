@@ -6,10 +6,10 @@
 // bytes, 16 rows beside each other.  A block goes global -> LDS as it is, one load a wave, and a 32x32x32 operand is one conflict-free 16-byte read a lane.
 //
 // What bounds the product: of few rows the weights' bytes (a vocabulary of 128256 by 2560 and one row 58 us, 5.7 TB/s; a library's product in bf16 119), of many
-// the matrix instructions, at 2400 of the 5000 Tera-operations a second that they could have: integers that are not all alike draw so much power that the clock falls
-// (8192 x 8192 x 8192 455 us; 4096 x 13824 x 2560 147 us, 1980), and a library's own product in 8-bit integers of the same shape reaches 2300.  Between
-// them it is what a CU can fetch: a stage of a 64 x 64 tile is 16 KB for 0.18 us (333 x 2501 x 6912, 240 workgroups: 14.8 us; a second group of four waves for
-// half of a stage's columns changes nothing there, nor do two parts with a launch that joins them, 19.6).
+// the matrix instructions, whose pipes are busy half of the clocks at 1.9 GHz (8192 x 8192 x 8192 460 us, 2390 Tera-operations a second, a library's own product in
+// 8-bit integers 480 to 500; 4096 x 13824 x 2560 147 us, 1980, of whose tiles the last round is a third full).  Between them it is what a CU can fetch: a stage of a
+// 64 x 64 tile is 16 KB for 0.18 us (333 x 2501 x 6912, 240 workgroups: 14.8 us; a second group of four waves for half of a stage's columns changes nothing there,
+// nor do two parts with a launch that joins them, 19.6).
 #pragma once
 
 #include "int8_plan.h"

@@ -13,13 +13,12 @@
 //   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 16 bits of them count, and the second product's extra instructions are hidden
 //     there by the cache.  With more rows the kernel is bound by its instructions and they are one bf16, their sum taken of the rounded ones, so that rounding
 //     leaves the weights a sum of one: 60 nodes of 4 heads over 32768 slots 42 us, with two 48; largest error of values of unit variance 2.1e-3, with two 1.7e-3.
-//     The running maximum is raised, and the output rescaled, only where it grows by more than
-//     2^3 -- a row's own.
+//     The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own.
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
 // What bounds it: of few rows a sequence and many sequences the cache's bytes (64 sequences of one token over 8000 slots 229 us, 5.7 TB/s; 32 of 13 nodes over
-// 3500 119 us, 4.9), of many rows the steps -- 32 slots of 128 rows: 512 clocks of matrix instructions a wave, 420 of exponentials and the like, 24 LDS reads;
-// they overlap in part, 0.64 us a step with one wave to a SIMD, 1.0 with two, which is 45 % of the rate that the matrix instructions alone would have -- and with little to
+// 7500 119 us, 4.9), of many rows the steps -- 32 slots of 128 rows: 512 clocks of matrix instructions a wave, 420 of exponentials and the like, 24 LDS reads;
+// of two waves to a SIMD they hardly overlap: 0.64 us a step with one wave, 1.0 with two, 43 % of the rate that the matrix instructions alone would have -- and with little to
 // read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 7 for the second launch.
 #pragma once
 
