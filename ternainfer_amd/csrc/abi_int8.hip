@@ -22,7 +22,7 @@ void launch_quantise(const E* x, long long row, void* packed, float* scale, int 
     uint8_t* const to = static_cast<uint8_t*>(packed);
     const int held = (4 * int8_k_blocks(K) + 63) / 64;
     auto kernel = held <= 1 ? terna_int8_quantise_kernel<E, 1> : held <= 3 ? terna_int8_quantise_kernel<E, 3> : terna_int8_quantise_kernel<E, 7>;
-    launch(kernel, dim3((R + 31) / 32 * 8), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
+    launch(kernel, dim3(static_cast<unsigned>((R + 31ll) / 32 * 8)), dim3(kInt8Threads), 0, st, x, row, to, scale, R, K, wide);
 }
 
 template <typename Out, int KIND, int WN, int WM, int NA, int MB, int SK, int ST>
@@ -66,7 +66,7 @@ long long ternaspmm_int8_bytes(int R, int K) { return int8_rows_ok(R, K) ? int8_
 
 int ternaspmm_int8_quantise(const void* x, long long row, int fp32, void* packed, float* scale, int R, int K, terna_stream stream)
 {
-    if (!int8_rows_ok(R, K) || !x || !packed || !scale || !aligned16(packed) || (reinterpret_cast<uintptr_t>(x) & (fp32 ? 3 : 1)) || row < 0 || !launch_fits((R + 3) / 4, kInt8Threads))
+    if (!int8_rows_ok(R, K) || !x || !packed || !scale || !aligned16(packed) || (reinterpret_cast<uintptr_t>(x) & (fp32 ? 3 : 1)) || row < 0 || !launch_fits((R + 31ll) / 32 * 8, kInt8Threads))
         return -1;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (fp32) launch_quantise(static_cast<const float*>(x), row, packed, scale, R, K, st);

@@ -568,6 +568,27 @@ def test_tree_step_is_the_operators_with_the_models_positions(act, shape, bsz, t
 
 
 @torch.inference_mode()
+def test_tree_step_behind_a_long_text(monkeypatch):
+    """More slots than the attention of other steps takes: every block's attention against 64 bits."""
+    model, t, start = _model(1), 11, 9000
+    a, cache, plain, calls = model.args, model.make_cache(1, start + t), model_module.tree_attention, []
+    for i, pair in enumerate(cache):
+        for j, c in enumerate(pair):
+            c[:, :, :start] = _randn(c[:, :, :start].shape, 300 + 2 * i + j)
+
+    def checked(q, k, v, first, mask, *rest):
+        got = plain(q, k, v, first, mask, *rest)
+        want, tol = P.attention(q, k, v, first, mask, a.head_dim ** -0.5)
+        assert same_or_near(got.view(1, t, a.n_heads, a.head_dim), want, tol) <= 0
+        calls.append(0)
+        return got
+
+    monkeypatch.setattr(model_module, "tree_attention", checked)
+    logits = model.tree_step(_tokens(1, t, seed=38), cache, torch.tensor([start], device="cuda"), T.draft_tree(P.random_parents(1, t, 39).cuda()))
+    assert torch.isfinite(logits).all() and len(calls) == 2
+
+
+@torch.inference_mode()
 def test_logits_of_a_node_do_not_depend_on_other_branches():
     """Bit for bit, whatever tokens the nodes have that are no ancestors of its."""
     model = _model(0)
