@@ -487,19 +487,27 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     }
 }
 
-// The parts' numerators of the sequences that have several, over their largest maximum: a wave a row, D / 64 dimensions a lane.
+// The parts' numerators of the sequences that have several, over their largest maximum: a wave a row, four dimensions a lane, so that two or four parts are read side by
+// side; the first of them on their way before their weights are known.
 template <int D>
 __global__ __launch_bounds__(256) void terna_tree_merge_kernel(const float* __restrict__ partial, uint16_t* __restrict__ out, int B, int rows, int parts)
 {
-    constexpr int E = D / 64, AHEAD = 8;
+    constexpr int LANES = D / 4, BESIDE = 64 / LANES, AHEAD = 8;           // lanes of a part; parts side by side; of a lane, in flight
     const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (at >= B * rows) return;
     const int b = at / rows, row = at - b * rows;                          // rows: of a sequence
     const size_t all = static_cast<size_t>(parts) * rows;
-    const TreeShare share = reinterpret_cast<const TreeShare*>(partial + all * (D + 2))[b];
+    const TreeShare share = B == 1 ? TreeShare{0, min(parts, kTreeMaxSplits)} : reinterpret_cast<const TreeShare*>(partial + all * (D + 2))[b];
     if (share.count == 1) return;                                          // written by its workgroups
-    const float* const x = partial + (static_cast<size_t>(share.first) * rows + row) * D + E * lane;
+    const int which = lane / LANES, piece = lane & (LANES - 1);
+    const float* const x = partial + (static_cast<size_t>(share.first) * rows + row) * D + 4 * piece;
+    f32x4 y[AHEAD];
+    auto fetch = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) y[i] = *reinterpret_cast<const f32x4*>(x + static_cast<size_t>(min(s0 + i * BESIDE + which, share.count - 1)) * rows * D);
+    };
     const float2 one = lane < share.count ? reinterpret_cast<const float2*>(partial + all * D)[static_cast<size_t>(share.first + lane) * rows + row] : float2{-INFINITY, 0.0f};
+    fetch(0);
     float m = one.x;
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
@@ -507,32 +515,27 @@ __global__ __launch_bounds__(256) void terna_tree_merge_kernel(const float* __re
     float l = one.y * weight;
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
-    float sum[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-    for (int s0 = 0; s0 < share.count; s0 += AHEAD) {
-        float y[AHEAD][E];
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0;;) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const float* const from = x + static_cast<size_t>(min(s0 + i, share.count - 1)) * rows * D;
-            if constexpr (E == 2) {
-                const float2 two = *reinterpret_cast<const float2*>(from);
-                y[i][0] = two.x, y[i][1] = two.y;
-            } else {
-                y[i][0] = *from;
-            }
-        }
+            const int part = s0 + i * BESIDE + which;
+            const float w = __shfl(weight, min(part, share.count - 1));
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const float w = __shfl(weight, min(s0 + i, share.count - 1));
-#pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += s0 + i < share.count ? y[i][e] * w : 0.0f;
+            for (int e = 0; e < 4; ++e) sum[e] += part < share.count ? y[i][e] * w : 0.0f;
         }
+        s0 += AHEAD * BESIDE;
+        if (s0 >= share.count) break;
+        fetch(s0);
     }
+#pragma unroll
+    for (int off = LANES; off < 64; off *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], off);
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* const to = out + static_cast<size_t>(at) * D + E * lane;
-    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(to) = l == 0.0f ? 0u : pack_bf16x2(sum[0] * inverse, sum[1] * inverse);
-    else *to = l == 0.0f ? static_cast<uint16_t>(0) : float_to_bf16_bits(sum[0] * inverse);
+    if (which != 0) return;
+    *reinterpret_cast<u32x2*>(out + static_cast<size_t>(at) * D + 4 * piece) =
+        l == 0.0f ? u32x2{0u, 0u} : u32x2{pack_bf16x2(sum[0] * inverse, sum[1] * inverse), pack_bf16x2(sum[2] * inverse, sum[3] * inverse)};
 }
 
 }  // namespace terna
