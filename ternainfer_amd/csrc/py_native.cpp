@@ -183,6 +183,21 @@ at::Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& li
         return at::Tensor(at::detail::empty_generic(shape, device_allocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
     return at::empty(shape, at::TensorOptions(type).device(like.device()));
 }
+// Several int64 results in one allocation (a tensor more is 0.15 us, an allocation 0.6).
+struct Longs {
+    at::Tensor all;
+    int64_t used = 0;
+
+    Longs(int64_t count, const at::Tensor& like) : all(make({count}, at::kLong, like)) {}
+    at::Tensor take(at::IntArrayRef shape)
+    {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+        t.unsafeGetTensorImpl()->set_storage_offset(used);
+        used += t.numel();
+        return t;
+    }
+};
 terna_stream stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
 // int8 rows and their bf16 scales, for the length of one call: (rows [m][k], scales [m]) on the current device
@@ -1243,7 +1258,8 @@ TERNA_FUNCTION(draft_tree, 1)
     on_device_of(guard, parents);
     Unlocked unlocked;
     const at::Tensor rows = parents.contiguous();
-    at::Tensor mask = make({b, t, (t + 63) / 64}, at::kLong, parents), depth = make({b, t}, at::kLong, parents);
+    Longs results(b * t * ((t + 63) / 64 + 1), parents);
+    at::Tensor mask = results.take({b, t, (t + 63) / 64}), depth = results.take({b, t});
     const int rc = depth.numel() == 0 ? 0 : lib.ternaspmm_draft_tree(longs(rows), mutable_longs(mask), mutable_longs(depth), b, t, stream());
     unlocked.end();
     if (rc != 0) refuse("%s: the library refused the launch", who);
@@ -1312,15 +1328,16 @@ TERNA_FUNCTION(tree_accept, 3)
     Guard guard;
     on_device_of(guard, logits);
     Unlocked unlocked;
-    at::Tensor path = make({b, t}, at::kLong, logits), count = make({b}, at::kLong, logits), next = make({b}, at::kLong, logits);
+    const bool fp32 = logits.scalar_type() == at::kFloat;
+    const int64_t work = b == 0 ? 0 : std::max(0ll, static_cast<long long>(lib.ternaspmm_tree_accept_workspace_bytes(b, t, v, fp32)));      // (no more than 2048 parts, or one a node)
+    Longs results(b * (t + 2) + work / 8, logits);
+    at::Tensor path = results.take({b, t}), count = results.take({b}), next = results.take({b});
     int rc = 0;
     if (b > 0) {
-        const bool fp32 = logits.scalar_type() == at::kFloat;
         const at::Tensor rows = (v == 1 || logits.stride(2) == 1) && (b == 1 || t == 1 || logits.stride(0) == t * logits.stride(1)) ? logits : logits.contiguous();
         const at::Tensor drafted = tokens.contiguous(), of = parents.contiguous();
-        const c10::DataPtr work = device_allocator()->allocate(std::max(0ll, static_cast<long long>(lib.ternaspmm_tree_accept_workspace_bytes(b, t, v, fp32))));
         rc = lib.ternaspmm_tree_accept(rows.const_data_ptr(), t == 1 ? rows.stride(0) : rows.stride(1), fp32, longs(drafted), longs(of), mutable_longs(path), mutable_longs(count),
-                                       mutable_longs(next), work.get(), b, t, v, stream());
+                                       mutable_longs(next), work == 0 ? nullptr : results.all.mutable_data_ptr<int64_t>() + results.used, b, t, v, stream());
     }
     unlocked.end();
     if (rc != 0) refuse("%s: the library refused the launch", who);
@@ -1350,10 +1367,15 @@ TERNA_FUNCTION(cache_move, 4)
                                          static_cast<int>(c.size(2)), static_cast<int>(c.size(3) * size)};
     }
     caches.erase(std::remove_if(caches.begin(), caches.end(), [](const ternaspmm_cache_rows& c) { return c.rows == nullptr; }), caches.end());
-    std::vector<const void*> sorted;
-    for (const ternaspmm_cache_rows& c : caches) sorted.push_back(c.rows);
-    std::sort(sorted.begin(), sorted.end());
-    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) refuse("%s: a cache is given twice", who);
+    size_t places = 16;
+    while (places < 4 * caches.size()) places *= 2;
+    std::vector<const void*> seen(places, nullptr);
+    for (const ternaspmm_cache_rows& c : caches) {
+        size_t at = (reinterpret_cast<uintptr_t>(c.rows) * 0x9e3779b97f4a7c15ull >> 32) & (places - 1);
+        for (; seen[at] != nullptr; at = (at + 1) & (places - 1))
+            if (seen[at] == c.rows) refuse("%s: a cache is given twice", who);
+        seen[at] = c.rows;
+    }
     Guard guard;
     on_device_of(guard, path);
     Unlocked unlocked;

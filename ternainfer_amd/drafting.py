@@ -54,4 +54,4 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
 def cache_move(caches: Sequence[torch.Tensor], start: torch.Tensor, path: torch.Tensor, count: torch.Tensor) -> None:
     """Slot start[b] + path[b, i] -> slot start[b] + i for i < count[b], in place and in every cache of the list: tensors [B, heads, S, D] of any type (bf16 keys and
     values, codes and scales of a `Kv4Cache`), rows contiguous, that share no element.  A path ascends (`tree_accept`'s does); rows outside the cache stay."""
-    _lib.native().cache_move(list(caches), start, path, count)
+    _lib.native().cache_move(caches if isinstance(caches, (list, tuple)) else list(caches), start, path, count)
