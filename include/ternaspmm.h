@@ -750,14 +750,14 @@ int ternaspmm_draft_tree(const long long* parents, long long* mask, long long* d
  * address and stride a multiple of 16 bytes, a slot's stride below 2^24; D 64 or 128, S <= 2^25, B * T * H <= 2^28.  Node j's key and value lie in slot start[b] + j.  Row (b, i) of out bf16 [B * T][H * D]:
  * the softmax of scale * q . k over the slots 0 .. start[b] - 1 and those of the nodes in its mask -- int64 [T][(T + 63) / 64], with per_sequence
  * [B][T][...] -- times the values.  A row without a bit, and a sequence with start[b] < 0: zeros.  A row that sees a slot from S on, or start[b] > S: NaN.
- * A slot that a row does not see does not reach it, whatever it holds.  scale is finite.
+ * A slot that a row does not see does not reach it, whatever it holds.  scale * log2(e) is finite in fp32.
  * workspace: ternaspmm_tree_attention_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for long caches of few rows. */
 long long ternaspmm_tree_attention_workspace_bytes(int B, int T, int H, int KV, int D, int S);
 int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, const terna_bf16* k, const long long* k_strides, const terna_bf16* v, const long long* v_strides,
                              const long long* start, const long long* mask, int per_sequence, terna_bf16* out, void* workspace, int B, int T, int H, int KV, int D, int S,
                              float scale, terna_stream stream);
 /* The branch that greedy decoding takes: logits (bf16, or fp32; rows `row` elements apart) of the nodes b * T + i, tokens int64 [B][T].  From node 0 on,
- * while a child of the node -- the first of them -- carries the token of the node's largest logit (equal ones: the lowest; NaN never wins), it is next.
+ * while a child of the node -- the first of them -- carries the token of the node's largest logit (equal ones: the lowest; NaN never wins; 0 where none is above -inf), it is next.
  * path int64 [B][T]: those nodes, then -1; count int64 [B]; next int64 [B]: the token behind the last.  Where node 0 is no root, count 0 and next -1.
  * V <= 2^19.  workspace: ternaspmm_tree_accept_workspace_bytes, 8-byte aligned. */
 long long ternaspmm_tree_accept_workspace_bytes(int B, int T, int V, int fp32);

@@ -17,9 +17,10 @@
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
 // What bounds it: of few rows a sequence and many sequences the cache's bytes (64 sequences of one token over 8000 slots 229 us, 5.7 TB/s; 32 of 13 nodes over
-// 7500 119 us, 4.9), of many rows the steps -- 32 slots of 128 rows: 512 clocks of matrix instructions a wave, 420 of exponentials and the like, 24 LDS reads;
-// of two waves to a SIMD they hardly overlap: 0.64 us a step with one wave, 1.0 with two, 43 % of the rate that the matrix instructions alone would have -- and with little to
-// read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 7 for the second launch.
+// 7500 119 us, 4.9), of many rows the steps -- 64 slots of 128 rows in two groups: 1024 clocks of a SIMD's matrix instructions, as many of its vector
+// instructions, 128 KB of LDS reads; 0.85 us where nothing comes from memory, 1.23 where all does, of which two workgroups that share their slots need 0.9 for the
+// memory alone -- and with little to read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 5 for the
+// second launch.
 #pragma once
 
 #include "draft_tree_kernel.h"

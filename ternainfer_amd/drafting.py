@@ -46,7 +46,7 @@ class TreeAccepted(NamedTuple):
 
 def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor) -> TreeAccepted:
     """The branch that greedy decoding takes, from the nodes' logits [B, T, V] (bfloat16 or float32) and their tokens, int64 [B, T]: from node 0 on the
-    first child that carries the token of the node's largest logit (equal ones: the lowest, NaN never), while there is one.  Where node 0 is no root
+    first child that carries the token of the node's largest logit (equal ones: the lowest, NaN never; 0 where none is above -inf), while there is one.  Where node 0 is no root
     (parents[b, 0] other than -1) the sequence has no step: count 0, next -1."""
     return TreeAccepted(*_lib.native().tree_accept(logits, tokens, parents))
 
