@@ -22,7 +22,7 @@ bool tree_shape_ok(int B, int T, int H, int KV, int D, int S)
 {
     if (!tree_nodes_ok(B, T) || H < 1 || KV < 1 || H % KV != 0 || (D != 64 && D != 128) || S < 1 || S > 1 << 25 || H > 4096 || static_cast<long long>(B) * T * H > 1 << 28) return false;
     const TreePlan plan = tree_plan(B, T, H, KV, D, S);
-    return launch_fits(((static_cast<long long>(B) * KV * plan.splits + 7) / 8) * 8 * plan.tiles, 512);
+    return launch_fits(tree_blocks(static_cast<long long>(B) * KV * plan.splits, plan.tiles), 512);
 }
 // Strides in elements of rows that are read 16 bytes at a time.
 bool strides_ok(const long long* s, int n)
@@ -104,7 +104,7 @@ int ternaspmm_tree_attention(const terna_bf16* q, const long long* q_strides, co
     a.B = B, a.T = T, a.H = H, a.KV = KV, a.S = S, a.W = (T + 63) / 64, a.per_seq = per_sequence != 0;
     a.parts = workspace && plan.splits > 1 ? B * plan.splits : 0, a.tiles = plan.tiles;
     a.scale = scale * static_cast<float>(M_LOG2E);
-    const long long grid = ((static_cast<long long>(a.parts == 0 ? B : a.parts) * KV + 7) / 8) * 8 * plan.tiles;
+    const long long grid = tree_blocks(static_cast<long long>(a.parts == 0 ? B : a.parts) * KV, plan.tiles);
     if (D == 128) launch_tree_attention<128>(a, plan, grid, static_cast<hipStream_t>(stream));
     else launch_tree_attention<64>(a, plan, grid, static_cast<hipStream_t>(stream));
     const hipError_t e = hipGetLastError();

@@ -160,11 +160,10 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     __shared__ float2 stat[Shape::kWaves][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wave / RW, rw = wave % RW, qi = lane & 31, half = lane >> 5;
-    // Workgroups go to the XCDs round robin: the row tiles of one part of a kv head -- which read the same slots -- eight apart, on one XCD.
-    const int G = a.H / a.KV, units = (a.parts == 0 ? a.B : a.parts) * a.KV;
-    const int block = blockIdx.x / (8 * a.tiles), within = blockIdx.x - block * (8 * a.tiles);
-    const int unit = 8 * block + (within & 7), tile = within >> 3;
-    if (unit >= units) return;
+    const int G = a.H / a.KV;
+    const TreePlace place_of = tree_place(blockIdx.x, (a.parts == 0 ? a.B : a.parts) * a.KV, a.tiles);
+    if (place_of.unit < 0) return;
+    const int unit = place_of.unit, tile = place_of.tile;
     const int kvh = unit % a.KV;
     const TreePart part = tree_part(a, unit / a.KV);
     if (part.b < 0) return;

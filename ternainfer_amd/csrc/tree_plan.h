@@ -17,9 +17,9 @@ struct TreePlan {
 };
 // The groups and the parts by the time they take, us: steps of a workgroup and what surrounds them, in rounds of the workgroups that there is room for, or the
 // cache's bytes -- at 5.8 TB/s, less where workgroups are fewer than the CUs or do not fill their last round --, and the launch that joins the parts, whose
-// numerators are written and read at 5.4 to 5.9.  Fitted to 250 measured shapes and numbers of parts of up to 64 rows (an error of 12 %) and 750 of more (13 %; the
-// plan chosen by it took 1.7 % longer than the best one in the mean of 31 shapes, 23 % at the worst).  128 rows in two groups are a workgroup of eight waves, one to a CU, with half
-// the numerators that two workgroups of four have: 240 rows over 32768 slots 40.6 us, with one group 45.0; where nothing is split and workgroups are many,
+// numerators are written and read at 5.4 to 5.9.  Fitted to 250 measured shapes and numbers of parts of up to 64 rows (an error of 12 %) and 750 of more (16 % over 1100; the
+// plan chosen by it took 1.7 % longer than the best one in the mean of 62 shapes, 16 % at the worst).  128 rows in two groups are a workgroup of eight waves, one to a CU, with half
+// the numerators that two workgroups of four have: 240 rows over 32768 slots 41 us, with one group 45; where nothing is split and workgroups are many,
 // those of one group start and end while others compute: 32 sequences of 256 rows over 2048 slots 81 us, with two groups 91.
 inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
 {
@@ -53,5 +53,21 @@ inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
             if (const float t = time(groups, n); t < best) best = t, p.groups = groups, p.splits = static_cast<int>(n);
     return p;
 }
+
+// Where a workgroup works: on which part of a kv head (unit; -1: nowhere), on which of its row tiles.  Workgroups go to the XCDs round robin: the tiles of a unit, which
+// read the same slots, are on one XCD, eight units on eight, and those of the last units, fewer than eight, on all in equal shares (20 units of 12 tiles: 36 on four of
+// the XCDs and 24 on the others 58 us, 30 on each 39).
+struct TreePlace {
+    int unit, tile;
+};
+constexpr TreePlace tree_place(int block, int units, int tiles)
+{
+    const int xcd = block & 7, at = block >> 3, whole = (units >> 3) * tiles, others = (units & 7) * tiles, each = (others + 7) >> 3;
+    const int index = at < whole ? at : xcd * each + at - whole;           // of a tile among those of its kind
+    if (at >= whole && (at - whole >= each || index >= others)) return TreePlace{-1, 0};
+    const int of = index / tiles;
+    return TreePlace{at < whole ? 8 * of + xcd : (units & ~7) + of, index - of * tiles};
+}
+constexpr long long tree_blocks(long long units, int tiles) { return 8 * (units / 8 * tiles + (units % 8 * tiles + 7) / 8); }
 
 }  // namespace terna

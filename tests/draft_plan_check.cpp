@@ -1,5 +1,6 @@
 // The plans of the tree attention and of the 8-bit product: their workgroups cover every row, their parts fit the launches that join them and hold something.
 #include <cstdio>
+#include <vector>
 
 #include "../ternainfer_amd/csrc/int8_plan.h"
 #include "../ternainfer_amd/csrc/tree_plan.h"
@@ -28,6 +29,16 @@ int main()
                                 ++wrong;
                             }
                         }
+    // every row tile of every unit is some workgroup's, and one's alone
+    for (int units = 1; units <= 300; units += units < 40 ? 1 : 13)
+        for (int tiles : {1, 2, 3, 5, 7, 12, 16, 64}) {
+            std::vector<int> taken(units * tiles, 0);
+            for (long long block = 0; block < tree_blocks(units, tiles); ++block) {
+                const TreePlace p = tree_place(static_cast<int>(block), units, tiles);
+                if (p.unit >= 0 && (p.unit >= units || p.tile < 0 || p.tile >= tiles || taken[p.unit * tiles + p.tile]++)) ++wrong;
+            }
+            for (int x : taken) wrong += x != 1;
+        }
     int reached[kInt8TileKinds] = {}, joined = 0;
     for (int M : {1, 2, 16, 17, 32, 33, 60, 64, 65, 128, 200, 333, 512, 1000, 2048, 4096, 8192, 100000})
         for (int N : {1, 16, 100, 254, 1000, 2501, 2560, 3840, 13824, 50021, 128256})
