@@ -1,8 +1,11 @@
 """ternainfer_amd/int8_linear.py against the definition: integers and sums exactly, the three fp32 operations behind them too."""
+import ctypes
+
 import pytest
 import torch
 
 import ternainfer_amd as T
+from ternainfer_amd import _lib
 from tests import _drafting as P
 
 pytestmark = pytest.mark.gpu
@@ -87,6 +90,22 @@ def test_product(m, n, k):
         got = T.int8_linear(rows, weight, dtype)
         assert got.dtype == dtype and got.shape == (m, n) and got.is_contiguous()
         assert torch.equal(got, P.linear(x, xs, w, ws, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(3, n) for n in (*range(1, 20), 127, 129, 130, 255, 258, 260)] + [(1, 50021), (33, 60001), (64, 50022), (130, 13825), (512, 13826), (500, 6145), (4096, 2563), (2049, 4100), (1500, 20001)])
+def test_results_of_rows_of_every_width(dtype, m, n):
+    """Every element, and nothing in front of the results or behind them."""
+    _say("width", dtype, m, n)
+    k, size = 64, 2 if dtype == torch.bfloat16 else 4
+    x, w, xs, ws = _int8((m, k), 14), _int8((n, k), 15), _scales(m, 16), _scales(n, 17)
+    rows, weight, lib = T.int8_rows(x, xs), T.int8_rows(w, ws), _lib.load()
+    room = torch.full((16 // size + m * n + 1024,), 7.0, dtype=dtype, device="cuda")
+    p = lambda t, by=0: ctypes.c_void_p(t.data_ptr() + by)
+    assert lib.ternaspmm_int8_linear(p(rows.packed), p(rows.scale), p(weight.packed), p(weight.scale), p(room, 16), int(dtype == torch.float32), None, m, n, k,
+                                     ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    got = room[16 // size:16 // size + m * n].view(m, n)
+    assert torch.equal(got, P.linear(x, xs, w, ws, dtype)) and (room[:16 // size] == 7).all() and (room[16 // size + m * n:] == 7).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
