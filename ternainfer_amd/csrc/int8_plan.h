@@ -9,8 +9,8 @@ namespace terna {
 constexpr int int8_k_blocks(int K) { return 2 * ((K + 127) / 128); }
 
 // Tiles that a workgroup computes, features x rows; which of them the kernel is instantiated for is the launch's list (abi_int8.hip), in this order.
-// Two workgroups share a CU.  Times in us, fitted to 400 measured products (an error of 12 %; of 45 shapes the choice was the fastest for 41, and 1.2 times
-// it at the worst): of a block of 64 columns of a workgroup alone on its CU and of one beside another, and of what surrounds them.
+// Two workgroups share a CU.  Times in us, fitted to 400 measured products (an error of 12 %; of 60 shapes the choice took 8 % longer than the fastest at
+// the worst): of a block of 64 columns of a workgroup alone on its CU and of one beside another, and of what surrounds them.
 struct Int8TileTime {
     int features, rows;
     float alone, beside, around;

@@ -748,7 +748,7 @@ class Transformer:
 
     def quantise_head(self, on: bool = True) -> None:
         """The projection to the vocabulary in 8 bits, a scale for every token of it (`int8_linear`), or, with `on` False, in bf16 again: half the bytes of what a step
-        reads most of (one row of the 128256 x 2560 shape 115 -> 60 us; 60 rows by a bf16 library product 173 -> 70).  Logits then differ by the rounding of weights and
+        reads most of (one row of the 128256 x 2560 shape 118 -> 58 us; 60 rows, in bf16 by a library's product, 147 -> 70).  Logits then differ by the rounding of weights and
         rows to 8 bits; the embedding itself stays as it is.  To be called again where the embedding is changed."""
         self.head8 = quantise_rows(self.tok_embeddings) if on else None
 
