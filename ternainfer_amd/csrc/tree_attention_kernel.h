@@ -10,7 +10,7 @@
 //     and many leave few numerators to join.  The groups' are joined in LDS at the end, the splits' by a second launch (which groups, how many splits: tree_plan.h).
 //   * Keys and values go global -> LDS directly, ST - 1 steps ahead; 16-byte pieces are XOR-swizzled on the way, so that neither the keys' 16-byte operand reads
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
-//   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 16 bits of them count, and the second product's extra instructions are hidden
+//   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 15 bits of them count, and the second product's extra instructions are hidden
 //     there by the cache.  With more rows the kernel is bound by its instructions and they are one bf16, their sum taken of the rounded ones, so that rounding
 //     leaves the weights a sum of one: 60 nodes of 4 heads over 32768 slots 42 us, with two 48; largest error of values of unit variance 2.1e-3, with two 1.7e-3.
 //     The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own.
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     active = active && r < rows && part.start >= 0;
     outside = outside && active;
     const bool needed = __syncthreads_or(active);
-    const int steps = needed ? all_steps : 0;
+    const int steps = !needed ? 0 : RW == 1 ? max(end - begin - group + KW - 1, 0) / KW : all_steps;      // (groups that wait for each other make as many)
 
     // a negative scale's sign, and a scale of zero (0 * -inf would unmask a slot), go into the queries
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
@@ -317,8 +317,8 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
         return tree_max3(tree_max3(tops[0], tops[1], s[14]), s[15], s[15]);
     };
     float l_run = 0.0f, m_run = -INFINITY;
-    // steps whose tiles lie in front of the tree, all of them
-    const int plain = needed ? max(min(start / kTreeTile, end) - begin, 0) / KW : 0;
+    // this group's steps whose tiles lie in front of the tree
+    const int plain = needed ? max(min(start / kTreeTile, end) - begin - group + KW - 1, 0) / KW : 0;
     int at = 0;                                                            // place in the ring
     auto take = [&](int step, auto last_tiles, auto place) __attribute__((always_inline)) {
         constexpr bool LAST = decltype(last_tiles)::value;                 // may have slots of the tree, or behind the end
@@ -356,18 +356,22 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
         u32x4 high[2], low[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float p[8], rounded[8];
+            float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[8 * i + e], scale, shift));
-            high[i] = pack_bf16x8(p);
-            unpack_bf16x8(high[i], rounded);
+            if constexpr (TWO) {
+                // high: the upper 16 bits as they are; low: the rest and 2^-20 of the whole, so that it is positive and an infinite value stays one in both products
+                float rest[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sum[e & 1] += TWO ? p[e] : 0.0f;
-                rounded[e] = p[e] - rounded[e];
-            }
-            if constexpr (TWO) low[i] = pack_bf16x8(rounded);
-            else {
+                for (int e = 0; e < 8; ++e) {
+                    sum[e & 1] += p[e];
+                    rest[e] = __fmaf_rn(p[e], 1.0f + 0x1p-20f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) high[i][e] = __builtin_amdgcn_perm(__float_as_uint(p[2 * e + 1]), __float_as_uint(p[2 * e]), 0x07060302u);
+                low[i] = pack_bf16x8(rest);
+            } else {
+                high[i] = pack_bf16x8(p);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e & 1] = tree_sum2(high[i][e], sum[e & 1]);
             }

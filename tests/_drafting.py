@@ -62,7 +62,7 @@ def attention(q, k, v, start, mask, scale):
     """q bf16 [B, H, T, D], k and v bf16 [B, KV, S, D], start [B], mask [B, T, W] -> (out float64 [B, T, H, D], tolerance).  The tolerance: the output's rounding, and
     (2 ds + rounding + n 2^-23) sum p |v|, where ds = (D + 4) 2^-24 |scale| max sum |q| |k| bounds a score's error (a sum of D products in fp32), in numerator and
     denominator, n 2^-23 the sums over n slots, their parts and the rescalings, and `rounding` the exponential's 2^-20 with the probabilities' own, in numerator and
-    denominator: in two bf16 2^-16 each up to 64 query rows a kv head (2^-14 covers both and the exponential), one bf16 beyond: 2 * 2^-8.  Below the normal numbers nothing is
+    denominator: in two bf16 2^-15 in the numerator up to 64 query rows a kv head (2^-14 covers it and the exponential), one bf16 beyond: 2 * 2^-8.  Below the normal numbers nothing is
     promised: a term under 2^-126 of the sum, which is 1 at least, may be lost, by itself, in its low half and in its part's weight: n 2^-124 max |v|."""
     b, h, t, d = q.shape
     kv, slots = k.shape[1:3]

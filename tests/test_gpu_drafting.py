@@ -125,7 +125,8 @@ def test_what_a_node_does_not_see_does_not_reach_it(t, h, kv, slots):
             assert torch.equal(got[node], want[node]), (fill, node)
 
 
-@pytest.mark.parametrize("t,h,kv,start,slots", [(5, 4, 2, 70, 100), (5, 4, 2, 0, 100), (70, 8, 1, 100, 200), (9, 20, 5, 7000, 7100), (40, 1200, 300, 190, 260)])
+@pytest.mark.parametrize("t,h,kv,start,slots", [(5, 4, 2, 70, 100), (5, 4, 2, 0, 100), (70, 8, 1, 100, 200), (9, 20, 5, 7000, 7100), (40, 1200, 300, 190, 260), (5, 4, 2, 1000, 1010), (9, 20, 5, 1000, 1010),
+                                                   (40, 20, 5, 2000, 2050), (5, 20, 5, 9000, 9010)])
 def test_values_that_are_not_finite_where_they_are_seen(t, h, kv, start, slots):
     """Infinities and NaN among the seen slots -- of the text and of the tree -- come out where the definition has them."""
     _say("not finite", t, h, kv, start, slots)
