@@ -10,6 +10,7 @@
 //     and many leave few numerators to join.  The groups' are joined in LDS at the end, the splits' by a second launch (which groups, how many splits: tree_plan.h).
 //   * Keys and values go global -> LDS directly, ST - 1 steps ahead; 16-byte pieces are XOR-swizzled on the way, so that neither the keys' 16-byte operand reads
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
+//     With 128 rows a workgroup the next step's keys are read ahead of this one's exponentials (800 rows over 8300 slots 65 us, so 63.6).
 //   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 15 bits of them count, and the second product's extra instructions are hidden
 //     there by the cache.  With more rows the kernel is bound by its instructions and they are one bf16, their sum taken of the rounded ones, so that rounding
 //     leaves the weights a sum of one: 60 nodes of 4 heads over 32768 slots 42 us, with two 48; largest error of values of unit variance 2.1e-3, with two 1.7e-3.
@@ -320,6 +321,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     // this group's steps whose tiles lie in front of the tree
     const int plain = needed ? max(min(start / kTreeTile, end) - begin - group + KW - 1, 0) / KW : 0;
     int at = 0;                                                            // place in the ring
+    bf16x8 key[KS];
     auto take = [&](int step, auto last_tiles, auto place) __attribute__((always_inline)) {
         constexpr bool LAST = decltype(last_tiles)::value;                 // may have slots of the tree, or behind the end
         constexpr int PLACE = decltype(place)::value;                      // known: offsets that instructions carry; -1: `at`
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
             load(step + ST - 1, behind);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * LOADS) : "memory");
         } else {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * LOADS) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RW == 4 ? ST - 3 : ST - 2) * LOADS) : "memory");
             load(step + ST - 1, behind);
         }
         const uint8_t *const keys = ring + here * (2 * TILE), *const vals = keys + TILE;
@@ -339,7 +341,12 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_operand(keys, ks), __builtin_bit_cast(bf16x8, q[ks]), s, 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(RW == 4 ? key[ks] : key_operand(keys, ks), __builtin_bit_cast(bf16x8, q[ks]), s, 0, 0, 0);
+        if constexpr (RW == 4) {
+            const uint8_t* const ahead = ring + (PLACE < 0 ? at : (PLACE + 1) % ST) * (2 * TILE);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) key[ks] = key_operand(ahead, ks);
+        }
         if constexpr (LAST) unseen(s, slot_of(step));
         const float top = tree_halves<true>(largest(s)) * scale;
         const bool more = top > m_run + kTreeGrowth;                // a row by its own growth alone: its bits do not hang on the rows beside it
@@ -394,6 +401,13 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     if (steps > 0) {
 #pragma unroll
         for (int i = 1; i < ST - 1; ++i) load(i, i);
+    }
+    if constexpr (RW == 4) {
+        if (steps > 0) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * LOADS) : "memory");
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) key[ks] = key_operand(ring, ks);
+        }
     }
     using Anywhere = std::integral_constant<int, -1>;
     int step = 0;
