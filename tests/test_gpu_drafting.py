@@ -259,6 +259,48 @@ def test_a_cache_of_more_than_four_gigabytes():
         assert ((got[node].double() - want).abs() <= tol).all(), node
 
 
+@pytest.mark.parametrize("t,h", [(5, 2), (11, 4), (40, 4)])
+def test_slots_far_apart(t, h):
+    """Slots 2^23 elements apart: 32 of them are a distance of 2^29 bytes."""
+    slots, d, start = 40 + t, 128, 39
+    _say("far apart", t, h)
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("3 GB of keys and values")
+    k, v = (torch.zeros((1, 1, slots * 65536, d), dtype=torch.bfloat16, device="cuda")[:, :, ::65536] for _ in range(2))
+    k.copy_(_randn(k.shape, 114))
+    v.copy_(_randn(v.shape, 115))
+    assert k.stride(2) == 1 << 23
+    _attend(_randn((1, h, t, d), 116), k, v, torch.tensor([start], device="cuda"), T.draft_tree(P.random_parents(1, t, 117).cuda()).mask)
+
+
+def test_many_sequences():
+    """As many as a call takes, of the smallest trees; more are refused."""
+    b = 65535
+    _say("sequences", b)
+    parents = torch.tensor([[-1, 0], [-1, -1], [-2, 0]], device="cuda").repeat(21845, 1)
+    tree = T.draft_tree(parents)
+    mask, depth = P.tree(parents[:3].cpu())
+    assert torch.equal(tree.mask.cpu(), mask.repeat(21845, 1, 1)) and torch.equal(tree.depth.cpu(), depth.repeat(21845, 1))
+    q, k, v = _randn((b, 1, 2, 64), 118), _randn((b, 1, 5, 64), 119), _randn((b, 1, 5, 64), 120)
+    start = torch.arange(b, device="cuda") % 5 - 1                                        # none; 0 .. 3, of which the last has no slot for the second node
+    got = T.tree_attention(q, k, v, start, tree.mask).view(b, 2, 1, 64)
+    for at in (slice(0, 60), slice(32700, 32760), slice(b - 60, b)):
+        want, tol = P.attention(q[at], k[at], v[at], start[at], tree.mask[at], 64 ** -0.5)
+        assert same_or_near(got[at], want, tol) <= 0
+    logits, tokens = _randn((b, 2, 3), 121), torch.ones((b, 2), dtype=torch.int64, device="cuda")
+    accepted = T.tree_accept(logits, tokens, parents)
+    for at in (slice(0, 60), slice(b - 60, b)):
+        assert [x[at].tolist() for x in accepted] == P.accept(logits[at], tokens[at], parents[at])
+    cache = v.clone()
+    T.cache_move([cache], torch.ones(b, dtype=torch.int64, device="cuda"), torch.tensor([[0, 3]], device="cuda").expand(b, 2), torch.full((b,), 2, device="cuda"))
+    v[:, :, 2] = v[:, :, 4]
+    assert torch.equal(cache, v)
+    more = torch.full((b + 1, 1), -1, device="cuda")
+    for call in (lambda: T.draft_tree(more), lambda: T.tree_accept(torch.zeros((b + 1, 1, 1), device="cuda"), more, more), lambda: T.cache_move([], more[:, 0], more, more[:, 0])):
+        with pytest.raises(ValueError, match="65535"):
+            call()
+
+
 # ---- acceptance --------------------------------------------------------------------------------------------------------------------
 
 

@@ -120,6 +120,37 @@ def test_product_of_rows_that_are_quantised_in_the_call(dtype, m, n, k):
     assert torch.equal(T.int8_linear(torch.cat([x, x], 1)[:, :k], weight, torch.float32), got)
 
 
+def test_more_than_two_to_the_31_results():
+    m, n, k = 17000, 128257, 16
+    _say("results", m, n, k)
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("4.4 GB of results")
+    x, w, xs, ws = _int8((m, k), 60), _int8((n, k), 61), _scales(m, 62), _scales(n, 63)
+    got = T.int8_linear(T.int8_rows(x, xs), T.int8_rows(w, ws))
+    for at in (slice(0, 40), slice(16730, 16760), slice(m - 40, m)):                      # (row 16744 holds the 2^31st)
+        assert torch.equal(got[at], P.linear(x[at], xs[at], w, ws, torch.bfloat16))
+
+
+def test_many_rows():
+    """Rows whose place is behind 2^31 bytes, in the tensor and packed."""
+    r, k = 1 << 20, 2100
+    _say("rows", r, k)
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("7 GB of rows")
+    x = torch.zeros((r, k), dtype=torch.bfloat16, device="cuda")
+    for at in (slice(0, 40), slice(r - 70, r)):
+        x[at] = _randn((at.stop - at.start, k), 64)
+    got = T.quantise_rows(x)
+    band = 2 * ((k + 127) // 128) * 1024
+    for first in (0, (r - 64) // 16):
+        q, scale = P.quantise(x[16 * first:16 * first + 32])
+        assert torch.equal(P.unpack(got.packed[first * band:(first + 2) * band], 32, k), q) and torch.equal(got.scale[16 * first:16 * first + 32], scale)
+    ints = torch.zeros((r, k), dtype=torch.int8, device="cuda")
+    ints[-33:] = _int8((33, k), 65)
+    packed = T.int8_rows(ints, got.scale).packed
+    assert torch.equal(P.unpack(packed[-3 * band:], 48, k), ints[-48:])
+
+
 def test_the_largest_sums():
     """Every product 2^14, at the most columns: 2147221504, below 2^31."""
     k = 131056
