@@ -32,21 +32,21 @@ bool strides_ok(const long long* s, int n)
     return true;
 }
 
-template <int D, int RW, int KW, int ST, bool TWO, int PER_SIMD>
+template <int D, int RW, int KW, int ST, int PER_SIMD>
 void launch_tree(const TreeAttention& a, long long grid, hipStream_t st)
 {
     using Shape = TreeShape<D, RW, KW, ST>;
-    auto kernel = terna_tree_attention_kernel<D, RW, KW, ST, TWO, PER_SIMD>;
+    auto kernel = terna_tree_attention_kernel<D, RW, KW, ST, PER_SIMD>;
     if (Shape::kBytes > kPlainLds - 4096) allow_dynamic_lds(kernel, Shape::kBytes, "hipFuncSetAttribute(tree attention)", __LINE__);
     launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(Shape::kThreads), Shape::kBytes, st, a);
 }
 template <int D>
 void launch_tree_attention(const TreeAttention& a, const TreePlan& plan, long long grid, hipStream_t st)
 {
-    if (plan.rows == 32) launch_tree<D, 1, 4, D == 128 ? 2 : 4, true, 1>(a, grid, st);
-    else if (plan.rows == 64) launch_tree<D, 2, 2, D == 128 ? 2 : 4, true, 2>(a, grid, st);
-    else if (plan.groups == 1) launch_tree<D, 4, 1, 4, false, 2>(a, grid, st);
-    else launch_tree<D, 4, 2, 4, false, 2>(a, grid, st);
+    if (plan.rows == 32) launch_tree<D, 1, 4, D == 128 ? 2 : 4, 1>(a, grid, st);
+    else if (plan.rows == 64) launch_tree<D, 2, 2, D == 128 ? 2 : 4, 2>(a, grid, st);
+    else if (plan.groups == 1) launch_tree<D, 4, 1, 4, 2>(a, grid, st);
+    else launch_tree<D, 4, 2, 4, 2>(a, grid, st);
     if (a.parts != 0) {
         const int all = a.T * a.H;
         launch(terna_tree_merge_kernel<D>, dim3((a.B * all + 3) / 4), dim3(256), 0, st, a.partial, a.out, a.B, all, a.parts);

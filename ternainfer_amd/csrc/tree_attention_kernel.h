@@ -11,9 +11,8 @@
 //   * Keys and values go global -> LDS directly, ST - 1 steps ahead; 16-byte pieces are XOR-swizzled on the way, so that neither the keys' 16-byte operand reads
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
 //     With 128 rows a workgroup the next step's keys are read ahead of this one's exponentials (800 rows over 8300 slots 65 us, so 63.6).
-//   * Probabilities of workgroups of up to 64 rows are two bf16, high and low part: 15 bits of them count, and the second product's extra instructions are hidden
-//     there by the cache.  With more rows the kernel is bound by its instructions and they are one bf16, their sum taken of the rounded ones, so that rounding
-//     leaves the weights a sum of one: 60 nodes of 4 heads over 32768 slots 42 us, with two 48; largest error of values of unit variance 2.1e-3, with two 1.7e-3.
+//   * Probabilities are two bf16, high and low part: 15 bits of them count.  One bf16 is 2^-9 of every term, which shows where large values nearly cancel: two slots
+//     with half of the weight each and values of 200 and -200 came out 0.3 off.
 //     The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own.
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
@@ -44,13 +43,6 @@ struct TreeAttention {
     int B, T, H, KV, S, W, parts, tiles, per_seq;       // parts: of all sequences together, 0 where none is split
     float scale;                               // times log2(e)
 };
-
-// Two bf16 added to a sum
-__device__ __forceinline__ float tree_sum2(uint32_t both, float sum)
-{
-    typedef __bf16 two __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, both), __builtin_bit_cast(two, 0x3f803f80u), sum, false);
-}
 
 // A sequence's parts: the first of them, and how many.
 struct TreeShare {
@@ -150,7 +142,7 @@ __device__ __forceinline__ TreePart tree_part(const TreeAttention& a, int part)
     }
 }
 
-template <int D, int RW, int KW, int ST, bool TWO, int PER_SIMD>
+template <int D, int RW, int KW, int ST, int PER_SIMD>
 __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_kernel(TreeAttention a)
 {
     static_assert(ST == 2 || ST == 4);
@@ -366,22 +358,16 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[8 * i + e], scale, shift));
-            if constexpr (TWO) {
-                // high: the upper 16 bits as they are; low: the rest and 2^-20 of the whole, so that it is positive and an infinite value stays one in both products
-                float rest[8];
+            // high: the upper 16 bits as they are; low: the rest and 2^-20 of the whole, so that it is positive and an infinite value stays one in both products
+            float rest[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum[e & 1] += p[e];
-                    rest[e] = __fmaf_rn(p[e], 1.0f + 0x1p-20f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) high[i][e] = __builtin_amdgcn_perm(__float_as_uint(p[2 * e + 1]), __float_as_uint(p[2 * e]), 0x07060302u);
-                low[i] = pack_bf16x8(rest);
-            } else {
-                high[i] = pack_bf16x8(p);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e & 1] = tree_sum2(high[i][e], sum[e & 1]);
+            for (int e = 0; e < 8; ++e) {
+                sum[e & 1] += p[e];
+                rest[e] = __fmaf_rn(p[e], 1.0f + 0x1p-20f, -__uint_as_float(__float_as_uint(p[e]) & 0xffff0000u));
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) high[i][e] = __builtin_amdgcn_perm(__float_as_uint(p[2 * e + 1]), __float_as_uint(p[2 * e]), 0x07060302u);
+            low[i] = pack_bf16x8(rest);
         }
         l_run += sum[0] + sum[1];
 #pragma unroll
@@ -394,7 +380,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
             for (int dt = 0; dt < DT; ++dt) {
                 const bf16x8 y = __builtin_bit_cast(bf16x8, x[dt]);
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, __builtin_bit_cast(bf16x8, high[i]), o[dt], 0, 0, 0);
-                if constexpr (TWO) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, __builtin_bit_cast(bf16x8, low[i]), o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, __builtin_bit_cast(bf16x8, low[i]), o[dt], 0, 0, 0);
             }
         }
     };
