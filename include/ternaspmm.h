@@ -749,7 +749,8 @@ int ternaspmm_draft_tree(const long long* parents, long long* mask, long long* d
 /* Attention of the nodes: q, k and v bf16 with strides (elements) of [B][H][T][D] and [B][KV][S][D]'s first three dimensions, the last contiguous; every
  * address and stride a multiple of 16 bytes, a slot's stride below 2^24; D 64 or 128, S <= 2^25, B * T * H <= 2^28.  Node j's key and value lie in slot start[b] + j.  Row (b, i) of out bf16 [B * T][H * D]:
  * the softmax of scale * q . k over the slots 0 .. start[b] - 1 and those of the nodes in its mask -- int64 [T][(T + 63) / 64], with per_sequence
- * [B][T][...] -- times the values.  A row without a bit, and a sequence with start[b] < 0: zeros.  A row that sees a slot from S on, or start[b] > S: NaN.
+ * [B][T][...] -- times the values.  A row without a bit, and a sequence with start[b] < 0: zeros.  A row that sees a slot from S on, or start[b] > S: NaN;
+ * so one with scale * q . k above what fp32 holds.
  * A slot that a row does not see does not reach it, whatever it holds.  scale * log2(e) is finite in fp32.
  * workspace: ternaspmm_tree_attention_workspace_bytes (0 where none is used), 16-byte aligned; NULL: slower for long caches of few rows. */
 long long ternaspmm_tree_attention_workspace_bytes(int B, int T, int H, int KV, int D, int S);

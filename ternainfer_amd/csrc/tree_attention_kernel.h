@@ -408,6 +408,7 @@ __global__ __launch_bounds__(64 * RW * KW, PER_SIMD) void terna_tree_attention_k
     for (; step < plain; ++step) take(step, std::false_type{}, Anywhere{});
     for (; step < steps; ++step) take(step, std::true_type{}, Anywhere{});
     l_run = tree_halves<false>(l_run);
+    if (m_run == INFINITY) l_run = NAN;                                    // a score above what fp32 holds: NaN, not a row that sees nothing
     if (__any(taken_out)) {                                                // rare: they are added where they are seen
         const int from = max(min(start / kTreeTile, end) - KW, begin);     // (whatever tile it can have been; added twice, they are what they were)
         for (int k_tile = from; k_tile < end; ++k_tile) {

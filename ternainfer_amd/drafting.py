@@ -33,7 +33,8 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     """Attention of a tree's nodes q bf16 [B, H, T, D] over the cache bf16 [B, KV, S, D] (any strides of whole 16 bytes; D 64 or 128, S up to 2^25): bf16
     [B * T, H * D].  Sequence b's node i sees the slots 0 .. start[b] - 1 (int64 [B]) and slot start[b] + j of every node j in its mask (`draft_tree`'s,
     or int64 [T, W] for all sequences) -- and nothing of what any other slot holds.  A node without a bit (padding), and a sequence with a negative start, give
-    zeros; a node that sees a slot behind the cache gives NaN.  scale: D ** -0.5 by default."""
+    zeros; a node that sees a slot behind the cache, or has a score above what float32 holds,
+    gives NaN.  scale: D ** -0.5 by default."""
     return _lib.native().tree_attention(q, cache_k, cache_v, start, mask, scale)
 
 

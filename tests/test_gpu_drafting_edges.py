@@ -48,3 +48,16 @@ def test_values_that_nearly_cancel(d, b, t, h, kv, slots):
         some = slice(0, 2)
         want, tol = P.attention(q[some, heads], k[some], v[some], at[some], mask[some], d ** -0.5)
         assert same_or_near(got[some][:, :, heads], want, tol) <= 0
+
+
+@pytest.mark.parametrize("b,t,h,kv,slots", SHAPES)
+def test_scores_that_overflow(b, t, h, kv, slots):
+    """Scores whose product with the scale is beyond float32: NaN, as in elementary operations, whatever the layout of the rows -- not the zeros of a row that sees
+    nothing.  Rows with nothing to see stay zeros."""
+    _say("overflow", b, t, h, kv, slots)
+    start = slots - t - 3
+    q, k, v = _randn((b, h, t, 128), 10).abs(), _randn((b, kv, slots, 128), 11).abs(), _randn((b, kv, slots, 128), 12)
+    parents = P.random_parents(b, t, 13)
+    parents[:, -1] = -2
+    got = T.tree_attention(q, k, v, torch.full((b,), start, device="cuda"), T.draft_tree(parents.cuda()).mask, 2e38).view(b, t, h, 128)
+    assert got[:, :-1].isnan().all() and not got[:, -1].any()
