@@ -353,8 +353,8 @@ TERNA_FUNCTION(quant_input, 1)
     return pack(unlocked, std::move(q), std::move(s));
 }
 
-// (x int8 [M, K], s, packed, ws, ws_num, out_features, workspace | None)
-TERNA_FUNCTION(linear_packed, 7)
+// (x int8 [M, K], s, packed, ws, ws_num, out_features, workspace | None), the weights' scales by the rule of M (route 0) or the decode rule (2)
+PyObject* linear_packed_by(PyObject* const* a, int route)
 {
     const char* who = "TernaInfer_linear_packed";
     const at::Tensor &x = tensor(a[0]), &s = tensor(a[1]), &packed = tensor(a[2]), &ws = tensor(a[3]);
@@ -369,9 +369,11 @@ TERNA_FUNCTION(linear_packed, 7)
     const at::Tensor rows = x.contiguous(), scales = s.contiguous();
     at::Tensor out = make({m, n}, at::kBFloat16, x);
     lib.bitlinear_TernaSpMM_packed_ws(data<int8_t>(&rows), data(&packed), data<terna_bf16>(&out), data<terna_bf16>(&scales), data<terna_bf16>(&ws),
-                                      ws_num, m, n, k, 0, data(workspace), workspace != nullptr ? workspace->numel() : 0, stream());
+                                      ws_num, m, n, k, route, data(workspace), workspace != nullptr ? workspace->numel() : 0, stream());
     return wrap(std::move(out), unlocked);
 }
+TERNA_FUNCTION(linear_packed, 7) { return linear_packed_by(a, 0); }
+TERNA_FUNCTION(linear_packed_decode_rule, 7) { return linear_packed_by(a, 2); }
 
 // (x bf16 [M, K], packed, scale fp32, ws_num, out_features, workspace | None)
 TERNA_FUNCTION(linear_bf16_packed, 6)
@@ -1514,7 +1516,7 @@ TERNA_FUNCTION(init, 1)
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(init), METHOD(bit_linear), METHOD(bit_linear_bf16), METHOD(quant_input), METHOD(linear_packed),
+PyMethodDef methods[] = {METHOD(init), METHOD(bit_linear), METHOD(bit_linear_bf16), METHOD(quant_input), METHOD(linear_packed), METHOD(linear_packed_decode_rule),
                          METHOD(linear_bf16_packed), METHOD(rmsnorm_quant), METHOD(relu2_mul_rmsnorm_quant), METHOD(quant_from_stats),
                          METHOD(fused_linear), METHOD(fused_linear_own_stats), METHOD(prompt_attention), METHOD(decode_attention), METHOD(block),
                          METHOD(attention_merge_rmsnorm_quant), METHOD(step_attention_merge), METHOD(step_inputs), METHOD(prompt_inputs), METHOD(decode_step),

@@ -82,10 +82,12 @@ class TernaryLinear:
         self.act = act
         self.lib = _lib.load()
 
-    def quantised(self, xq: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
-        """int8 activations [M, K] + per-row scale bf16 [M] (as the fused prologue kernels write them)."""
+    def quantised(self, xq: torch.Tensor, s: torch.Tensor, decode_rule: bool = False) -> torch.Tensor:
+        """int8 activations [M, K] + per-row scale bf16 [M] (as the fused prologue kernels write them).  `decode_rule`: the weights' scales by the decode rule
+        also above 64 rows."""
         work = get_global_workspace(xq.device) if xq.shape[0] > 64 else None     # large M: room for split-K partial sums
-        return _lib.native().linear_packed(xq, s, self.packed, self.ws, self.ws_num, self.n, work)
+        native = _lib.native()
+        return (native.linear_packed_decode_rule if decode_rule else native.linear_packed)(xq, s, self.packed, self.ws, self.ws_num, self.n, work)
 
     def dense(self, x: torch.Tensor) -> torch.Tensor:
         """bf16 activations [M, K]."""
@@ -123,6 +125,7 @@ KERNEL_ATTENTION = object()    # in place of a mask: several new tokens, attenti
 class TreeNodes:                   # in place of a mask: the new tokens are the nodes of trees, attention by tree_attention
     start: torch.Tensor            # int64 [B]: slots in front of them
     mask: torch.Tensor             # int64 [B, T, words]: whom each sees among them
+    decode_rule: bool = False      # see Transformer.tree_step
 
 
 class Block:
@@ -177,7 +180,7 @@ class Block:
         blk.attn_sub_norm, blk.ffn_sub_norm = norm("attention.attn_sub_norm"), norm("feed_forward.ffn_sub_norm")
         return blk
 
-    def _norm_linear(self, lin, x, weight, residual=None, glu=False, name=None):
+    def _norm_linear(self, lin, x, weight, residual=None, glu=False, name=None, decode_rule=False):
         """[x + residual | relu(x1)^2 * x3] -> RMSNorm -> lin.  Returns (lin output, x + residual).  With `capture` set the
         quantised activations go through memory (norm kernel + linear, never the one-launch form) and are recorded."""
         eps = self.args.norm_eps
@@ -194,7 +197,7 @@ class Block:
                 if x.shape[0] <= 4 and cap is None:
                     return relu2_mul_rmsnorm_linear_packed(x, weight, eps, lin.packed, lin.ws, lin.ws_num, lin.n), None
                 xq, s = relu2_mul_rmsnorm_quant(x, weight, eps)
-                out = lin.quantised(xq, s)
+                out = lin.quantised(xq, s, decode_rule)
                 if cap is not None:
                     cap.append((name, xq, s, out))
                 return out, None
@@ -203,7 +206,7 @@ class Block:
             if x.shape[0] <= 8 and cap is None:   # decode step: prologue and linear in one launch where that is faster
                 return rmsnorm_linear_packed(x, weight, eps, lin.packed, lin.ws, lin.ws_num, lin.n, residual=residual)
             xq, s, h = rmsnorm_quant(x, weight, eps, residual=residual)
-            out = lin.quantised(xq, s)
+            out = lin.quantised(xq, s, decode_rule)
             if cap is not None:
                 cap.append((name, xq, s, out))
             return out, h
@@ -379,7 +382,8 @@ class Block:
                 self.ffn_sub_norm, wqkv.packed, wqkv.ws, wqkv.ws_num, wqkv.n, wo.packed, wo.ws, wo.ws_num, wo.n, w13.packed, w13.ws, w13.ws_num, w13.n,
                 w2.packed, w2.ws, w2.ws_num, w2.n,
                 self.gate_up_interleaved() if self.gate_linear_reads(x.shape[0]) else None)
-        qkv, x = self._norm_linear(self.wqkv, x, self.attention_norm, residual=pending, name="wqkv")
+        rule = isinstance(mask, TreeNodes) and mask.decode_rule
+        qkv, x = self._norm_linear(self.wqkv, x, self.attention_norm, residual=pending, name="wqkv", decode_rule=rule)
         rep = a.n_heads // a.n_kv_heads
         native = _lib.native()
         attend = (qkv, cos, sin, pos_idx, cache_k, cache_v, a.n_heads, a.head_dim, a.head_dim ** -0.5, int(a.rope_adjacent))
@@ -440,9 +444,9 @@ class Block:
         else:
             if self.capture is not None:
                 self.capture.append(("attention", None, None, o))
-            attn, _ = self._norm_linear(self.wo, o.contiguous(), self.attn_sub_norm, name="wo")
-        x13, x = self._norm_linear(self.w13, x, self.ffn_norm, residual=attn, name="w13")
-        ffn, _ = self._norm_linear(self.w2, x13, self.ffn_sub_norm, glu=True, name="w2")
+            attn, _ = self._norm_linear(self.wo, o.contiguous(), self.attn_sub_norm, name="wo", decode_rule=rule)
+        x13, x = self._norm_linear(self.w13, x, self.ffn_norm, residual=attn, name="w13", decode_rule=rule)
+        ffn, _ = self._norm_linear(self.w2, x13, self.ffn_sub_norm, glu=True, name="w2", decode_rule=rule)
         return x, ffn
 
 
@@ -772,10 +776,12 @@ class Transformer:
             return rmsnorm_quant(x, self.norm, a.norm_eps, residual=pending, quant=False)[0]     # (pending None: the stream has it)
         return rms_norm(x + pending, self.norm, a.norm_eps)
 
-    def tree_step(self, tokens: torch.Tensor, cache, start: torch.Tensor, tree: DraftTree) -> torch.Tensor:
+    def tree_step(self, tokens: torch.Tensor, cache, start: torch.Tensor, tree: DraftTree, decode_rule: bool = False) -> torch.Tensor:
         """The nodes of trees in one pass: tokens int64 [B, T], `start` int64 [B] cache slots in front of each tree, `tree` of `draft_tree`.  Node i's key and
         value go to slot start + i, at the position start + depth; every node sees the slots in front and its ancestors.  Returns logits [B, T, vocab].  (Padding writes
-        nothing, and its logits do not matter; so all of a sequence with a negative start.)  For the bf16 cache and the fused kernels."""
+        nothing, and its logits do not matter; so all of a sequence with a negative start.)  For the bf16 cache and the fused kernels.
+        Ternary linears of more than 64 rows, here B * T, follow the prefill rule of the weights' scales: where a scale's columns do not end at a multiple of 128, columns take
+        another scale than in a step of fewer rows.  `decode_rule`: they follow the decode rule whatever the number of rows, as a step of one token does."""
         a = self.args
         bsz, t = tokens.shape
         if isinstance(cache[0], Kv4Cache) or not self.layers[0].fused or not tokens.is_cuda or a.head_dim not in (64, 128) or a.dim % 8:
@@ -787,7 +793,7 @@ class Transformer:
         slots = torch.where(real, start[:, None] + torch.arange(t, device=tokens.device), -1)
         table = self.rope_tables(max_seq, tokens.device)
         x, cos, sin = prompt_inputs(tokens, (start[:, None] + tree.depth).clamp(0, max_seq - 1), self.tok_embeddings, table)
-        nodes, pending = TreeNodes(start, tree.mask), None
+        nodes, pending = TreeNodes(start, tree.mask, decode_rule), None
         for layer, (ck, cv) in zip(self.layers, cache):
             x, pending = layer.forward(x, pending, ck, cv, slots, cos, sin, nodes)
         return self.head(x, pending, bsz * t).view(bsz, t, -1)
@@ -920,12 +926,14 @@ def ngram_drafts(text: torch.Tensor, length: torch.Tensor, branches: int = 2, de
 
 
 @torch.inference_mode()
-def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, draft=ngram_drafts, prompt_lens=None, use_graph: Optional[bool] = None):
+def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, draft=ngram_drafts, prompt_lens=None, use_graph: Optional[bool] = None,
+                       decode_rule: bool = False):
     """Prefill `prompt` [B, P], then greedy decoding by drafted tokens: a step runs a tree of them through the model (`Transformer.tree_step`), keeps the branch that the
     model would have written itself and the token behind it (`tree_accept`), and puts its keys and values where the text ends (`cache_move`) -- one token a
     step at least.  `draft(text, length)` proposes: int64 (tokens, parents) [B, T] from the text so far, int64 [B, L], and its length [B]; node 0 is the text's last
     token, whatever they say there.  It is called once before the first step, for T, which later calls do not exceed.  Returns (tokens [B, gen_tokens], steps).  The
-    tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the two ways.  `prompt_lens` as there.
+    tokens are those of `greedy_decode` but where two logits of a step are as near as the roundings of the two ways -- with more than 64 rows in a step (B * T) only where
+    the weights' scales end at multiples of 128 columns, or with `decode_rule` (Transformer.tree_step), for up to 64 sequences.  `prompt_lens` as there.
     `use_graph`: the step is captured once and replayed; `draft` is called for the first step and the captured one alone then and works on the device only.  By
     default where it is `ngram_drafts`."""
     bsz, plen = prompt.shape
@@ -958,7 +966,7 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
         on = length < whole
         tokens, parents = drafted(length, on)
         start = length - 1                                                    # (the last token is not in the cache yet)
-        step_logits = model.tree_step(tokens, cache, start, draft_tree(parents))
+        step_logits = model.tree_step(tokens, cache, start, draft_tree(parents), decode_rule)
         path, count, behind = tree_accept(step_logits, tokens, parents)
         cache_move(caches, start, path, count)
         # the accepted nodes but the root, and the token behind them

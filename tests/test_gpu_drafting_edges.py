@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import ternainfer_amd as T
+from ternainfer_amd.model import ModelArgs, Transformer, speculative_decode
 from tests import _drafting as P
 from tests._long_context import same_or_near
 
@@ -61,3 +62,59 @@ def test_scores_that_overflow(b, t, h, kv, slots):
     parents[:, -1] = -2
     got = T.tree_attention(q, k, v, torch.full((b,), start, device="cuda"), T.draft_tree(parents.cuda()).mask, 2e38).view(b, t, h, 128)
     assert got[:, :-1].isnan().all() and not got[:, -1].any()
+
+
+# ---- the model -----------------------------------------------------------------------------------------------------------------------
+
+
+def _model(**more):
+    """Scales that end at no multiple of 128 columns: 512 columns of three."""
+    return Transformer(ModelArgs(n_layers=2, vocab_size=1000, ffn_dim=384, dim=256, n_heads=4, n_kv_heads=2, **more), seed=31)
+
+
+# How far logits of two ways to the same step may be apart, in deviations of a row of logits.  Where the bfloat16 roundings of the two ways differ, an int8 code in front
+# of a linear may be its neighbour: a unit, a 127th of the row's largest element.  That is 3 times the rms of 256 elements of a normal row and some 10 times that of 384 gated ones
+# (squares times another), so that codes that all move change an output by 3 / 127 = 2.4 % and 8 %.  A code of 30 units is moved by up to 30 * 2^-8 = 0.12 units before it is
+# rounded, so about one in ten changes: 0.1 ** 0.5 of that, 0.8 % and 2.5 %.  Two blocks have six linears of the one kind and two of the other, whose errors are independent: (6 * 0.8 ** 2 +
+# 2 * 2.5 ** 2) ** 0.5 = 4 % a logit, 5.7 % the difference of two.  Four deviations of that are 23 % (one of 16000 is beyond), five of a single logit's 20 % (one of 1.7 million).
+NEAR = 0.25
+
+
+def _tokens(*shape, seed=32):
+    return torch.randint(0, 1000, shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+@torch.inference_mode()
+def test_more_than_64_rows_by_the_decode_rule():
+    """Keys and values of the first block, bit for bit those of the sequences' own steps, of fewer rows."""
+    bsz, t, plen = 4, 30, 17
+    model, prompt, tokens = _model(), _tokens(bsz, plen), _tokens(bsz, t, seed=33)
+    tree, start = T.draft_tree(P.random_parents(bsz, t, 34).cuda()), torch.full((bsz,), plen, device="cuda")
+    cache = model.make_cache(bsz, plen + t)
+    model.forward(prompt, cache, torch.arange(plen, device="cuda"))
+    alone = [tuple(c.clone() for c in pair) for pair in cache]
+    logits = model.tree_step(tokens, cache, start, tree, decode_rule=True)
+    for b in range(bsz):
+        mine = [tuple(c[b:b + 1].contiguous() for c in pair) for pair in alone]
+        own = model.tree_step(tokens[b:b + 1], mine, start[b:b + 1], T.DraftTree(tree.mask[b:b + 1], tree.depth[b:b + 1]))
+        assert all(torch.equal(c[b], m[0]) for c, m in zip(cache[0], mine[0])), b
+        assert (logits[b].float() - own[0].float()).abs().max() <= NEAR * own.float().std()
+
+
+@pytest.mark.parametrize("head8", [False, True])
+def test_speculative_decode_of_more_than_64_rows_against_greedy_steps(head8):
+    """Eight sequences of nine nodes: every token is the likeliest behind the same text of `greedy_decode`'s steps, but for logits nearer to it than the two ways' roundings
+    (by the rule of the scales that more rows follow, they are up to five deviations apart)."""
+    model, count, bsz = _model(), 30, 8
+    if head8:
+        model.quantise_head()
+    prompt = _tokens(bsz, 8, seed=35).repeat(1, 2)
+    got, steps = speculative_decode(model, prompt, count, decode_rule=True)
+    assert got.shape == (bsz, count) and steps < count
+    with torch.inference_mode():
+        cache = model.make_cache(bsz, 16 + count)
+        logits = model.forward(prompt, cache, torch.arange(16, device="cuda"))
+        for i in range(count):
+            rows = logits.float()
+            assert (rows.amax(-1) - rows.gather(1, got[:, i:i + 1])[:, 0] <= NEAR * rows.std(-1)).all(), i
+            logits = model.forward(got[:, i:i + 1].contiguous(), cache, torch.tensor([16 + i], device="cuda"))
