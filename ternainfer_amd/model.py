@@ -783,11 +783,15 @@ class Transformer:
         Ternary linears of more than 64 rows, here B * T, follow the prefill rule of the weights' scales: where a scale's columns do not end at a multiple of 128, columns take
         another scale than in a step of fewer rows.  `decode_rule`: they follow the decode rule whatever the number of rows, as a step of one token does."""
         a = self.args
+        if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= 512 or tokens.shape[0] < 1:
+            raise ValueError("tree_step: tokens [B, T] of trees of 1 to 512 nodes")
         bsz, t = tokens.shape
         if isinstance(cache[0], Kv4Cache) or not self.layers[0].fused or not tokens.is_cuda or a.head_dim not in (64, 128) or a.dim % 8:
             raise ValueError("tree_step: only with a bf16 cache and the fused kernels, on a GPU, heads of 64 or 128 dimensions")
-        if tuple(start.shape) != (bsz,) or tuple(tree.depth.shape) != (bsz, t):
-            raise ValueError("tree_step: one start a sequence, a tree of its tokens")
+        # (all of what the blocks' kernels would refuse: by then they have written keys and values)
+        given = (tokens, (bsz, t)), (start, (bsz,)), (tree.depth, (bsz, t)), (tree.mask, (bsz, t, (t + 63) // 64))
+        if any(x.dtype != torch.int64 or tuple(x.shape) != shape or x.device != cache[0][0].device for x, shape in given) or cache[0][0].shape[0] != bsz:
+            raise ValueError("tree_step: tokens, one start a sequence and the tree of its tokens, int64 on the cache's device")
         max_seq = cache[0][0].shape[2]
         real = (tree.depth >= 0) & (start >= 0)[:, None]
         slots = torch.where(real, start[:, None] + torch.arange(t, device=tokens.device), -1)

@@ -118,3 +118,20 @@ def test_speculative_decode_of_more_than_64_rows_against_greedy_steps(head8):
             rows = logits.float()
             assert (rows.amax(-1) - rows.gather(1, got[:, i:i + 1])[:, 0] <= NEAR * rows.std(-1)).all(), i
             logits = model.forward(got[:, i:i + 1].contiguous(), cache, torch.tensor([16 + i], device="cuda"))
+
+
+@torch.inference_mode()
+def test_what_a_tree_step_refuses_leaves_the_cache_as_it_was():
+    model, tokens = _model(), _tokens(2, 5)
+    tree, start = T.draft_tree(P.random_parents(2, 5, 40).cuda()), torch.tensor([3, 4], device="cuda")
+    cache = model.make_cache(2, 20)
+    wide = tree.mask.expand(2, 5, 2).contiguous()
+    for bad in ((tokens.int(), start, tree), (tokens[0], start, tree), (tokens[:, :0], start, tree), (tokens[:1], start[:1], T.DraftTree(tree.mask[:1], tree.depth[:1])), (tokens, start.int(), tree),
+                (tokens, start.cpu(), tree), (tokens, start[:1], tree), (tokens, start, tree._replace(mask=wide)), (tokens, start, tree._replace(mask=tree.mask.int())),
+                (tokens, start, tree._replace(mask=tree.mask[:, :4])), (tokens, start, tree._replace(mask=tree.mask.cpu())), (tokens, start, tree._replace(depth=tree.depth.int())),
+                (tokens, start, tree._replace(depth=tree.depth[:, :4])), (tokens, start, tree._replace(depth=tree.depth.cpu())), (tokens.repeat(1, 103), start, tree)):
+        with pytest.raises(ValueError, match="tree_step"):
+            model.tree_step(bad[0], cache, *bad[1:])
+        assert not any(c.any() for pair in cache for c in pair)
+    model.tree_step(tokens, cache, start, tree)
+    assert all(c.any() for pair in cache for c in pair)
