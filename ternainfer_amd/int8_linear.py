@@ -30,10 +30,11 @@ def quantise_rows(x: torch.Tensor) -> Int8Rows:
 
 def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     """Rows that are integers already: q int8 [R, K], scale float32 [R]."""
-    packed = _lib.native().int8_pack(q)
+    if not isinstance(q, torch.Tensor) or not isinstance(scale, torch.Tensor):
+        raise TypeError("int8_rows: rows and scales are tensors")
     if scale.dtype != torch.float32 or scale.shape != q.shape[:1] or scale.device != q.device:
         raise ValueError("int8_rows: scale is float32 [R] beside the rows")
-    return Int8Rows(packed, scale.contiguous(), *q.shape)
+    return Int8Rows(_lib.native().int8_pack(q), scale.contiguous(), *q.shape)
 
 
 def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

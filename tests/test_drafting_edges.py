@@ -1,0 +1,21 @@
+"""What ternainfer_amd/drafting.py, int8_linear.py and the model's drafts do at the edges of their documentation, where no GPU is needed."""
+import pytest
+import torch
+
+import ternainfer_amd as T
+from ternainfer_amd import _lib
+
+
+def test_scales_are_looked_at_before_rows_are_packed(monkeypatch):
+    """TypeError where an argument is no tensor, ValueError for scales that do not belong to the rows; nothing is enqueued by then."""
+    def enqueued(*_):
+        raise AssertionError("enqueued")
+
+    monkeypatch.setattr(_lib, "native", lambda: type("Native", (), {"int8_pack": staticmethod(enqueued)}))
+    rows, scale = torch.zeros((2, 3), dtype=torch.int8), torch.zeros(2)
+    for q, s in ((rows, [0.0, 0.0]), (rows, None), ([[1]], scale), (rows, 1.0)):
+        with pytest.raises(TypeError, match="int8_rows"):
+            T.int8_rows(q, s)
+    for s in (scale.double(), torch.zeros(3), torch.zeros((2, 1)), torch.zeros(2, device="meta")):
+        with pytest.raises(ValueError, match="int8_rows"):
+            T.int8_rows(rows, s)
