@@ -760,12 +760,12 @@ class Transformer:
         """Logits of the rows x (+ pending): last residual add, final norm, LM head."""
         return self.project(self.final_norm(x, pending), bsz)
 
-    def project(self, x, bsz):
-        """Logits of normed rows."""
+    def project(self, x, bsz=None):
+        """Logits of normed rows: those of a step of bsz rows, or (None) rows of a text, by one matrix product whatever their number."""
         a = self.args
         if self.head8 is not None:
             return int8_linear(x, self.head8)
-        if x.is_cuda and bsz <= 16 and a.dim % 32 == 0 and bsz * (2 * a.dim + 16) <= 160 * 1024:
+        if x.is_cuda and bsz is not None and bsz <= 16 and a.dim % 32 == 0 and bsz * (2 * a.dim + 16) <= 160 * 1024:
             return lm_head(x, self.tok_embeddings)                            # tied LM head (model.py:367): one HBM-bound pass
         return F.linear(x, self.tok_embeddings)
 
@@ -821,7 +821,7 @@ class Transformer:
         if lens is not None:
             targets = targets.masked_fill(torch.arange(1, t, device=dev) >= lens.to(dev)[:, None], -1)
         targets, h = targets.view(-1), self.final_norm(x, pending)
-        parts = [token_logprobs(self.project(h[i:i + self.score_rows], self.score_rows), targets[i:i + self.score_rows], top)
+        parts = [token_logprobs(self.project(h[i:i + self.score_rows]), targets[i:i + self.score_rows], top)
                  for i in range(0, h.shape[0], self.score_rows)]
         join = lambda field: None if field[0] is None else torch.cat(field).view(bsz, t - 1, *field[0].shape[1:])
         return TokenLogprobs(*map(join, zip(*parts)))

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import ternainfer_amd as T
+import ternainfer_amd.model as model_module
 from ternainfer_amd.model import ModelArgs, Transformer, speculative_decode
 from tests import _drafting as P
 from tests._long_context import same_or_near
@@ -135,3 +136,14 @@ def test_what_a_tree_step_refuses_leaves_the_cache_as_it_was():
         assert not any(c.any() for pair in cache for c in pair)
     model.tree_step(tokens, cache, start, tree)
     assert all(c.any() for pair in cache for c in pair)
+
+
+def test_scores_a_few_rows_at_a_time(monkeypatch):
+    """Rows of a text are projected by the matrix product of many rows, however few `score_rows` are."""
+    model, tokens = _model(), _tokens(2, 20)
+    monkeypatch.setattr(model_module, "lm_head", None)
+    rows, plain = [], model_module.F.linear
+    monkeypatch.setattr(model_module.F, "linear", lambda x, w: rows.append(x.shape[0]) or plain(x, w))
+    for model.score_rows in (3, 16, 1024):
+        assert model.score(tokens).logprob.shape == (2, 19)
+    assert rows == [3] * 12 + [2] + [16, 16, 6] + [38]
