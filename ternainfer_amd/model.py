@@ -902,7 +902,10 @@ def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use
         if ragged:
             pos.add_(1)
 
+    # A captured step reads the rotary table where it was: kept here, for the model keeps the last length's alone (a decode of another one, on another thread, replaces it).
+    rotary = None if kv_bits == 4 else model.rope_tables(plen + gen_tokens, tok.device)
     seconds = _greedy_steps(step, gen_tokens, use_graph)
+    del rotary
     result = out, ev[0].elapsed_time(ev[1]) * 1e-3, seconds
     return result if history is None else (*result, TokenLogprobs(*[None if f is None else f[:, :gen_tokens] for f in history]))
 
@@ -983,6 +986,7 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
         left.copy_((length < whole).any())
 
     steps, again, captured = 0, step, draft is ngram_drafts if use_graph is None else use_graph
+    rotary = model.rope_tables(cache[0][0].shape[2], dev)                     # (kept for the captured step, as in greedy_decode)
     left.copy_((length < whole).any())
     while bool(left):
         if captured and steps == 1:
@@ -992,4 +996,5 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
             again = graph.replay
         again()
         steps += 1
+    del rotary
     return text.gather(1, lens[:, None] + torch.arange(gen_tokens, device=dev)), steps

@@ -4,7 +4,7 @@ import torch
 
 import ternainfer_amd as T
 import ternainfer_amd.model as model_module
-from ternainfer_amd.model import ModelArgs, Transformer, speculative_decode
+from ternainfer_amd.model import ModelArgs, Transformer, greedy_decode, speculative_decode
 from tests import _drafting as P
 from tests._long_context import same_or_near
 
@@ -147,3 +147,21 @@ def test_scores_a_few_rows_at_a_time(monkeypatch):
     for model.score_rows in (3, 16, 1024):
         assert model.score(tokens).logprob.shape == (2, 19)
     assert rows == [3] * 12 + [2] + [16, 16, 6] + [38]
+
+
+@pytest.mark.parametrize("decode", [speculative_decode, greedy_decode])
+@pytest.mark.parametrize("scaling", [None, {"type": "linear", "factor": 2.0}])
+def test_a_decode_of_another_length_between_replays(decode, scaling, monkeypatch):
+    """A captured step keeps its rotary table while other lengths are decoded with the same model: the same tokens."""
+    model, prompt = _model(rope_scaling=scaling), _tokens(2, 8, seed=50).repeat(1, 2)
+    want, replay, kept, replays = decode(model, prompt, 20)[0], torch.cuda.CUDAGraph.replay, [], []
+
+    def disturbed(graph):
+        replays.append(0)
+        model.rope_tables(50 + len(replays), prompt.device)
+        kept.extend(torch.full((36 + 9 * (decode is speculative_decode), 2, 32), float("nan"), device="cuda") for _ in range(8))      # where a table that was let go of may lie
+        replay(graph)
+
+    monkeypatch.setattr(torch.cuda.CUDAGraph, "replay", disturbed)
+    got = decode(model, prompt, 20)[0]
+    assert len(replays) > 3 and torch.equal(got, want)
