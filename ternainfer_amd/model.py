@@ -947,6 +947,9 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
     dev = prompt.device
     if gen_tokens < 1:
         return prompt.new_empty((bsz, 0)), 0
+    if prompt.is_cuda and dev.index != torch.cuda.current_device():           # (a step is captured on the current device's streams)
+        with torch.cuda.device(dev):
+            return speculative_decode(model, prompt, gen_tokens, draft, prompt_lens, use_graph, decode_rule)
     if prompt.dtype != torch.int64 or plen < 1 or (prompt_lens is not None and (tuple(prompt_lens.shape) != (bsz,) or not bool(((prompt_lens >= 1) & (prompt_lens <= plen)).all()))):
         raise ValueError(f"speculative_decode: prompts are int64 [B, P], their lengths [B], each 1 .. P = {plen}")
     lens = torch.full((bsz,), plen, dtype=torch.int64, device=dev) if prompt_lens is None else prompt_lens.to(device=dev, dtype=torch.int64)
@@ -991,7 +994,7 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
     while bool(left):
         if captured and steps == 1:
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream(dev)):      # (torch's own stream for this is that of the first device that captured)
                 step()
             again = graph.replay
         again()
