@@ -1362,9 +1362,9 @@ TERNA_FUNCTION(cache_move, 4)
         const at::Tensor& c = tensor(PySequence_Fast_GET_ITEM(a[0], i));
         if (c.dim() != 4 || c.size(0) != b || c.size(1) > 65535 || c.size(2) > INT32_MAX || c.size(3) > 1 << 20) refuse("%s: a cache is [B, heads, S, D] with the path's B", who);
         check_device(who, "a cache", c, path);
-        if (c.numel() != 0 && !c.is_contiguous() && ((c.size(3) > 1 && c.stride(3) != 1) || overlaps_itself(c) || c.stride(2) < c.size(3))) refuse("%s: a cache's rows are contiguous and apart from each other", who);
+        const bool empty = c.numel() == 0 || c.size(2) == 1;               // (of one slot nothing moves, whatever its stride)
+        if (!empty && !c.is_contiguous() && ((c.size(3) > 1 && c.stride(3) != 1) || overlaps_itself(c) || c.stride(2) < c.size(3))) refuse("%s: a cache's rows are contiguous and apart from each other", who);
         const long long size = c.element_size();
-        const bool empty = c.numel() == 0;
         caches[i] = ternaspmm_cache_rows{empty ? nullptr : c.mutable_data_ptr(), c.stride(0) * size, c.stride(1) * size, c.stride(2) * size, static_cast<int>(c.size(1)),
                                          static_cast<int>(c.size(2)), static_cast<int>(c.size(3) * size)};
     }

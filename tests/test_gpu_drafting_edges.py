@@ -65,6 +65,20 @@ def test_scores_that_overflow(b, t, h, kv, slots):
     assert got[:, :-1].isnan().all() and not got[:, -1].any()
 
 
+# ---- moving rows -------------------------------------------------------------------------------------------------------------------
+
+
+def test_caches_of_one_slot_stay():
+    """Nothing moves in them; a stride between slots that are not there says nothing."""
+    start, path, count = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.tensor([[0, 2], [1, 3]], device="cuda"), torch.tensor([2, 2], device="cuda")
+    one = torch.randn(2 * 3 * 16, device="cuda").as_strided((2, 3, 1, 16), (48, 16, 1, 1))
+    more, was = _randn((2, 3, 5, 16), 60), _randn((2, 3, 5, 16), 60)
+    before = one.clone()
+    T.cache_move([one, more], start, path, count)
+    was[0, :, 1], was[1, :, 0], was[1, :, 1] = was[0, :, 2].clone(), was[1, :, 1].clone(), was[1, :, 3].clone()
+    assert torch.equal(one, before) and torch.equal(more, was)
+
+
 # ---- the model -----------------------------------------------------------------------------------------------------------------------
 
 
