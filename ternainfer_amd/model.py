@@ -913,23 +913,30 @@ def greedy_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int, use
 def ngram_drafts(text: torch.Tensor, length: torch.Tensor, branches: int = 2, depth: int = 4):
     """Drafts by looking the text up in itself: where its last two tokens stood before -- the latest `branches` places -- what followed there, `depth` tokens
     each.  text int64 [B, L], `length` int64 [B] tokens of it that count.  Returns (tokens, parents) int64 [B, 1 + branches * depth]: the last token and, behind it, a
-    branch for every place; parents of -2 (padding) where there is none, or where the text ends.  On the device alone: it can be captured."""
+    branch for every place; branches that begin alike share the nodes of the first of them.  Parents of -2 (padding) where there is none, where the text ends, and for what is
+    shared.  On the device alone: it can be captured."""
     bsz, cap = text.shape
     dev = text.device
     last = length[:, None] - 1
-    root, before = text.gather(1, last.clamp(min=0)), text.gather(1, (last - 1).clamp(min=0))
-    at = torch.arange(cap, device=dev)
-    match = (text == root) & (torch.cat([text[:, :1] - text[:, :1] - 1, text[:, :-1]], 1) == before) & (at < last) & (last >= 2)
-    places = torch.topk(torch.where(match, at, -1), min(branches, cap), 1).values                            # latest first
-    places = torch.cat([places, places.new_full((bsz, branches - places.shape[1]), -1)], 1)
-    ahead = places[:, :, None] + 1 + torch.arange(depth, device=dev)                                         # [B, branches, depth]
+    root, head = text.gather(1, last.clamp(min=0)), torch.where(length[:, None] > 0, -1, -2)
+    if branches * depth == 0:
+        return root, head
+    before = text.gather(1, (last - 1).clamp(min=0))
+    at = torch.arange(1, cap, device=dev)
+    match = (text[:, 1:] == root) & (text[:, :-1] == before) & (at < last)
+    places = torch.topk(torch.where(match, at, -1), min(branches, max(cap - 1, 0)), 1).values                # latest first
+    if places.shape[1] < branches:
+        places = torch.cat([places, places.new_full((bsz, branches - places.shape[1]), -1)], 1)
+    step, branch = torch.arange(depth, device=dev), torch.arange(branches, device=dev)[:, None]
+    ahead = places[:, :, None] + 1 + step                                                                    # [B, branches, depth]
     real = (places >= 0)[:, :, None] & (ahead <= last[:, :, None])
-    tokens = torch.where(real, text.gather(1, ahead.clamp(0, cap - 1).view(bsz, -1)).view_as(ahead), 0)
-    node = 1 + torch.arange(branches * depth, device=dev).view(branches, depth)
-    parents = torch.where(torch.arange(depth, device=dev) == 0, 0, node - 1)
-    parents = torch.where(real, parents, -2)
-    head = torch.where(length[:, None] > 0, -1, -2)
-    return torch.cat([root, tokens.view(bsz, -1)], 1), torch.cat([head, parents.view(bsz, -1)], 1)
+    says = torch.where(real, text.gather(1, ahead.clamp(max=cap - 1).view(bsz, -1)).view_as(ahead), -1)
+    # of every node, the first branch that says the same up to it: [B, branches, those, depth, step] -> [B, branches, depth]
+    alike = ((says[:, :, None] == says[:, None])[..., None, :] | (step[:, None] < step)).all(-1)
+    first = torch.where(alike, branch, branches).amin(2)
+    above = torch.cat([first.new_zeros((bsz, branches, 1)), torch.add(step[1:], first[..., :-1], alpha=depth)], 2)
+    parents = torch.where(real & (first == branch), above, -2)
+    return torch.cat([root, says.clamp(min=0).view(bsz, -1)], 1), torch.cat([head, parents.view(bsz, -1)], 1)
 
 
 @torch.inference_mode()

@@ -6,7 +6,8 @@ import torch
 
 import ternainfer_amd as T
 from ternainfer_amd import _lib
-from ternainfer_amd.model import speculative_decode
+from ternainfer_amd.model import ngram_drafts, speculative_decode
+from tests import _drafting as P
 
 
 def test_scales_are_looked_at_before_rows_are_packed(monkeypatch):
@@ -45,3 +46,35 @@ def test_decoding_goes_by_the_prompts_device(monkeypatch):
     with pytest.raises(ValueError, match="speculative_decode"):                          # (refused there: int32)
         speculative_decode(None, prompt, 5)
     assert entered == [1] and current == [0]
+
+
+def _branches(text, branches, depth):
+    """What followed the last two tokens of a text (a list) at the latest places where they stood before."""
+    places = [i for i in range(len(text) - 2, 0, -1) if text[i - 1:i + 1] == text[-2:]][:branches]
+    return [text[i + 1:i + 1 + depth] for i in places]
+
+
+@pytest.mark.parametrize("branches,depth", [(1, 1), (2, 4), (3, 7), (5, 2), (0, 3), (3, 0)])
+@pytest.mark.parametrize("kinds", [1, 2, 5, 40])
+def test_drafts_that_begin_alike_share_their_nodes(branches, depth, kinds):
+    """The lines of the tree are the beginnings of the branches, each of them once, so that none hides what continues another."""
+    gen = torch.Generator().manual_seed(10 * branches + kinds)
+    text = torch.randint(0, kinds, (60, 30), generator=gen)
+    text[40:] = torch.randint(0, kinds, (20, 4), generator=gen).repeat(1, 8)[:, :30]     # periodic ones
+    length = torch.randint(1, 31, (60,), generator=gen)
+    tokens, parents = ngram_drafts(text, length, branches, depth)
+    assert tokens.shape == parents.shape == (60, 1 + branches * depth) and tokens.dtype == parents.dtype == torch.int64 and tokens.min() >= 0
+    for row, n, says, of in zip(text.tolist(), length.tolist(), tokens.tolist(), parents.tolist()):
+        assert says[0] == row[n - 1] and of[0] == -1
+        got = sorted([says[i] for i in line[1:]] for line in P.lines(of) if line)
+        want = {tuple(b[:j]) for b in _branches(row[:n], branches, depth) for j in range(len(b) + 1)} | {()}
+        assert got == sorted(map(list, want))
+
+
+def test_drafts_of_periodic_texts_are_accepted():
+    """A model that goes on with the period accepts two drafts of 20 equal tokens (the places end with the text) and four of a period of two."""
+    for text, steps in (([7] * 20, 2), ([1, 2] * 10, 4)):
+        tokens, parents = ngram_drafts(torch.tensor([text]), torch.tensor([20]))
+        follows = torch.nn.functional.one_hot(torch.tensor([[{7: 7, 1: 2, 2: 1, 0: 0}[t] for t in tokens[0].tolist()]]), 8)
+        _, count, behind = P.accept(follows, tokens, parents)
+        assert count == [1 + steps] and behind == [(text + text)[20 + steps]]
