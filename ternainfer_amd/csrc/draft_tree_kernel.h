@@ -9,8 +9,7 @@
 
 namespace terna {
 
-constexpr int kTreeMaxNodes = 512, kTreeMaxWords = kTreeMaxNodes / 64;
-constexpr int kTreeThreads = 256, kTreeEach = kTreeMaxNodes / kTreeThreads;      // nodes of a thread
+constexpr int kTreeMaxNodes = 512, kTreeThreads = 256;
 
 // One workgroup a sequence.  Ancestors by doubling: a node takes over what the node that it points at has seen, and points where that one points;
 // nine rounds for the longest chain of 512, where walking it node by node is 512 reads of LDS one after the other.  16 nodes 2.5 us, 64 sequences of 512 10.6.
@@ -195,7 +194,7 @@ struct MoveCaches {
 };
 
 template <typename P>
-__device__ __forceinline__ void move_column(uint8_t* column, long long slot_bytes, long long start, const int* line, int n, int slots)
+__device__ __forceinline__ void move_column(uint8_t* column, long long slot_bytes, long long start, const int* line, int n)
 {
     for (int i0 = 0; i0 < n; i0 += kMoveAhead) {
         P x[kMoveAhead];
@@ -227,11 +226,11 @@ __global__ __launch_bounds__(kTreeThreads) void terna_cache_move_kernel(MoveCach
         const int head = x / c.pieces, piece = x - head * c.pieces;
         uint8_t* const column = c.rows + b * c.sequence + head * c.head + (static_cast<long long>(piece) << c.piece_shift);
         switch (c.piece_shift) {
-        case 4: move_column<u32x4>(column, c.slot, start, line, n, c.slots); break;
-        case 3: move_column<u32x2>(column, c.slot, start, line, n, c.slots); break;
-        case 2: move_column<uint32_t>(column, c.slot, start, line, n, c.slots); break;
-        case 1: move_column<uint16_t>(column, c.slot, start, line, n, c.slots); break;
-        default: move_column<uint8_t>(column, c.slot, start, line, n, c.slots); break;
+        case 4: move_column<u32x4>(column, c.slot, start, line, n); break;
+        case 3: move_column<u32x2>(column, c.slot, start, line, n); break;
+        case 2: move_column<uint32_t>(column, c.slot, start, line, n); break;
+        case 1: move_column<uint16_t>(column, c.slot, start, line, n); break;
+        default: move_column<uint8_t>(column, c.slot, start, line, n); break;
         }
     }
 }

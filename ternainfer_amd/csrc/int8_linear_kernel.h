@@ -259,7 +259,7 @@ __device__ __forceinline__ void int8_finish(const Int8Linear& a, const Int8Place
 }
 
 template <typename Out, int WN, int WM, int NA, int MB, int SK, int ST>
-__global__ __launch_bounds__(256, (NA * MB > 8 ? 1 : 2)) void terna_int8_linear_kernel(Int8Linear a)
+__global__ __launch_bounds__(256, 2) void terna_int8_linear_kernel(Int8Linear a)
 {
     using Tile = Int8Tile<WN, WM, NA, MB, SK, ST>;
     constexpr int BN = Tile::BN, BM = Tile::BM, LOADS = Tile::kLoads;
