@@ -17,10 +17,10 @@ struct TreePlan {
 };
 // The groups and the parts by the time they take, us: steps of a workgroup and what surrounds them, in rounds of the workgroups that there is room for, or the
 // cache's bytes -- at 5.8 TB/s, less where workgroups are fewer than the CUs or do not fill their last round --, and the launch that joins the parts, whose
-// numerators are written and read at 5.4 to 5.9.  Fitted to 250 measured shapes and numbers of parts of up to 64 rows (an error of 12 %) and 750 of more (16 % over 1100; the
-// plan chosen by it took 1.7 % longer than the best one in the mean of 62 shapes, 16 % at the worst).  128 rows in two groups are a workgroup of eight waves, one to a CU, with half
-// the numerators that two workgroups of four have: 240 rows over 32768 slots 41 us, with one group 45; where nothing is split and workgroups are many,
-// those of one group start and end while others compute: 32 sequences of 256 rows over 2048 slots 81 us, with two groups 91.
+// numerators are written and read at 5.4 to 5.9.  Fitted to 250 measured shapes and numbers of parts of up to 64 rows (an error of 12 %) and 555 of more (11 %; the
+// plan chosen by it took 1.3 % longer than the best one in the mean of 30 shapes, 10 % at the worst; one group alone 3.8 % in the mean, two 4.4).  128 rows in two groups are a
+// workgroup of eight waves, one to a CU, with half the numerators that two workgroups of four have: 240 rows over 32768 slots 47 us, with one group 50; where workgroups are many,
+// those of one group start and end while others compute: 33 sequences of 720 rows over 399 slots 103 us, with two groups 128.
 inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
 {
     const long long rows = static_cast<long long>(T) * (H / KV), heads = static_cast<long long>(B) * KV, tiles = (S + kTreeTile - 1) / kTreeTile;
@@ -35,14 +35,14 @@ inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
         float step, around = 8.0f;
         if (p.rows == 32) step = 0.97f;
         else if (p.rows == 64) step = 1.03f;
-        else if (groups == 2) step = 0.97f, around = 6.7f;
-        else if (places == 256.0f) step = 0.64f, around = 7.3f;
-        else step = 1.02f, around = 3.5f;
-        if (D == 64) step *= p.rows == 128 ? 0.52f : 0.67f;
+        else if (groups == 2) step = 1.09f, around = 7.5f;
+        else if (places == 256.0f) step = 0.72f, around = 7.7f;
+        else step = 1.31f, around = 3.3f;
+        if (D == 64) step *= p.rows == 128 ? 0.66f : 0.67f;
         const float full = std::max(1.0f, wgs / places), whole = std::ceil(full), rounds = full > 3.0f ? full : p.rows == 128 ? whole : 0.5f * (full + whole);
         const float memory = cache * std::pow(std::max(1.0f, 0.9f * places * whole / wgs), 0.6f);
         return std::max(rounds * (around + steps * step), memory + 8.0f) +
-               (n == 1 ? 0.0f : (p.rows == 128 ? 7.1f : 4.0f) + static_cast<float>(rows * heads) * static_cast<float>(8 * D * n) * (p.rows == 128 ? 0.185e-6f : 0.171e-6f));
+               (n == 1 ? 0.0f : (p.rows == 128 ? 6.6f : 4.0f) + static_cast<float>(rows * heads) * static_cast<float>(8 * D * n) * (p.rows == 128 ? 0.193e-6f : 0.171e-6f));
     };
     const int least = 128 / p.rows, widest = std::max(least, 2);
     p.groups = least, p.splits = 1;
