@@ -180,9 +180,9 @@ class Block:
         blk.attn_sub_norm, blk.ffn_sub_norm = norm("attention.attn_sub_norm"), norm("feed_forward.ffn_sub_norm")
         return blk
 
-    def _norm_linear(self, lin, x, weight, residual=None, glu=False, name=None, decode_rule=False):
+    def _norm_linear(self, lin, x, weight, residual=None, glu=False, name=None, **how):
         """[x + residual | relu(x1)^2 * x3] -> RMSNorm -> lin.  Returns (lin output, x + residual).  With `capture` set the
-        quantised activations go through memory (norm kernel + linear, never the one-launch form) and are recorded."""
+        quantised activations go through memory (norm kernel + linear, never the one-launch form) and are recorded.  `how`: of TernaryLinear.quantised."""
         eps = self.args.norm_eps
         if not self.fused:
             if glu:
@@ -197,7 +197,7 @@ class Block:
                 if x.shape[0] <= 4 and cap is None:
                     return relu2_mul_rmsnorm_linear_packed(x, weight, eps, lin.packed, lin.ws, lin.ws_num, lin.n), None
                 xq, s = relu2_mul_rmsnorm_quant(x, weight, eps)
-                out = lin.quantised(xq, s, decode_rule)
+                out = lin.quantised(xq, s, **how)
                 if cap is not None:
                     cap.append((name, xq, s, out))
                 return out, None
@@ -206,7 +206,7 @@ class Block:
             if x.shape[0] <= 8 and cap is None:   # decode step: prologue and linear in one launch where that is faster
                 return rmsnorm_linear_packed(x, weight, eps, lin.packed, lin.ws, lin.ws_num, lin.n, residual=residual)
             xq, s, h = rmsnorm_quant(x, weight, eps, residual=residual)
-            out = lin.quantised(xq, s, decode_rule)
+            out = lin.quantised(xq, s, **how)
             if cap is not None:
                 cap.append((name, xq, s, out))
             return out, h
@@ -382,8 +382,8 @@ class Block:
                 self.ffn_sub_norm, wqkv.packed, wqkv.ws, wqkv.ws_num, wqkv.n, wo.packed, wo.ws, wo.ws_num, wo.n, w13.packed, w13.ws, w13.ws_num, w13.n,
                 w2.packed, w2.ws, w2.ws_num, w2.n,
                 self.gate_up_interleaved() if self.gate_linear_reads(x.shape[0]) else None)
-        rule = isinstance(mask, TreeNodes) and mask.decode_rule
-        qkv, x = self._norm_linear(self.wqkv, x, self.attention_norm, residual=pending, name="wqkv", decode_rule=rule)
+        how = {"decode_rule": True} if isinstance(mask, TreeNodes) and mask.decode_rule else {}
+        qkv, x = self._norm_linear(self.wqkv, x, self.attention_norm, residual=pending, name="wqkv", **how)
         rep = a.n_heads // a.n_kv_heads
         native = _lib.native()
         attend = (qkv, cos, sin, pos_idx, cache_k, cache_v, a.n_heads, a.head_dim, a.head_dim ** -0.5, int(a.rope_adjacent))
@@ -444,9 +444,9 @@ class Block:
         else:
             if self.capture is not None:
                 self.capture.append(("attention", None, None, o))
-            attn, _ = self._norm_linear(self.wo, o.contiguous(), self.attn_sub_norm, name="wo", decode_rule=rule)
-        x13, x = self._norm_linear(self.w13, x, self.ffn_norm, residual=attn, name="w13", decode_rule=rule)
-        ffn, _ = self._norm_linear(self.w2, x13, self.ffn_sub_norm, glu=True, name="w2", decode_rule=rule)
+            attn, _ = self._norm_linear(self.wo, o.contiguous(), self.attn_sub_norm, name="wo", **how)
+        x13, x = self._norm_linear(self.w13, x, self.ffn_norm, residual=attn, name="w13", **how)
+        ffn, _ = self._norm_linear(self.w2, x13, self.ffn_sub_norm, glu=True, name="w2", **how)
         return x, ffn
 
 
@@ -963,7 +963,7 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
     room = torch.cat([prompt, prompt.new_zeros((bsz, gen_tokens + 1))], 1)    # (a last column for what is not kept)
     text = room[:, :-1]
     text[torch.arange(plen + gen_tokens, device=dev) >= lens[:, None]] = 0
-    whole, widest = lens + gen_tokens, 512
+    whole, widest, how = lens + gen_tokens, 512, {"decode_rule": True} if decode_rule else {}
 
     def drafted(length, on):
         tokens, parents = draft(text, length)
@@ -983,7 +983,7 @@ def speculative_decode(model: Transformer, prompt: torch.Tensor, gen_tokens: int
         on = length < whole
         tokens, parents = drafted(length, on)
         start = length - 1                                                    # (the last token is not in the cache yet)
-        step_logits = model.tree_step(tokens, cache, start, draft_tree(parents), decode_rule)
+        step_logits = model.tree_step(tokens, cache, start, draft_tree(parents), **how)
         path, count, behind = tree_accept(step_logits, tokens, parents)
         cache_move(caches, start, path, count)
         # the accepted nodes but the root, and the token behind them

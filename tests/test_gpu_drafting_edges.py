@@ -179,3 +179,33 @@ def test_a_decode_of_another_length_between_replays(decode, scaling, monkeypatch
     monkeypatch.setattr(torch.cuda.CUDAGraph, "replay", disturbed)
     got = decode(model, prompt, 20)[0]
     assert len(replays) > 3 and torch.equal(got, want)
+
+
+@torch.inference_mode()
+def test_blocks_and_linears_that_know_no_rule():
+    """A prompt and a step over trees through blocks and linears of a caller's own, which take what they took before there was a rule to choose."""
+    model, tokens = _model(), _tokens(2, 9)
+    calls = []
+
+    class Linear:
+        def __init__(self, of):
+            self.__dict__.update(of.__dict__)
+            self.of = of
+
+        def quantised(self, xq, s):
+            calls.append(xq.shape[0])
+            return self.of.quantised(xq, s)
+
+    class Own(model_module.Block):
+        def _norm_linear(self, lin, x, weight, residual=None, glu=False, name=None):
+            return super()._norm_linear(lin, x, weight, residual, glu, name)
+
+    tree, start = T.draft_tree(P.random_parents(2, 9, 70).cuda()), torch.tensor([0, 0], device="cuda")
+    want = model.tree_step(tokens, model.make_cache(2, 12), start, tree)
+    for blk in model.layers:
+        blk.__class__ = Own
+        blk.w2 = Linear(blk.w2)
+    assert torch.equal(model.tree_step(tokens, model.make_cache(2, 12), start, tree), want) and calls == [18, 18]
+    plain = model.tree_step
+    model.tree_step = lambda tokens, cache, start, tree: plain(tokens, cache, start, tree)
+    assert speculative_decode(model, tokens, 5)[0].shape == (2, 5)
