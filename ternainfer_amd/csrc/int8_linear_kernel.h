@@ -7,9 +7,10 @@
 //
 // What bounds the product: of few rows the weights' bytes (a vocabulary of 128256 by 2560 and one row 58 us, 5.7 TB/s; a library's product in bf16 119), of many
 // the matrix instructions, whose pipes are busy half of the clocks at 1.9 GHz (8192 x 8192 x 8192 460 us, 2390 Tera-operations a second, a library's own product in
-// 8-bit integers 480 to 500; 4096 x 13824 x 2560 147 us, 1980, of whose tiles the last round is a third full).  Between them it is what a CU can fetch: a stage of a
-// 64 x 64 tile is 16 KB for 0.18 us (333 x 2501 x 6912, 240 workgroups: 14.8 us; a second group of four waves for half of a stage's columns changes nothing there,
-// nor do two parts with a launch that joins them, 19.6).
+// 8-bit integers 480 to 500; 4096 x 13824 x 2560 147 us, 1980, of whose tiles the last round is a third full).  Between them it is a CU's reads: a stage of a
+// 64 x 64 tile is 16 KB for 0.18 us with four stages under way -- 40 bytes a clock, or a read's 0.7 us: not told apart (333 x 2501 x 6912, 240 workgroups: 14.4 to 14.8 us
+// replayed, 15.3 and more under a profiler; a second group of four waves for half of a stage's columns changes nothing there, nor do two parts with a launch that joins
+// them, 19.6).
 #pragma once
 
 #include "int8_plan.h"

@@ -10,16 +10,16 @@
 //     and many leave few numerators to join.  The groups' are joined in LDS at the end, the splits' by a second launch (which groups, how many splits: tree_plan.h).
 //   * Keys and values go global -> LDS directly, ST - 1 steps ahead; 16-byte pieces are XOR-swizzled on the way, so that neither the keys' 16-byte operand reads
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
-//     With 128 rows a workgroup the next step's keys are read ahead of this one's exponentials (800 rows over 8300 slots 65 us, so 63.6).
+//     With 128 rows a workgroup the next step's keys are read ahead of this one's exponentials (measured with probabilities in one bf16: 800 rows over 8300 slots 65.2 us, so 63.6; now 76).
 //   * Probabilities are two bf16, high and low part: 15 bits of them count.  One bf16 is 2^-9 of every term, which shows where large values nearly cancel: two slots
-//     with half of the weight each and values of 200 and -200 came out 0.3 off.
+//     with half of the weight each and values of 200 and -200 came out 0.3 off, for 10 % less time with more than 64 rows a kv head (60 nodes of 4 heads over 32001 slots 40.0 us, so 43.3 to 44.1).
 //     The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own.
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
 // What bounds it: of few rows a sequence and many sequences the cache's bytes (64 sequences of one token over 8000 slots 229 us, 5.7 TB/s; 32 of 13 nodes over
-// 7500 119 us, 4.9), of many rows the steps -- 64 slots of 128 rows in two groups: 1024 clocks of a SIMD's matrix instructions, as many of its vector
-// instructions, 128 KB of LDS reads; 0.85 us where nothing comes from memory, 1.23 where all does, of which two workgroups that share their slots need 0.9 for the
-// memory alone -- and with little to read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 5 for the
+// 7500 119 us, 4.9), of many rows the steps -- 64 slots of 128 rows in two groups: 1536 clocks of a SIMD's matrix instructions, 1450 of its vector
+// instructions, 128 KB of LDS reads; 1.0 to 1.15 us where nothing comes from memory, 1.5 to 1.6 where all does, of which two workgroups that share their slots need 0.9 for
+// the memory alone -- and with little to read what surrounds the steps: 3 us until the first tile is there, 3.5 for the join in LDS and the rows' way out, 4 to 5 for the
 // second launch.
 #pragma once
 

@@ -56,7 +56,7 @@ inline TreePlan tree_plan(int B, int T, int H, int KV, int D, int S)
 
 // Where a workgroup works: on which part of a kv head (unit; -1: nowhere), on which of its row tiles.  Workgroups go to the XCDs round robin: the tiles of a unit, which
 // read the same slots, are on one XCD, eight units on eight, and those of the last units, fewer than eight, on all in equal shares (20 units of 12 tiles: 36 on four of
-// the XCDs and 24 on the others 58 us, 30 on each 39).
+// the XCDs and 24 on the others 58 us, 30 on each 39, both with probabilities in one bf16; in two 45).
 struct TreePlace {
     int unit, tile;
 };
