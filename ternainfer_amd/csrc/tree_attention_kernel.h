@@ -12,7 +12,7 @@
 //     nor the values' transposing ones conflict.  A wave that shares its slots with nobody waits for its own requests only.
 //     With 128 rows a workgroup the next step's keys are read ahead of this one's exponentials (measured with probabilities in one bf16: 800 rows over 8300 slots 65.2 us, so 63.6; now 76).
 //   * Probabilities are two bf16, high and low part: 15 bits of them count.  One bf16 is 2^-9 of every term, which shows where large values nearly cancel: two slots
-//     with half of the weight each and values of 200 and -200 came out 0.3 off, for 10 % less time with more than 64 rows a kv head (60 nodes of 4 heads over 32001 slots 40.0 us, so 43.3 to 44.1).
+//     with half of the weight each and values of 200 and -200 came out 0.3 off, for 10 % less time with more than 64 rows a kv head (60 nodes of 4 heads over 32001 slots 40.0 us, so 43.3 to 45.4).
 //     The running maximum is raised, and the output rescaled, only where it grows by more than 2^3 -- a row's own.
 //   * Only the last tiles have slots of the tree.  There the mask's bits select the scores, and values that are not finite are taken out -- a slot that
 //     one node sees and another does not must not reach the other through 0 * NaN; the rows that do see them get them back at the end.
